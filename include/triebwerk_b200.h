@@ -401,6 +401,64 @@ int tq_engine_decode_step_host(tq_engine* e, const void* q_host, const void* k_h
                                void* out_host, tq_stream_t s);
 
 /* ===================================================================================================================
+ * 3. Paged packed caches.  No counterpart in the reference, whose sequences own max_seq_len rows each.
+ *
+ * A cache array is that of the calls above (codes [rows][kv_dim / codes per byte], norms [rows][num_kv_heads]), cut into num_pages
+ * pages of page_size consecutive rows; page_size is a power of two from 32 to 65536.  Row g of a block table (int32, device,
+ * [G][table_width], rows table_stride elements apart) names the pages of request g in order: its token t is row
+ * block_table[g][t / page_size] * page_size + t % page_size.  Entries behind a request's last page are never read.  Several rows may
+ * name the same page (a shared prompt), as long as nothing is appended to it; tq_page_plan's release of ended requests knows no
+ * owners, so such rows are the caller's to release.  A page number outside the pool reads as the pool's last page.  Lengths are
+ * those in device memory at the time the kernels run: all calls can be captured into a graph, whose replays follow new lengths.
+ * kv_bits 4 and 2, head_dim 128, num_heads a multiple of num_kv_heads.  Codes, q, out, K, V, rotation: 16-byte aligned; strides are in
+ * elements, multiples of 8.  Calls check their arguments before anything is enqueued.
+ * =================================================================================================================== */
+
+/* Block tables and slot maps of one step, from lengths.  Request g holds context_lens[g] tokens (a negative value x: ~x, see below)
+ * and is to get new_tokens[g] more (negative: none).
+ *   - Where finished (uint8 [G], may be NULL) is not zero, the request has ended: its pages go back to the stack free_pages
+ *     [num_pages] (which holds *free_count of them), in order of requests and pages, and it holds no tokens; the row may get a new
+ *     request's tokens in the same call.
+ *   - New tokens get pages from the top of the stack, in order of requests.  A request is admitted if its tokens fit its row of
+ *     the table and, where it wants any, all new tokens up to and including its own fit the slot map and the new pages wanted up
+ *     to and including its own are there (a request that fits no row counts for none); what needs no page waits for none.
+ *   - seq_lens[g] = tokens held with the new ones, or ~(tokens held), a negative number, where the request was not admitted: the
+ *     attentions give zeros for it, and the next step's context_lens may hold that value.  May be context_lens itself.
+ *   - query_start[G + 1]: running sum of new_tokens from 0, at most T.  slots[t] and positions[t] (may be NULL): row and position of new
+ *     token t of the batch; -1 for those of requests not admitted and behind the last one (T: what the arrays hold).
+ *   - free_count_out: pages left (may be free_count itself). */
+int tq_page_plan(int* block_table, int table_stride, int table_width, int* free_pages, const int* free_count, int* free_count_out,
+                 int num_pages, int page_size, const int* context_lens, const int* new_tokens, const unsigned char* finished, int G,
+                 int* seq_lens, int* query_start, long long* slots, int* positions, int T, tq_stream_t s);
+
+/* Quantises token t of k_buf and v_buf ([T], kv_stride apart, num_kv_heads * 128 each) into row slots[t] of the caches: the bytes of
+ * launch_turbo_kv_quantize.  A slot outside 0 .. total_rows - 1 (padding: -1) stores nothing; slots of one call are distinct otherwise. */
+int tq_paged_append(uint8_t* ck_q, void* k_norms, uint8_t* cv_q, void* v_norms, const void* k_buf, const void* v_buf,
+                    const void* rotation, const long long* slots, long long total_rows, int T, int num_kv_heads, int head_dim,
+                    long long kv_stride, int bits, tq_stream_t s);
+
+/* The inverse: K and V vectors that the rows slots[t] stand for, norm * R^T centroids, as fp16 (zeros for a slot that is no row). */
+int tq_paged_read(void* k_out, void* v_out, const uint8_t* ck_q, const void* k_norms, const uint8_t* cv_q, const void* v_norms,
+                  const void* rotation, const long long* slots, long long total_rows, int T, int num_kv_heads, int head_dim,
+                  long long kv_stride, int bits, tq_stream_t s);
+
+/* Bytes of device workspace (256-byte aligned) of the two attentions for T query tokens of G requests.  Calls that share one
+ * must not overlap on the GPU. */
+size_t tq_paged_workspace_bytes(int T, int G, int num_heads);
+
+/* Decode attention: query g attends to tokens 0 .. seq_lens[g] - 1 of request g (0 and less: its row of out is zeros; lengths count up to
+ * table_width * page_size).  q rows q_stride, out rows out_stride apart.  The number of columns (table_width) bounds the lengths for the
+ * choice of kernel: hand over a narrower table where the host knows a smaller bound. */
+int tq_paged_decode_attention(void* out, const void* q, const uint8_t* ck_q, const uint8_t* cv_q, const void* k_norms,
+                              const void* v_norms, const void* rotation, const int* block_table, int table_stride, int table_width,
+                              const int* seq_lens, int num_pages, int page_size, int G, int num_heads, int num_kv_heads, int head_dim,
+                              int q_stride, int out_stride, int bits, void* workspace, size_t workspace_bytes, tq_stream_t s);
+
+/* Reads (and clears) the status word that all paged calls on the current device share: 0, or a code as tq_workspace_status gives.
+ * Synchronises the stream. */
+int tq_paged_status(tq_stream_t s);
+
+/* ===================================================================================================================
  * Peer exchange for sequence-sharded ranks (one process per GPU).  No counterpart in the reference, which runs on one
  * GPU.  Every rank owns one buffer (made here with cudaMalloc so that a CUDA IPC handle names it); its peers open the
  * handle, copy their attention outputs into their slice with plain device-to-device copies (copy engines over NVLink:

@@ -1,0 +1,71 @@
+"""Refusals of the paged calls: every one happens before anything is enqueued, so no GPU is needed."""
+import ctypes as C
+
+import pytest
+
+import triebwerk_b200 as tq
+
+P = C.c_void_p(1 << 20)  # never followed: the call is refused first
+ODD = C.c_void_p((1 << 20) + 2)
+
+
+def plan(**kw):
+    a = dict(table=P, stride=8, width=8, free=P, count=P, count_out=P, pages=16, page=32, context=P, new=P, finished=None, G=4, lens=P, start=P, slots=P,
+             positions=None, T=4)
+    a.update(kw)
+    return tq.lib().tq_page_plan(*a.values(), None)
+
+
+def rows(name, **kw):
+    a = dict(ck=P, kn=P, cv=P, vn=P, k=P, v=P, R=P, slots=P, rows=64, T=2, Hkv=8, D=128, stride=1024, bits=4)
+    a.update(kw)
+    if name == "tq_paged_read":
+        a = {k: a[k] for k in ("k", "v", "ck", "kn", "cv", "vn", "R", "slots", "rows", "T", "Hkv", "D", "stride", "bits")}
+    return getattr(tq.lib(), name)(*a.values(), None)
+
+
+def attention(**kw):
+    a = dict(out=P, q=P, ck=P, cv=P, kn=P, vn=P, R=P, table=P, stride=8, width=8, lens=P, pages=16, page=32, G=4, H=16, Hkv=8, D=128, qs=2048, os=2048, bits=4,
+             ws=P, bytes=1 << 30)
+    a.update(kw)
+    return tq.lib().tq_paged_decode_attention(*a.values(), None)
+
+
+@pytest.mark.parametrize("change, status", [
+    (dict(page=16), -4), (dict(page=48), -4), (dict(page=0), -4), (dict(page=131072), -4), (dict(width=0), -1), (dict(stride=7), -1), (dict(pages=0), -1),
+    (dict(pages=1 << 27), -4), (dict(width=1 << 26, stride=1 << 26), -4), (dict(table=None), -1), (dict(free=None), -1), (dict(count=None), -1),
+    (dict(count_out=None), -1), (dict(context=None), -1), (dict(new=None), -1), (dict(lens=None), -1), (dict(start=None), -1), (dict(slots=None), -1),
+    (dict(G=0), -1), (dict(T=-1), -1)])
+def test_plan_refuses(change, status):
+    assert plan(**change) == status
+
+
+@pytest.mark.parametrize("name", ["tq_paged_append", "tq_paged_read"])
+@pytest.mark.parametrize("change, status", [
+    (dict(D=64), -4), (dict(bits=0), -1), (dict(bits=3), -1), (dict(Hkv=0), -1), (dict(rows=0), -1), (dict(rows=1 << 31), -4), (dict(stride=1016), -1),
+    (dict(stride=1028), -1), (dict(T=-1), -1), (dict(T=1 << 28), -4), (dict(ck=None), -1), (dict(kn=None), -1), (dict(cv=None), -1), (dict(vn=None), -1),
+    (dict(k=None), -1), (dict(v=None), -1), (dict(R=None), -1), (dict(slots=None), -1), (dict(ck=ODD), -1), (dict(k=ODD), -1), (dict(v=ODD), -1),
+    (dict(R=ODD), -1)])
+def test_rows_refuse(name, change, status):
+    assert rows(name, **change) == status
+
+
+@pytest.mark.parametrize("name", ["tq_paged_append", "tq_paged_read"])
+def test_no_tokens_is_no_work(name):
+    assert rows(name, T=0, k=None, v=None, slots=None) == 0
+
+
+@pytest.mark.parametrize("change, status", [
+    (dict(page=16), -4), (dict(page=96), -4), (dict(D=64), -4), (dict(bits=0), -1), (dict(bits=8), -1), (dict(G=0), -1), (dict(H=15), -1), (dict(Hkv=0), -1),
+    (dict(H=0), -1), (dict(qs=2040), -1), (dict(qs=2052), -1), (dict(os=2047), -1), (dict(stride=4), -1), (dict(width=0), -1), (dict(pages=0), -1),
+    (dict(pages=1 << 26), -4), (dict(out=None), -1), (dict(q=None), -1), (dict(ck=None), -1), (dict(cv=None), -1), (dict(kn=None), -1), (dict(vn=None), -1),
+    (dict(R=None), -1), (dict(table=None), -1), (dict(lens=None), -1), (dict(ws=None), -3), (dict(ws=ODD), -3), (dict(bytes=1000), -3), (dict(q=ODD), -1),
+    (dict(out=ODD), -1), (dict(kn=ODD), -1)])
+def test_decode_refuses(change, status):
+    assert attention(**change) == status
+
+
+def test_workspace_sizes():
+    f = tq.lib().tq_paged_workspace_bytes
+    assert f(1, 0, 16) == 0 and f(-1, 1, 16) == 0 and f(1, 1, 0) == 0
+    assert 0 < f(4, 4, 16) < f(64, 64, 16) < f(64, 64, 32)

@@ -41,8 +41,15 @@ def build_hostcall(force: bool = False) -> str:
 def build(force: bool = False, verbose: bool = False) -> str:
     """Compile whatever is missing or older than its sources.  Returns the library's path."""
     if force or _stale(LIB, sources()):
-        cmd = [NVCC] + FLAGS + (["-Xptxas", "-v"] if verbose else []) + ["-o", LIB, os.path.join(CSRC, "tq_capi.cu")]
-        subprocess.check_call(cmd)
+        # one object per translation unit, side by side
+        units = [os.path.join(CSRC, f) for f in sorted(os.listdir(CSRC)) if f.endswith(".cu")]
+        objects = [u[:-3] + ".o" for u in units]
+        running = [(u, subprocess.Popen([NVCC] + FLAGS + (["-Xptxas", "-v"] if verbose else []) + ["-c", "-o", o, u]))
+                   for u, o in zip(units, objects) if force or _stale(o, [u] + [s for s in sources() if not s.endswith(".cu")])]
+        failed = [u for u, p in running if p.wait() != 0]  # (every compiler has ended before anything is raised)
+        if failed:
+            raise RuntimeError("nvcc failed on " + ", ".join(failed))
+        subprocess.check_call([NVCC] + FLAGS + ["-o", LIB] + objects)
     build_hostcall(force)
     return LIB
 

@@ -109,6 +109,11 @@ struct AttnParams {
     int* table_out;                // [G + 4]: the tile table, then {workers taking part, total tiles}, for the merge kernel
     const __half* q_rot16;         // layer and whole-step form: pre-rotated, pre-scaled fp16 queries of layer0, [layers][G][H][128]
                                    // (layer_prep_kernel, rotate_queries_kernel); a sequence's block reaches shared memory by one bulk copy
+    // PAGED (MODE 1): positions holds LENGTHS (0 and less: no token), and token t of sequence g is row table[g][t >> page_shift] <<
+    // page_shift plus t's place in its page.  A tile lies within one page.  Page numbers outside the pool are taken as its last page.
+    const int* block_table;
+    int table_stride, page_shift, num_pages;
+    int most_tokens;               // of a sequence: what the table has pages for
 #ifdef TQ_TIMING_SWITCHES
     int debug;                 // timing-experiment builds only: bit 0 = skip the math, bit 1 = skip the loads, ... (results are then wrong)
     unsigned long long* stamps;  // timing-experiment builds only: [8] summed clock deltas of the tile loop's sections
@@ -403,12 +408,13 @@ __device__ __forceinline__ void merge_sequence(const float* part0, int parts, in
 template <int HKV, int MODE>
 constexpr int attn_threads() { return ATTN_GROUPS * 32 * HKV + (MODE == 1 || MODE == 2 ? (HKV == 8 ? 128 : 64) : 0); }
 constexpr int ATTN_REGS_WORK = 112, ATTN_REGS_COPY = 32;
-template <int BITS, int HKV, int MODE>
+template <int BITS, int HKV, int MODE, bool PAGED = false>
 __global__ void __launch_bounds__(attn_threads<HKV, MODE>(), 1)
 decode_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                         const AttnParams p) {
     using Geo = AttnGeom<BITS>;
     constexpr bool LAYER = MODE == 1;
+    static_assert(!PAGED || LAYER, "pages: one layer at a time, nothing appended");
     constexpr bool PERSIST = MODE == 2 || MODE == 4;
     constexpr bool PUBLISH = LAYER || PERSIST;
     constexpr bool COPIER = MODE == 1 || MODE == 2;
@@ -528,7 +534,7 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
             if (gq < G) {
                 int pos = LAYER && base == 0 ? first_pos : p.positions ? __ldcg(p.positions + gq) : p.pos_value;
                 if (pos < 0) pos = 0;
-                n = (pos + TILE_TOKENS) / TILE_TOKENS;
+                n = PAGED ? (min(pos, p.most_tokens) + TILE_TOKENS - 1) / TILE_TOKENS : (pos + TILE_TOKENS) / TILE_TOKENS;
             }
             int incl = n;
 #pragma unroll
@@ -598,6 +604,11 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
     int cl_gend = ts[g + 1];
     // first cache row of tile j of sequence gq (j counted from the sequence's first tile)
     auto tile_row = [&](int gq, int j) -> int {
+        if constexpr (PAGED) {
+            const int t = j * TILE_TOKENS;
+            const uint32_t page = (uint32_t)__ldcg(p.block_table + (size_t)gq * p.table_stride + (t >> p.page_shift));
+            return (int)(min(page, (uint32_t)p.num_pages - 1u) << p.page_shift) + (t & ((1 << p.page_shift) - 1));
+        }
         if (p.prefix_tiles && j < p.prefix_tiles[gq]) return (int)p.prefix_base[gq] + j * TILE_TOKENS;
         return (int)(p.row_base ? p.row_base[gq] : (long long)gq * p.max_seq_len) + j * TILE_TOKENS;
     };
@@ -607,6 +618,11 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
     int cl_layer = 0;                           // whole-step form: layer (relative to layer0) the cursor is in
     const int g_lo = g;
     const int n_layers = PERSIST ? p.n_layers : 1;
+    auto next_sequence = [&](int gq) {  // (called while there are tiles left: one of the next ones has some)
+        do ++gq;
+        while (PAGED && ts[gq + 1] == ts[gq]);
+        return gq;
+    };
     auto cursor_advance = [&]() {
         ++cl_tile;
         cl_row += TILE_TOKENS;
@@ -618,10 +634,14 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
             cl_row = row_lo;
             if (p.prefix_tiles) cl_switch = ts[g_lo] + p.prefix_tiles[g_lo];
         } else if (cl_tile == cl_gend && cl_tile < hi_i) {
-            ++cl_g;
+            cl_g = next_sequence(cl_g);
             cl_gend = ts[cl_g + 1];
             cl_row = tile_row(cl_g, 0);
             if (p.prefix_tiles) cl_switch = cl_tile + p.prefix_tiles[cl_g];
+        } else if (PAGED) {
+            // (the page number is on its way while the copy warp waits for the ring)
+            const int j = cl_tile - ts[cl_g];
+            if (cl_tile < hi_i && (j & ((1 << (p.page_shift - 5)) - 1)) == 0) cl_row = tile_row(cl_g, j);
         } else if (cl_tile == cl_switch) {  // from the shared prefix into the sequence's own rows
             cl_row = tile_row(cl_g, cl_tile - ts[cl_g]);
         }
@@ -738,7 +758,7 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
             pdl_wait();
             pdl_launch_dependents();
         }
-        if (gtid == 0 && loads_on) issue_queries(0, g);
+        if (gtid == 0 && loads_on && (!PAGED || lo_i < hi_i)) issue_queries(0, g);  // (no tokens at all: nobody would wait for it)
     } else {
         fill_ring();
     }
@@ -779,7 +799,8 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
         const int ts_g1 = ts[g + 1];
         const int seg_end = hi_i < ts_g1 ? hi_i : ts_g1;
         const int pos = p.positions ? p.positions[g] : p.pos_value;
-        const int L = (pos < 0 ? 0 : pos) + 1;
+        const int L = PAGED ? min(pos, p.most_tokens) : (pos < 0 ? 0 : pos) + 1;
+        const int g_next = seg_end < hi_i ? next_sequence(g) : g + 1;
         TQ_STAMP(8);   // loop tail + publishing of the previous segment + this segment's table / position reads
         // query fragments (B operand of the score product): lane (gl, t4) holds coordinates 32*t4 .. 32*t4+31 of head
         // head*grp + gl as fp16
@@ -897,7 +918,7 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
             TQ_STAMP(11);  // barrier of the worker's warps
             if (gtid == 0 && !dead && loads_on) {
                 fence_proxy_async_smem();
-                if (seg_end < hi_i) issue_queries(layer, g + 1);
+                if (seg_end < hi_i) issue_queries(layer, g_next);
                 else if (layer + 1 < n_layers) issue_queries(layer + 1, g_lo);
             }
         } else {
@@ -1254,9 +1275,9 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
                 }
             }
         }
-        if (TQ_DBG(4)) { ++g; continue; }
+        if (TQ_DBG(4)) { g = g_next; continue; }
         if constexpr (PUBLISH) {  // the partials are merged by a launch of its own
-            ++g;
+            g = g_next;
             continue;
         }
         // number of workers that hold a part of sequence g: owners of the sequence's first and last tile
@@ -1328,7 +1349,7 @@ struct MergeParams {
 };
 
 // Merge of a whole step's partials: one CTA of 8 warps per (sequence, layer), two heads per warp.
-__global__ void __launch_bounds__(256) merge_partials_kernel(const MergeParams p) {
+static __global__ void __launch_bounds__(256) merge_partials_kernel(const MergeParams p) {
     __shared__ __align__(16) uint8_t merge_buf[RegionA::MERGE_GROUP_BYTES];
     pdl_wait();  // the partials and the table come from the previous kernel in the stream
     const int g = blockIdx.x, layer = blockIdx.y;
@@ -1369,11 +1390,13 @@ struct MergeLayerParams {
     float* out_f32;              // optional [G][H][128]
     int pos_value, G, H, q_dim;
     int workers;                 // workers of the attention launch
+    int most_tokens;             // PAGED: positions holds lengths, of which no more than this count
 };
 // HEADS = 1: a CTA per (sequence, head) instead, an eighth of its parts for every warp: for few sequences, which are cut into many parts
 // each (launch_merge_layer, tq_host.cuh).
 constexpr int MERGE_WARPS = 8;
-template <int HEADS, int PER_SM>
+// PAGED: sequences without tokens get zeros.
+template <int HEADS, int PER_SM, bool PAGED = false>
 __global__ void __launch_bounds__(MERGE_WARPS * 32, PER_SM) merge_layer_kernel(const MergeLayerParams p) {
     static_assert(HEADS == 1 || HEADS == MERGE_WARPS, "a warp per head, or all warps for one");
     constexpr bool SPLIT = HEADS == 1;
@@ -1393,6 +1416,7 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32, PER_SM) merge_layer_kernel(c
             bf[i][m] = ldg128_l2(reinterpret_cast<const uint4*>(p.rotation_t + (size_t)(8 * (warp + MERGE_WARPS * i) + gl) * HEAD_DIM) + t4 + 4 * m);
     auto tiles_of = [&](int i) {
         const int pos = p.positions ? __ldcg(p.positions + i) : p.pos_value;
+        if (PAGED) return (min(max(pos, 0), p.most_tokens) + TILE_TOKENS - 1) / TILE_TOKENS;
         return ((pos < 0 ? 0 : pos) + TILE_TOKENS) / TILE_TOKENS;
     };
     int before = 0, all = 0;  // tiles before sequence g, of all sequences
@@ -1415,10 +1439,11 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32, PER_SM) merge_layer_kernel(c
         all += sums[0][w];
         before += sums[1][w];
     }
+    if (PAGED) all = max(all, 1);
     // owners of the sequence's first and last tile, as in the attention kernel's cut of the list
     const long long W = attention_workers(p.workers, all, p.G);
     const int first_w = (int)(((long long)(before + 1) * W - 1) / all);
-    const int all_parts = (int)(((long long)(before + own) * W - 1) / all) - first_w + 1;
+    const int all_parts = PAGED && own == 0 ? 0 : (int)(((long long)(before + own) * W - 1) / all) - first_w + 1;
     const int part_lo = SPLIT ? all_parts * warp / MERGE_WARPS : 0, parts = SPLIT ? all_parts * (warp + 1) / MERGE_WARPS - part_lo : all_parts;
     const size_t pstride = (size_t)p.H * PART_STRIDE;
     const float* const part0 = p.partials + ((size_t)(first_w + g) * p.H + h) * PART_STRIDE + (size_t)part_lo * pstride;

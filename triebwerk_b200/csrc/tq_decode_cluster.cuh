@@ -76,6 +76,10 @@ struct ClusterDecodeParams {
     int head_blocks;             // clusters per KV head: ceil(query heads per KV head / 8)
     int early;                   // as in AttnParams: positions and old rows may be read before the previous kernel has finished
     int static_rotation;         // R is not written by any kernel of the stream: staged before the wait
+    // PAGED: as in AttnParams -- positions holds lengths, of which capacity_rows count
+    const int* block_table;
+    int table_stride, page_shift, num_pages;
+    int out_dim;                 // halves between the results of consecutive sequences (otherwise q_dim)
 };
 
 __device__ __forceinline__ uint32_t cluster_ctarank() {
@@ -176,10 +180,12 @@ inline size_t cd_smem_bytes(int bits, int heads, bool exact) {
 // MB: 16-token blocks per tile (2 for throughput, 1 where every warp gets a single tile anyway and its latency counts)
 // HOST: q, new_k, new_v (and out) are pinned host memory: every byte of them is fetched once per CTA, not once per warp
 // EXACT: rotated queries, centroids and weights as fp16 high + low parts (see above)
-template <int BITS, int MB, bool HOST, bool EXACT>
+// PAGED: rows by way of a block table; nothing is appended, a sequence without tokens gives zeros
+template <int BITS, int MB, bool HOST, bool EXACT, bool PAGED = false>
 __global__ void __launch_bounds__(CD_THREADS, EXACT && BITS != 0 ? 1 : 2) cluster_decode_kernel(const ClusterDecodeParams p_in) {
     extern __shared__ __align__(1024) uint8_t cd_smem[];
     ClusterDecodeParams p = p_in;
+    static_assert(!PAGED || (BITS != 0 && !HOST), "packed caches on the device");
     constexpr int BPH = BITS == 0 ? 256 : (BITS == 4 ? 64 : 32);  // bytes of a head's row
     constexpr int TT = 16 * MB;                                   // tokens per tile
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -194,6 +200,7 @@ __global__ void __launch_bounds__(CD_THREADS, EXACT && BITS != 0 ? 1 : 2) cluste
         p.new_k += layer * p.kv_layer_stride; p.new_v += layer * p.kv_layer_stride;
         if (p.out_f32) p.out_f32 += (long long)layer * p.G * p.H * HEAD_DIM;
     }
+    const size_t out_at = (size_t)g * (PAGED ? p.out_dim : p.q_dim);
     const int grp = p.H / p.Hkv;
     const int nh = min(CD_HEADS, grp - CD_HEADS * hblk);  // query heads of this cluster
     const int head0 = kvh * grp + CD_HEADS * hblk;
@@ -239,7 +246,8 @@ __global__ void __launch_bounds__(CD_THREADS, EXACT && BITS != 0 ? 1 : 2) cluste
         pos_ok = pos >= 0 && (cap <= 0 || pos < cap);
         int L = (pos < 0 ? 0 : pos) + 1;
         if (cap > 0 && L > cap) L = cap;  // a position outside its slot is reported; rows outside the slot are not read
-        appends = p.new_k != nullptr && pos_ok;
+        if (PAGED) L = min(max(pos, 0), cap);
+        appends = !PAGED && p.new_k != nullptr && pos_ok;
         lim = appends ? L - 1 : L;        // (the row this very step writes is never read from the cache)
         const int W = p.new_k != nullptr && S >= 4u ? (int)S - 1 : (int)S;  // CTAs that take the cached tokens
         tile_end = (int)rank < W ? (lim + TT - 1) / TT : 0;
@@ -256,6 +264,14 @@ __global__ void __launch_bounds__(CD_THREADS, EXACT && BITS != 0 ? 1 : 2) cluste
     uint4 vw[MB][4][VV4];                      // V rows 2 t4, 2 t4 + 1, 2 t4 + 8, 2 t4 + 9: the lane's 16 coordinates 16 gl ..
     __half kn_h[MB][2], vn_h[MB][2];           // norms of rows gl, gl + 8
     auto token_row = [&](int t) -> size_t { return (size_t)(t < ptok ? prow0 + t : row0 + t); };
+    // PAGED: a tile lies within one page, whose number is requested one tile ahead
+    uint32_t page = 0;
+    auto fetch_page = [&](int tile) { page = ldg32_if(p.block_table + (size_t)g * p.table_stride + ((tile * TT) >> p.page_shift), tile < tile_end); };
+    auto use_page = [&](int tile) {  // (row0: such that token_row gives the tile's rows)
+        const int t0 = tile * TT;
+        row0 = ((long long)min(page, (uint32_t)p.num_pages - 1u) << p.page_shift) + (t0 & ((1 << p.page_shift) - 1)) - t0;
+        fetch_page(tile + tile_step);
+    };
     // rows at or past `lim` are not read: they count as zero codes with zero norm, and are masked anyway
     auto load_k = [&](int tile, int lim) {
 #pragma unroll
@@ -308,6 +324,10 @@ __global__ void __launch_bounds__(CD_THREADS, EXACT && BITS != 0 ? 1 : 2) cluste
     auto first_tile = [&]() {
         use_position();
         if (tile < tile_end) {
+            if (PAGED) {
+                fetch_page(tile);
+                use_page(tile);
+            }
             load_k(tile, lim);
             load_v(tile, lim);
         }
@@ -710,7 +730,10 @@ __global__ void __launch_bounds__(CD_THREADS, EXACT && BITS != 0 ? 1 : 2) cluste
                 sv[2 * b + r][1] = on ? c[b][2 * r + 1] * n : -1e30f;
             }
         const int next = tile + tile_step;
-        if (next < tile_end) load_k(next, lim);
+        if (next < tile_end) {
+            if (PAGED) use_page(next);
+            load_k(next, lim);
+        }
         float mx0 = sv[0][0], mx1 = sv[0][1];
 #pragma unroll
         for (int i = 1; i < 2 * MB; ++i) {
@@ -954,7 +977,7 @@ __global__ void __launch_bounds__(CD_THREADS, EXACT && BITS != 0 ? 1 : 2) cluste
                 if (S == 1) {
                     const size_t at = (size_t)(head0 + gl) * HEAD_DIM + 8 * nb + 2 * t4;
                     if (HOST) stage_out(gl * HEAD_DIM + 8 * nb + 2 * t4, pack_half2(o0, o1));
-                    else *reinterpret_cast<__half2*>(p.out + (size_t)g * p.q_dim + at) = __floats2half2_rn(o0, o1);
+                    else *reinterpret_cast<__half2*>(p.out + out_at + at) = __floats2half2_rn(o0, o1);
                     if (p.out_f32) *reinterpret_cast<float2*>(p.out_f32 + (size_t)g * p.H * HEAD_DIM + at) = make_float2(o0, o1);
                 } else {
                     send(gl, 8 * nb + 2 * t4, o0, o1);
@@ -990,7 +1013,7 @@ __global__ void __launch_bounds__(CD_THREADS, EXACT && BITS != 0 ? 1 : 2) cluste
             if (r == 0) {
                 a = __fdividef(a, Z + 1e-8f);
                 const size_t at = (size_t)(head0 + h) * HEAD_DIM + ((int)rank << share_log) + n;
-                p.out[(size_t)g * p.q_dim + at] = __float2half_rn(a);
+                p.out[out_at + at] = __float2half_rn(a);
                 if (p.out_f32) p.out_f32[(size_t)g * p.H * HEAD_DIM + at] = a;
             }
         }

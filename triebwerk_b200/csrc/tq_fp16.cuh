@@ -41,7 +41,7 @@ struct Fp16AttnParams {
                                    // rows of one real KV head, each serving GRP of its query heads)
 };
 
-__global__ void fp16_cache_write_kernel(__half* ck, __half* cv, const __half* k, const __half* v, const int* positions,
+static __global__ void fp16_cache_write_kernel(__half* ck, __half* cv, const __half* k, const __half* v, const int* positions,
                                         const long long* row_base, int max_seq_len, int capacity_rows, int G,
                                         int kv_dim, int* status, const int* seq_capacity = nullptr, int* tickets = nullptr, int n_tickets = 0) {
     const int g = blockIdx.x;
@@ -79,7 +79,7 @@ struct Fp16PromptParams {
     long long row0, seq_rows;
     int first_pos, T, kv_dim;
 };
-__global__ void __launch_bounds__(256) fp16_prompt_write_kernel(const Fp16PromptParams p) {
+static __global__ void __launch_bounds__(256) fp16_prompt_write_kernel(const Fp16PromptParams p) {
     pdl_launch_dependents();
     pdl_wait();
     const int seq = blockIdx.y;

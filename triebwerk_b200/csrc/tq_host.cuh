@@ -371,16 +371,16 @@ inline int attention_ctas(int G, int max_seq_len) {
     return (int)(w < 1 ? 1 : w);
 }
 
-template <int BITS, int HKV, int MODE>
+template <int BITS, int HKV, int MODE, bool PAGED = false>
 inline int launch_attention_t(const CUtensorMap& tmK, const CUtensorMap& tmV, const AttnParams& p, int ctas, cudaStream_t s,
                               bool pdl) {
-    int ar = ensure_dynamic_smem((const void*)decode_attention_kernel<BITS, HKV, MODE>, ATTN_DYN_SMEM);
+    int ar = ensure_dynamic_smem((const void*)decode_attention_kernel<BITS, HKV, MODE, PAGED>, ATTN_DYN_SMEM);
     if (ar != TQ_OK) return ar;
     if constexpr ((MODE == 1 || MODE == 2) && HKV == 8) {
         // the register split inside the kernel draws on what the launch brings: never launch with less
         static const int regs = [] {
             cudaFuncAttributes f{};
-            return cudaFuncGetAttributes(&f, (const void*)decode_attention_kernel<BITS, HKV, MODE>) == cudaSuccess ? f.numRegs : 0;
+            return cudaFuncGetAttributes(&f, (const void*)decode_attention_kernel<BITS, HKV, MODE, PAGED>) == cudaSuccess ? f.numRegs : 0;
         }();
         if (regs * attn_threads<HKV, MODE>() < 32 * (ATTN_GROUPS * HKV * ATTN_REGS_WORK + 4 * ATTN_REGS_COPY)) return TQ_ERR_UNSUPPORTED;
     }
@@ -394,7 +394,7 @@ inline int launch_attention_t(const CUtensorMap& tmK, const CUtensorMap& tmV, co
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = pdl ? 1 : 0;
-    return cuda_status(cudaLaunchKernelEx(&cfg, decode_attention_kernel<BITS, HKV, MODE>, tmK, tmV, p));
+    return cuda_status(cudaLaunchKernelEx(&cfg, decode_attention_kernel<BITS, HKV, MODE, PAGED>, tmK, tmV, p));
 }
 
 // mode 0: after append_rotate_kernel (rotated queries and tile table in the workspace, merge in the kernel); 1: one layer, after
@@ -427,9 +427,9 @@ inline int launch_layer_prep(int bits, const LayerPrepParams& p, cudaStream_t s,
 
 // One cluster per (sequence, KV head, block of 8 query heads): tq_decode_cluster.cuh.  `max_tokens`: rows a sequence may hold.
 constexpr size_t CD_ONE_PER_SM = 118 * 1024;  // more than half of an SM's shared memory
-template <int BITS, int MB, bool HOST, bool EXACT>
+template <int BITS, int MB, bool HOST, bool EXACT, bool PAGED = false>
 inline int launch_cluster_decode_t(const ClusterDecodeParams& p, int S, int layers, cudaStream_t s, bool pdl) {
-    const void* kernel = (const void*)cluster_decode_kernel<BITS, MB, HOST, EXACT>;
+    const void* kernel = (const void*)cluster_decode_kernel<BITS, MB, HOST, EXACT, PAGED>;
     int r = ensure_dynamic_smem(kernel, std::max(cd_smem_bytes(BITS, CD_HEADS, EXACT), CD_ONE_PER_SM), true);
     if (r != TQ_OK) return r;
     cudaLaunchConfig_t cfg{};
@@ -450,7 +450,7 @@ inline int launch_cluster_decode_t(const ClusterDecodeParams& p, int S, int laye
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = pdl ? 2 : 1;
-    return cuda_status(cudaLaunchKernelEx(&cfg, cluster_decode_kernel<BITS, MB, HOST, EXACT>, p));
+    return cuda_status(cudaLaunchKernelEx(&cfg, cluster_decode_kernel<BITS, MB, HOST, EXACT, PAGED>, p));
 }
 // CTAs per cluster.  As many as give every warp a 16-token block of its own, up to one CTA per SM over the whole launch: two share
 // the SM's L1 and issue slots, and the CTAs of the next launch find no room for their prologue (8 sequences x 1023 tokens through
@@ -523,41 +523,44 @@ inline int cluster_launch_split(int bits, int G, int split_layers, int H, int Hk
     const bool streams = fast_shape(H, Hkv, bits != 0), one_per_sm = bits != 0 && !streams;  // (EXACT, packed: as with 8 heads)
     return cluster_split(bits, (long long)G * split_layers * Hkv * head_blocks, one_per_sm ? CD_HEADS : std::min(CD_HEADS, H / Hkv), max_tokens, split_layers == 1, streams);
 }
-template <bool HOST, bool EXACT>
+template <bool HOST, bool EXACT, bool PAGED = false>
 inline int launch_cluster_decode_e(int bits, const ClusterDecodeParams& p, int layers, int split_layers, int max_tokens, cudaStream_t s, bool pdl) {
     const int blocks = (max_tokens + 15) / 16;
     const int S = cluster_launch_split(bits, p.G, split_layers, p.H, p.Hkv, max_tokens);
-    if (bits == 0) return launch_cluster_decode_t<0, 1, HOST, EXACT>(p, S, layers, s, pdl);
+    if constexpr (!PAGED) {
+        if (bits == 0) return launch_cluster_decode_t<0, 1, HOST, EXACT>(p, S, layers, s, pdl);
+    }
     // 16-token tiles where every warp of the cluster has one at most.  (From four CTAs on the new token's takes none, so that the last
     // S-th of a full slot is a second tile for some warps.  Two blocks per tile there: 8 layers of 1 x 980 tokens in 1024 rows, 4-bit 16/8
     // heads, 46.3 -> 42.5 us, but of 4 x 300 in 512 rows 44.3 -> 46.3: the contexts that fit are seven eighths or three quarters.)
     const bool one = S * CD_WARPS >= blocks;
-    if (bits == 4) return one ? launch_cluster_decode_t<4, 1, HOST, EXACT>(p, S, layers, s, pdl) : launch_cluster_decode_t<4, 2, HOST, EXACT>(p, S, layers, s, pdl);
-    return one ? launch_cluster_decode_t<2, 1, HOST, EXACT>(p, S, layers, s, pdl) : launch_cluster_decode_t<2, 2, HOST, EXACT>(p, S, layers, s, pdl);
+    if (bits == 4) return one ? launch_cluster_decode_t<4, 1, HOST, EXACT, PAGED>(p, S, layers, s, pdl) : launch_cluster_decode_t<4, 2, HOST, EXACT, PAGED>(p, S, layers, s, pdl);
+    return one ? launch_cluster_decode_t<2, 1, HOST, EXACT, PAGED>(p, S, layers, s, pdl) : launch_cluster_decode_t<2, 2, HOST, EXACT, PAGED>(p, S, layers, s, pdl);
 }
-template <bool HOST = false>
+template <bool HOST = false, bool PAGED = false>
 inline int launch_cluster_decode(int bits, const ClusterDecodeParams& p, int layers, int split_layers, int max_tokens, cudaStream_t s, bool pdl) {
-    return fast_shape(p.H, p.Hkv, bits != 0) ? launch_cluster_decode_e<HOST, false>(bits, p, layers, split_layers, max_tokens, s, pdl)
-                                             : launch_cluster_decode_e<HOST, true>(bits, p, layers, split_layers, max_tokens, s, pdl);
+    return fast_shape(p.H, p.Hkv, bits != 0) ? launch_cluster_decode_e<HOST, false, PAGED>(bits, p, layers, split_layers, max_tokens, s, pdl)
+                                             : launch_cluster_decode_e<HOST, true, PAGED>(bits, p, layers, split_layers, max_tokens, s, pdl);
 }
 
 // Merge of a layer's partials.  Few sequences are cut into many parts each, and a warp that adds up a head's alone, 16 in flight, was up to
 // half of the layer: from 14 workers per sequence on, a CTA per head, while these are not many more than the SMs (eight heads per CTA / one, 4-bit
 // 16/8 heads 3 x 30000 tokens 51.3 / 34.4 us a layer, 5 x 16384 40.7 / 31.7, 10 x 8192 35.0 / 31.3, 2-bit 32/8 8 x 8000 29.0 / 26.0; 288 heads: 9 x 8000 28.3 /
 // 28.7, 4-bit 16/8 18 x 6000 37.2 / 38.0; nine parts: 8/8 36 x 2000 27.7 / 30.3).
+template <bool PAGED = false>
 inline int launch_merge_layer(const MergeLayerParams& p, cudaStream_t s, bool pdl) {
     const long long sms = device_props().sm_count, each = (long long)p.G * p.H;
     const dim3 threads(MERGE_WARPS * 32);
     if (p.workers >= 14 * p.G && 4 * each <= 7 * sms) {
         const dim3 grid((unsigned)p.G, (unsigned)p.H);
-        return each <= sms ? launch_kernel(merge_layer_kernel<1, 1>, grid, threads, 0, s, pdl, p) : launch_kernel(merge_layer_kernel<1, 2>, grid, threads, 0, s, pdl, p);
+        return each <= sms ? launch_kernel(merge_layer_kernel<1, 1, PAGED>, grid, threads, 0, s, pdl, p) : launch_kernel(merge_layer_kernel<1, 2, PAGED>, grid, threads, 0, s, pdl, p);
     }
     const dim3 grid((unsigned)p.G, (unsigned)((p.H + MERGE_WARPS - 1) / MERGE_WARPS));
-    return (long long)grid.x * grid.y <= sms ? launch_kernel(merge_layer_kernel<MERGE_WARPS, 1>, grid, threads, 0, s, pdl, p)
-                                             : launch_kernel(merge_layer_kernel<MERGE_WARPS, 2>, grid, threads, 0, s, pdl, p);
+    return (long long)grid.x * grid.y <= sms ? launch_kernel(merge_layer_kernel<MERGE_WARPS, 1, PAGED>, grid, threads, 0, s, pdl, p)
+                                             : launch_kernel(merge_layer_kernel<MERGE_WARPS, 2, PAGED>, grid, threads, 0, s, pdl, p);
 }
 
-__global__ void transpose_rotation_kernel(__half* dst, const __half* src) {
+static __global__ void transpose_rotation_kernel(__half* dst, const __half* src) {
     // dst[d][k] = src[k][d]; one block per 32x32 tile would be overkill for 32 KB: a plain strided copy
     for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < HEAD_DIM * HEAD_DIM; i += gridDim.x * blockDim.x) {
         const int d = i >> 7, k = i & 127;

@@ -45,9 +45,13 @@ struct LayerPrepParams {
     int* status;
     int pos_value, max_seq_len, capacity_rows;
     int G, H, Hkv, q_dim;
+    // SLOTS: token i of new_k, new_v goes to row slots[i] (nowhere outside 0 .. total_rows - 1)
+    const long long* slots;
+    long long total_rows;
+    long long kv_stride;         // halves between the vectors of consecutive tokens
 };
 
-template <int BITS>
+template <int BITS, bool SLOTS = false>
 __global__ void __launch_bounds__(PREP_THREADS, 2) layer_prep_kernel(const LayerPrepParams p) {
     __shared__ __align__(16) __half raw[16][HEAD_DIM];  // the new token's vectors as they arrived
     __shared__ __align__(16) __half r_s[HEAD_DIM][PREP_ROW];  // R, for the exact chains
@@ -90,6 +94,7 @@ __global__ void __launch_bounds__(PREP_THREADS, 2) layer_prep_kernel(const Layer
         for (int i = (int)blockIdx.x * PREP_THREADS + tid; i < HEAD_DIM * HEAD_DIM; i += (int)gridDim.x * PREP_THREADS)
             p.rotation_t[i] = R[(i & (HEAD_DIM - 1)) * HEAD_DIM + (i >> 7)];
     const int nvec = 2 * p.Hkv;
+    const size_t kv_stride = SLOTS ? (size_t)p.kv_stride : (size_t)p.Hkv * HEAD_DIM;
     for (long long item = blockIdx.x; item < n_items; item += gridDim.x) {
         const bool app = item < n_app;
         // rows gl and gl + 8 of the A operand
@@ -100,7 +105,7 @@ __global__ void __launch_bounds__(PREP_THREADS, 2) layer_prep_kernel(const Layer
             const int v = gl + 8 * r;
             if (app) {
                 on[r] = v < nvec;
-                src[r] = (v < p.Hkv ? p.new_k : p.new_v) + ((size_t)item * p.Hkv + (v < p.Hkv ? v : v - p.Hkv)) * HEAD_DIM;
+                src[r] = (v < p.Hkv ? p.new_k : p.new_v) + (size_t)item * kv_stride + (size_t)(v < p.Hkv ? v : v - p.Hkv) * HEAD_DIM;
             } else {
                 const long long vec = (item - n_app) * 16 + v, g = vec / p.H;
                 on[r] = vec < n_vec;
@@ -119,19 +124,23 @@ __global__ void __launch_bounds__(PREP_THREADS, 2) layer_prep_kernel(const Layer
         long long row = 0;
         float x4[2][4];  // append: the vectors 2 warp and 2 warp + 1, coordinates lane + 32 c
         if (app) {
-            if (p.positions) pos = p.positions[item];
-            if (p.seq_capacity) cap = p.seq_capacity[item];
-            row = p.row_base ? p.row_base[item] : (long long)item * p.max_seq_len;
+            if constexpr (SLOTS) {
+                row = p.slots[item];
+            } else {
+                if (p.positions) pos = p.positions[item];
+                if (p.seq_capacity) cap = p.seq_capacity[item];
+                row = p.row_base ? p.row_base[item] : (long long)item * p.max_seq_len;
+            }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int v = 2 * warp + i;
-                const __half* const x = (v < p.Hkv ? p.new_k : p.new_v) + ((size_t)item * p.Hkv + (v < p.Hkv ? v : v - p.Hkv)) * HEAD_DIM;
+                const __half* const x = (v < p.Hkv ? p.new_k : p.new_v) + (size_t)item * kv_stride + (size_t)(v < p.Hkv ? v : v - p.Hkv) * HEAD_DIM;
 #pragma unroll
                 for (int c = 0; c < 4; ++c) x4[i][c] = v < nvec ? __half2float(x[lane + 32 * c]) : 0.0f;
             }
         }
-        const bool ok = pos >= 0 && (cap <= 0 || pos < cap);
-        row += pos;
+        const bool ok = SLOTS ? row >= 0 && row < p.total_rows : pos >= 0 && (cap <= 0 || pos < cap);
+        if constexpr (!SLOTS) row += pos;
         float c[2][2][4];  // [block][chain]
 #pragma unroll
         for (int i = 0; i < 2; ++i)
@@ -182,7 +191,7 @@ __global__ void __launch_bounds__(PREP_THREADS, 2) layer_prep_kernel(const Layer
                 if (v < nvec && ok) (v < p.Hkv ? p.kn : p.vn)[(size_t)row * p.Hkv + (v < p.Hkv ? v : v - p.Hkv)] = __float2half_rn(sqrt_approx_ftz(t));
             }
         }
-        if (tid == 0 && !ok) atomicMax(p.status, ST_BAD_POSITION);
+        if (!SLOTS && tid == 0 && !ok) atomicMax(p.status, ST_BAD_POSITION);
         __syncthreads();
         // the codes: how many bounds a coordinate has reached (NaN: as the reference's comparisons fall out); value 4 r + e: row gl + 8 r,
         // block e >> 1, coordinate 2 t4 + (e & 1) of it.  (All eight a step at a time: their look-ups are in flight together.)

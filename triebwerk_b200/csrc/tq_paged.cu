@@ -1,0 +1,217 @@
+// extern "C" calls over paged packed caches (declared in include/triebwerk_b200.h): a translation unit of its own, so that it compiles
+// beside tq_capi.cu.
+
+#include "tq_host.cuh"
+#include "tq_paged.cuh"
+
+using namespace tq;
+
+static inline cudaStream_t cs(tq_stream_t s) { return reinterpret_cast<cudaStream_t>(s); }
+
+static inline bool use_pdl() {
+    static const bool on = !(getenv("TQ_PDL") && atoi(getenv("TQ_PDL")) == 0);
+    return on;
+}
+
+// The status word of all paged calls on a device: a wait that gave up, a shared-memory layout refused.
+static __device__ int g_paged_status;
+static int paged_status_word(int** out) {
+    static std::mutex mu;
+    static std::map<int, int*> known;
+    int dev = 0;
+    TQ_CUDA(cudaGetDevice(&dev));
+    std::lock_guard<std::mutex> lock(mu);
+    int*& p = known[dev];
+    if (!p) {
+        void* a = nullptr;
+        TQ_CUDA(cudaGetSymbolAddress(&a, g_paged_status));
+        p = (int*)a;
+    }
+    *out = p;
+    return TQ_OK;
+}
+
+static bool page_size_ok(int page_size) { return page_size >= TILE_TOKENS && page_size <= 65536 && (page_size & (page_size - 1)) == 0; }
+static int log2_of(int x) {
+    int s = 0;
+    while ((1 << s) < x) ++s;
+    return s;
+}
+static int check_pages(int table_stride, int table_width, int num_pages, int page_size) {
+    if (!page_size_ok(page_size)) return TQ_ERR_UNSUPPORTED;
+    if (num_pages <= 0 || table_width <= 0 || table_stride < table_width) return TQ_ERR_ARG;
+    if ((long long)num_pages * page_size >= (1ll << 31) || (long long)table_width * page_size >= (1ll << 31)) return TQ_ERR_UNSUPPORTED;
+    return TQ_OK;
+}
+// Cache arrays and R are moved 16 bytes at a time, norms and rows of fewer bytes by their own size.
+static bool aligned(std::initializer_list<const void*> p, unsigned to) {
+    uintptr_t all = 0;
+    for (const void* a : p) all |= (uintptr_t)a;
+    return (all & (to - 1u)) == 0;
+}
+
+extern "C" {
+
+int tq_paged_status(tq_stream_t s) {
+    int* word = nullptr;
+    int r = paged_status_word(&word);
+    return r != TQ_OK ? r : tq_workspace_status(word, s);
+}
+
+int tq_page_plan(int* block_table, int table_stride, int table_width, int* free_pages, const int* free_count, int* free_count_out, int num_pages,
+                 int page_size, const int* context_lens, const int* new_tokens, const unsigned char* finished, int G, int* seq_lens,
+                 int* query_start, long long* slots, int* positions, int T, tq_stream_t s) {
+    int r = check_pages(table_stride, table_width, num_pages, page_size);
+    if (r != TQ_OK) return r;
+    if (!block_table || !free_pages || !free_count || !free_count_out || !context_lens || !new_tokens || !seq_lens || !query_start || G <= 0 || T < 0 || (T > 0 && !slots))
+        return TQ_ERR_ARG;
+    PagePlanParams p{};
+    p.table = block_table; p.free_pages = free_pages; p.free_count = free_count; p.free_count_out = free_count_out;
+    p.context = context_lens; p.new_tokens = new_tokens; p.finished = finished; p.lens = seq_lens; p.start = query_start; p.slots = slots; p.positions = positions;
+    p.G = G; p.T = T; p.num_pages = num_pages; p.table_stride = table_stride; p.width = table_width; p.page_shift = log2_of(page_size);
+    r = launch_kernel(page_plan_kernel, dim3(1), dim3(PLAN_THREADS), 0, cs(s), use_pdl(), p);
+    if (r != TQ_OK || T <= PLAN_ONE_LAUNCH) return r;
+    const int ctas = std::min((T + SLOTS_THREADS - 1) / SLOTS_THREADS, 4 * device_props().sm_count);
+    return launch_kernel(page_slots_kernel, dim3((unsigned)ctas), dim3(SLOTS_THREADS), 0, cs(s), use_pdl(), p);
+}
+
+// (head_dim, head counts, bits, rows)
+static int check_rows(int T, int Hkv, int head_dim, long long kv_stride, int bits, long long total_rows) {
+    if (head_dim != HEAD_DIM) return TQ_ERR_UNSUPPORTED;
+    if (T < 0 || Hkv <= 0 || (bits != 2 && bits != 4) || total_rows <= 0 || kv_stride < (long long)Hkv * HEAD_DIM || kv_stride % 8 != 0) return TQ_ERR_ARG;
+    if (total_rows >= (1ll << 31) || (long long)T * Hkv >= (1ll << 30) || kv_stride >= (1ll << 30)) return TQ_ERR_UNSUPPORTED;
+    return TQ_OK;
+}
+
+int tq_paged_append(uint8_t* ck_q, void* k_norms, uint8_t* cv_q, void* v_norms, const void* k_buf, const void* v_buf, const void* rotation,
+                    const long long* slots, long long total_rows, int T, int num_kv_heads, int head_dim, long long kv_stride, int bits, tq_stream_t s) {
+    int r = check_rows(T, num_kv_heads, head_dim, kv_stride, bits, total_rows);
+    if (r != TQ_OK) return r;
+    if (!ck_q || !k_norms || !cv_q || !v_norms || !rotation || (T > 0 && (!k_buf || !v_buf || !slots))) return TQ_ERR_ARG;
+    if (!aligned({ck_q, cv_q, k_buf, v_buf, rotation}, 16)) return TQ_ERR_ARG;
+    if (T == 0) return TQ_OK;
+    int* status = nullptr;
+    r = paged_status_word(&status);
+    if (r != TQ_OK) return r;
+    // A CTA per token (2 * KV heads <= 16 vectors) while that is no more than a few turns of the SMs, tiles of 128 vectors behind that.
+    if (num_kv_heads <= 8 && T <= 4 * device_props().sm_count) {
+        LayerPrepParams p{};
+        p.ck = ck_q; p.cv = cv_q; p.kn = (__half*)k_norms; p.vn = (__half*)v_norms;
+        p.new_k = (const __half*)k_buf; p.new_v = (const __half*)v_buf; p.rotation = (const __half*)rotation; p.rot_copies = 1; p.status = status;
+        p.G = T; p.H = 0; p.Hkv = num_kv_heads;
+        p.slots = slots; p.total_rows = total_rows; p.kv_stride = kv_stride;
+        const dim3 grid((unsigned)std::min(T, 2 * device_props().sm_count));
+        return bits == 4 ? launch_kernel(layer_prep_kernel<4, true>, grid, dim3(PREP_THREADS), 0, cs(s), use_pdl(), p)
+                         : launch_kernel(layer_prep_kernel<2, true>, grid, dim3(PREP_THREADS), 0, cs(s), use_pdl(), p);
+    }
+    PrefillTcParams t{};
+    t.ck = ck_q; t.cv = cv_q; t.kn = (__half*)k_norms; t.vn = (__half*)v_norms;
+    t.k_buf = (const __half*)k_buf; t.v_buf = (const __half*)v_buf; t.rotation = (const __half*)rotation; t.status = status;
+    t.row_base = slots; t.total_rows = total_rows;
+    t.n_seq = T; t.T = 1; t.Hkv = num_kv_heads; t.kv_dim = (int)kv_stride; t.bits = bits;
+    const long long tiles = 2 * (((long long)T * num_kv_heads + TC_TILE - 1) / TC_TILE);
+    CUtensorMap tmk{}, tmv{};
+    const bool tma = make_append_input_map(&tmk, k_buf, T, num_kv_heads, t.kv_dim) == TQ_OK && make_append_input_map(&tmv, v_buf, T, num_kv_heads, t.kv_dim) == TQ_OK;
+    auto kernel = tma ? prefill_append_tc_kernel<false, true, false, true> : prefill_append_tc_kernel<false, false, false, true>;
+    r = ensure_dynamic_smem((const void*)kernel, TC_DYN_SMEM);
+    if (r != TQ_OK) return r;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)std::min<long long>(tiles, (long long)TC_CTAS_PER_SM * device_props().sm_count));
+    cfg.blockDim = dim3(TC_THREADS);
+    cfg.dynamicSmemBytes = TC_DYN_SMEM;
+    cfg.stream = cs(s);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = use_pdl() ? 1 : 0;
+    return cuda_status(cudaLaunchKernelEx(&cfg, kernel, tmk, tmv, t));
+}
+
+int tq_paged_read(void* k_out, void* v_out, const uint8_t* ck_q, const void* k_norms, const uint8_t* cv_q, const void* v_norms, const void* rotation,
+                  const long long* slots, long long total_rows, int T, int num_kv_heads, int head_dim, long long kv_stride, int bits, tq_stream_t s) {
+    int r = check_rows(T, num_kv_heads, head_dim, kv_stride, bits, total_rows);
+    if (r != TQ_OK) return r;
+    if (!ck_q || !k_norms || !cv_q || !v_norms || !rotation || (T > 0 && (!k_out || !v_out || !slots))) return TQ_ERR_ARG;
+    if (!aligned({ck_q, cv_q, rotation, k_out, v_out}, 16)) return TQ_ERR_ARG;
+    if (T == 0) return TQ_OK;
+    PagedReadParams p{};
+    p.ck = ck_q; p.kn = (const __half*)k_norms; p.cv = cv_q; p.vn = (const __half*)v_norms; p.rotation = (const __half*)rotation;
+    p.slots = slots; p.k_out = (__half*)k_out; p.v_out = (__half*)v_out; p.total_rows = total_rows; p.stride = kv_stride; p.T = T; p.Hkv = num_kv_heads;
+    const long long tiles = 2 * (((long long)T * num_kv_heads + READ_VECTORS - 1) / READ_VECTORS);
+    const dim3 grid((unsigned)std::min<long long>(tiles, 2ll * device_props().sm_count));
+    return bits == 4 ? launch_kernel(paged_read_kernel<4>, grid, dim3(READ_THREADS), 0, cs(s), use_pdl(), p)
+                     : launch_kernel(paged_read_kernel<2>, grid, dim3(READ_THREADS), 0, cs(s), use_pdl(), p);
+}
+
+size_t tq_paged_workspace_bytes(int T, int G, int num_heads) {
+    if (T < 0 || G <= 0 || num_heads <= 0) return 0;
+    return carve_full(nullptr, G, num_heads).bytes;
+}
+
+// What both attentions check of their arguments.
+static int check_attention(const void* out, const void* q, const uint8_t* ck, const uint8_t* cv, const void* kn, const void* vn, const void* rotation,
+                           const int* table, int table_stride, int table_width, const int* lens, int num_pages, int page_size, int G, int H, int Hkv,
+                           int head_dim, int q_stride, int out_stride, int bits) {
+    int r = check_pages(table_stride, table_width, num_pages, page_size);
+    if (r != TQ_OK) return r;
+    if (head_dim != HEAD_DIM) return TQ_ERR_UNSUPPORTED;
+    if (G <= 0 || H <= 0 || Hkv <= 0 || H % Hkv != 0 || (bits != 2 && bits != 4)) return TQ_ERR_ARG;
+    if ((long long)q_stride < (long long)H * HEAD_DIM || (long long)out_stride < (long long)H * HEAD_DIM || q_stride % 8 != 0 || out_stride % 8 != 0) return TQ_ERR_ARG;
+    if (!out || !q || !ck || !cv || !kn || !vn || !rotation || !table || !lens) return TQ_ERR_ARG;
+    if (!aligned({out, q, ck, cv, kn, vn, rotation}, 16)) return TQ_ERR_ARG;
+    return TQ_OK;
+}
+
+int tq_paged_decode_attention(void* out, const void* q, const uint8_t* ck_q, const uint8_t* cv_q, const void* k_norms, const void* v_norms,
+                              const void* rotation, const int* block_table, int table_stride, int table_width, const int* seq_lens, int num_pages,
+                              int page_size, int G, int num_heads, int num_kv_heads, int head_dim, int q_stride, int out_stride, int bits,
+                              void* workspace, size_t workspace_bytes, tq_stream_t s) {
+    int r = check_attention(out, q, ck_q, cv_q, k_norms, v_norms, rotation, block_table, table_stride, table_width, seq_lens, num_pages, page_size, G,
+                            num_heads, num_kv_heads, head_dim, q_stride, out_stride, bits);
+    if (r != TQ_OK) return r;
+    if (!workspace || workspace_bytes < tq_paged_workspace_bytes(G, G, num_heads) || !aligned({workspace}, 256)) return TQ_ERR_WORKSPACE;
+    int* status = nullptr;
+    r = paged_status_word(&status);
+    if (r != TQ_OK) return r;
+    const int H = num_heads, Hkv = num_kv_heads, most = table_width * page_size, head_blocks = (H / Hkv + CD_HEADS - 1) / CD_HEADS;
+    const long long rows = (long long)num_pages * page_size;
+    const bool streams = fast_shape(H, Hkv, true) && G <= FUSED_MAX_G;
+    if (!streams || cluster_layer_faster(bits, G, Hkv, H / Hkv, (long long)G * most, most, LayerCaller::Launchers)) {
+        if (G > 65535 || (long long)Hkv * head_blocks > 65535) return TQ_ERR_UNSUPPORTED;
+        ClusterDecodeParams p{};
+        p.ck = ck_q; p.cv = cv_q; p.kn = (const __half*)k_norms; p.vn = (const __half*)v_norms; p.q = (const __half*)q; p.rotation = (const __half*)rotation;
+        p.out = (__half*)out; p.positions = seq_lens; p.capacity_rows = most; p.max_seq_len = most; p.status = status;
+        p.G = G; p.H = H; p.Hkv = Hkv; p.q_dim = q_stride; p.out_dim = out_stride; p.head_blocks = head_blocks;
+        p.block_table = block_table; p.table_stride = table_stride; p.page_shift = log2_of(page_size); p.num_pages = num_pages;
+        return launch_cluster_decode<false, true>(bits, p, 1, 1, most, cs(s), use_pdl());
+    }
+    const FullWorkspace fw = carve_full(workspace, G, H);
+    CUtensorMap tmK, tmV;
+    r = make_code_map(&tmK, ck_q, rows, Hkv * (bits == 4 ? 64 : 32));
+    if (r == TQ_OK) r = make_code_map(&tmV, cv_q, rows, Hkv * (bits == 4 ? 64 : 32));
+    if (r != TQ_OK) return r;
+    LayerPrepParams lp{};
+    lp.q = (const __half*)q; lp.rotation = (const __half*)rotation; lp.rot_copies = 1; lp.rotation_t = fw.rot_t; lp.status = status;
+    if (bits == 2 && Hkv == 8) lp.q_rot32 = fw.w.q_rot;
+    else lp.q_rot16 = (__half*)fw.w.q_rot;
+    lp.G = G; lp.H = H; lp.Hkv = Hkv; lp.q_dim = q_stride;
+    r = launch_layer_prep(bits, lp, cs(s), use_pdl());
+    if (r != TQ_OK) return r;
+    AttnParams p{};
+    p.ck = ck_q; p.cv = cv_q; p.kn = (const __half*)k_norms; p.vn = (const __half*)v_norms;
+    p.q_rot16 = lp.q_rot16; p.q_rot32 = lp.q_rot32; p.rotation_t = fw.rot_t; p.out = (__half*)out;
+    p.positions = seq_lens; p.partials = fw.w.partials; p.status = status; p.total_rows = rows;
+    p.G = G; p.H = H; p.Hkv = Hkv; p.q_dim = out_stride; p.n_layers = 1; p.l2_ahead = 1 << 28;
+    p.block_table = block_table; p.table_stride = table_stride; p.page_shift = log2_of(page_size); p.num_pages = num_pages; p.most_tokens = most;
+    const int ctas = attention_ctas(G, most);
+    if (Hkv == 8) r = bits == 4 ? launch_attention_t<4, 8, 1, true>(tmK, tmV, p, ctas, cs(s), use_pdl()) : launch_attention_t<2, 8, 1, true>(tmK, tmV, p, ctas, cs(s), use_pdl());
+    else r = bits == 4 ? launch_attention_t<4, 4, 1, true>(tmK, tmV, p, ctas, cs(s), use_pdl()) : launch_attention_t<2, 4, 1, true>(tmK, tmV, p, ctas, cs(s), use_pdl());
+    if (r != TQ_OK) return r;
+    MergeLayerParams m{};
+    m.partials = p.partials; m.positions = seq_lens; m.rotation_t = fw.rot_t; m.out = (__half*)out; m.G = G; m.H = H; m.q_dim = out_stride;
+    m.workers = ctas * ATTN_GROUPS; m.most_tokens = most;
+    return launch_merge_layer<true>(m, cs(s), use_pdl());
+}
+
+}  // extern "C"

@@ -1,0 +1,305 @@
+// Paged packed caches, sm_100a: block tables and slot maps from request lengths, and rows of a slot map back as vectors.
+//
+// A cache array is the packed one of the other kernels ([rows][kv_dim / codes per byte], norms [rows][KV heads]) cut into pages of
+// 1 << page_shift consecutive rows; request g's token t is row table[g][t >> page_shift] << page_shift plus t's place in the page.
+// The writes into such a cache are the append kernels' (tq_layer_prep.cuh, tq_prefill_tc.cuh, SLOTS), the attention of single tokens is
+// the decode kernels' (tq_attention.cuh, tq_decode_cluster.cuh, PAGED).
+#pragma once
+
+#include "tq_prefill_fa.cuh"
+
+namespace tq {
+
+// ---- block tables and slot maps -----------------------------------------------------------------------------------------------------
+// With c the tokens that request g holds (0 where it has ended), n its new ones, P the page size:
+//   pages back      ceil(old / P) of every ended request, in order, on top of the stack of free pages;
+//   pages taken     need = ceil((c + n) / P) - ceil(c / P); the k-th page of the call, in the order of requests, is the k-th from the top;
+//   admitted        c + n fits the table, and nothing is wanted, or the slot map holds it and (no page is wanted, or the pages wanted
+//                   up to and including it are there).  A request that does not fit the table counts for no page;
+//   token t         of the slot map belongs to the request whose range of running sums of n holds t.
+// Three running sums over the requests, then scattered writes of a few bytes each: bound by latency (a trip for the lengths, one for the
+// table entries and free pages, one for the stores), so one CTA does the bookkeeping, and the slot map too where it is short.  A long map
+// is filled by a second launch over all SMs, which takes lengths and starts from the first.
+struct PagePlanParams {
+    int* table;                      // [G][width], rows table_stride apart
+    int* free_pages;                 // the stack: [num_pages]
+    const int* free_count;
+    int* free_count_out;
+    const int* context;              // [G] tokens held; ~tokens of a request that was not admitted
+    const int* new_tokens;           // [G]
+    const unsigned char* finished;   // [G] or null
+    int* lens;                       // [G]
+    int* start;                      // [G + 1]
+    long long* slots;                // [T]
+    int* positions;                  // [T] or null
+    int G, T, num_pages, table_stride, width, page_shift;
+};
+
+constexpr int PLAN_THREADS = 1024;
+constexpr int PLAN_ONE_LAUNCH = 4096;  // slots that the first launch writes itself
+
+// Token t of the slot map is request a's, start[a] <= t < start[a + 1].
+constexpr int SLOTS_THREADS = 256, SLOTS_SHARED = 8192;  // starts that are searched in shared memory
+static __global__ void __launch_bounds__(SLOTS_THREADS) page_slots_kernel(const PagePlanParams p) {
+    __shared__ int start_s[SLOTS_SHARED];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int* start = p.start;
+    if (p.G < SLOTS_SHARED) {
+        for (int i = threadIdx.x; i <= p.G; i += SLOTS_THREADS) start_s[i] = p.start[i];
+        __syncthreads();
+        start = start_s;
+    }
+    const int used = start[p.G];
+    for (int t = blockIdx.x * SLOTS_THREADS + threadIdx.x; t < p.T; t += gridDim.x * SLOTS_THREADS) {
+        long long slot = -1;
+        int pos = -1;
+        if (t < used) {
+            int a = 0, b = p.G;
+            while (b - a > 1) {
+                const int mid = (a + b) >> 1;
+                if (start[mid] <= t) a = mid;
+                else b = mid;
+            }
+            const int len = p.lens[a];
+            if (len > 0) {  // (a request that was not admitted: negative)
+                pos = len - (start[a + 1] - t);
+                slot = ((long long)p.table[(size_t)a * p.table_stride + (pos >> p.page_shift)] << p.page_shift) + (pos & ((1 << p.page_shift) - 1));
+            }
+        }
+        p.slots[t] = slot;
+        if (p.positions) p.positions[t] = pos;
+    }
+}
+
+static __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(const PagePlanParams p) {
+    __shared__ long long sums[2][PLAN_THREADS / 32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    pdl_launch_dependents();
+    pdl_wait();
+    const int P1 = (1 << p.page_shift) - 1;
+    auto pages_of = [&](long long tokens) { return (int)((tokens + P1) >> p.page_shift); };
+    // running sums over the threads: of `a` before this thread's own, and of all
+    auto scan = [&](long long a, int buf, long long& all) {
+        long long incl = a;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += v;
+        }
+        if (lane == 31) sums[buf][warp] = incl;
+        __syncthreads();
+        long long s = lane < PLAN_THREADS / 32 ? sums[buf][lane] : 0, before = 0;
+        before = lane < warp ? s : 0;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            s += __shfl_xor_sync(0xffffffffu, s, o);
+            before += __shfl_xor_sync(0xffffffffu, before, o);
+        }
+        all = s;
+        __syncthreads();  // (the buffer may be written again)
+        return before + incl - a;
+    };
+    auto held = [&](int g) {
+        const int c = p.context[g];
+        return c < 0 ? ~c : c;
+    };
+    long long have = min(max(*p.free_count, 0), p.num_pages);
+    // ---- pages of ended requests ----
+    if (p.finished) {
+        for (int base = 0; base < p.G; base += PLAN_THREADS) {
+            const int g = base + tid;
+            const bool ended = g < p.G && p.finished[g] != 0;
+            if (!__syncthreads_or(ended)) continue;
+            const int back = ended ? min(pages_of(held(g)), p.width) : 0;
+            long long all;
+            const long long at = have + scan(back, 0, all);
+            // (a warp takes its lanes' rows in turn)
+            unsigned rows = __ballot_sync(0xffffffffu, back > 0);
+            while (rows) {
+                const int l = __ffs((int)rows) - 1;
+                rows &= rows - 1u;
+                const int n = __shfl_sync(0xffffffffu, back, l);
+                const long long to = __shfl_sync(0xffffffffu, at, l);
+                const int* const row = p.table + (size_t)(base + 32 * warp + l) * p.table_stride;
+                for (int j = lane; j < n; j += 32)
+                    if (to + j < p.num_pages) p.free_pages[to + j] = row[j];  // (a stack that is full takes no more)
+            }
+            have = min(have + all, (long long)p.num_pages);
+        }
+        __syncthreads();  // (the stack's new entries, and the rows that new tokens may now replace)
+    }
+    // ---- new tokens ----
+    long long wanted = 0, tokens = 0, taken = 0;
+    for (int base = 0; base < p.G; base += PLAN_THREADS) {
+        const int g = base + tid;
+        long long c = 0, n = 0;
+        if (g < p.G) {
+            c = p.finished && p.finished[g] != 0 ? 0 : held(g);
+            n = max(p.new_tokens[g], 0);
+        }
+        const bool fits = c + n <= (long long)p.width << p.page_shift;
+        const int first = pages_of(c), need = fits ? pages_of(c + n) - first : 0;
+        long long all_pages, all_tokens;
+        const long long k = wanted + scan(need, 0, all_pages);
+        const long long t = tokens + scan(n, 1, all_tokens);
+        const bool ok = fits && (n == 0 || (t + n <= p.T && (need == 0 || k + need <= have)));
+        if (g < p.G) {
+            p.lens[g] = ok ? (int)(c + n) : ~(int)min(c, 0x7fffffffll);
+            p.start[g] = (int)min(t, (long long)p.T);
+            if (g == p.G - 1) p.start[p.G] = (int)min(t + n, (long long)p.T);
+        }
+        unsigned rows = __ballot_sync(0xffffffffu, ok && need > 0);
+        while (rows) {
+            const int l = __ffs((int)rows) - 1;
+            rows &= rows - 1u;
+            const int m = __shfl_sync(0xffffffffu, need, l), j0 = __shfl_sync(0xffffffffu, first, l);
+            const long long from = have - 1 - __shfl_sync(0xffffffffu, k, l);
+            int* const row = p.table + (size_t)(base + 32 * warp + l) * p.table_stride + j0;
+            for (int j = lane; j < m; j += 32) row[j] = p.free_pages[from - j];
+        }
+        if (p.T <= PLAN_ONE_LAUNCH) {
+            // token i of a request: its page is in the table already, or on the stack
+            auto put = [&](bool ok, int g, int c, int i, long long t, int first, long long top) {
+                if (t + i >= p.T) return;
+                const int pos = c + i, j = pos >> p.page_shift;
+                if (ok) {
+                    const int page = j < first ? p.table[(size_t)g * p.table_stride + j] : p.free_pages[top - (j - first)];
+                    p.slots[t + i] = ((long long)page << p.page_shift) + (pos & P1);
+                } else {
+                    p.slots[t + i] = -1;
+                }
+                if (p.positions) p.positions[t + i] = ok ? pos : -1;
+            };
+            if (n == 1) put(ok, g, (int)c, 0, t, first, have - 1 - k);
+            unsigned more = __ballot_sync(0xffffffffu, n > 1 && t < p.T);  // (a warp takes its lanes' requests in turn)
+            while (more) {
+                const int l = __ffs((int)more) - 1;
+                more &= more - 1u;
+                const bool ok_l = __shfl_sync(0xffffffffu, ok, l);
+                const int c_l = __shfl_sync(0xffffffffu, (int)c, l), first_l = __shfl_sync(0xffffffffu, first, l);
+                const long long t_l = __shfl_sync(0xffffffffu, t, l), k_l = __shfl_sync(0xffffffffu, k, l);
+                const int n_l = (int)min(__shfl_sync(0xffffffffu, n, l), p.T - t_l);
+                for (int i = lane; i < n_l; i += 32) put(ok_l, base + 32 * warp + l, c_l, i, t_l, first_l, have - 1 - k_l);
+            }
+        }
+        long long got;
+        scan(ok ? need : 0, 0, got);
+        taken += got;
+        wanted += all_pages;
+        tokens += all_tokens;
+    }
+    if (tid == 0) *p.free_count_out = (int)(have - taken);
+    if (p.T > PLAN_ONE_LAUNCH) return;
+    for (long long t = tokens + tid; t < p.T; t += PLAN_THREADS) {
+        p.slots[t] = -1;
+        if (p.positions) p.positions[t] = -1;
+    }
+}
+
+// ---- rows of a slot map as vectors ------------------------------------------------------------------------------------------------------
+// out[t][h] = norm * R^T c, c the centroids of row slots[t], head h (zeros where the slot is no row).  Vectors are the M dimension, 64 at a
+// time, of mma.sync: a warp owns 16 output coordinates, whose part of R stays in its registers; the centroids go through shared memory.
+struct PagedReadParams {
+    const uint8_t* ck;
+    const __half* kn;
+    const uint8_t* cv;
+    const __half* vn;
+    const __half* rotation;      // R row-major
+    const long long* slots;      // [T]
+    __half* k_out;               // [T][stride]
+    __half* v_out;
+    long long total_rows, stride;
+    int T, Hkv;
+};
+constexpr int READ_THREADS = 256, READ_VECTORS = 64;
+
+template <int BITS>
+__global__ void __launch_bounds__(READ_THREADS, 2) paged_read_kernel(const PagedReadParams p) {
+    constexpr int BPH = HEAD_DIM * BITS / 8, ENTRIES = BITS == 4 ? 256 : 16;
+    __shared__ uint32_t lut[ENTRIES * 8];
+    __shared__ __align__(16) __half a_s[READ_VECTORS][HEAD_DIM + 8];
+    __shared__ float norm_s[READ_VECTORS];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gl = lane >> 2, t4 = lane & 3;
+    for (int i = tid; i < ENTRIES * 8; i += READ_THREADS) {
+        const int e = i >> 3;
+        lut[i] = BITS == 4 ? pack_half2(kCent4[e & 15], kCent4[(e >> 4) & 15]) : pack_half2(kCent2[e & 3], kCent2[(e >> 2) & 3]);
+    }
+    pdl_launch_dependents();
+    pdl_wait();
+    // B fragments: coordinates n = 16 warp + 8 i + gl, k = 16 j + 2 t4, + 1 (+ 8); R passes through the operand's place, 64 rows at a time
+    uint32_t bf[2][8][2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int at = tid + READ_THREADS * i;
+            *reinterpret_cast<uint4*>(&a_s[at >> 4][8 * (at & 15)]) = reinterpret_cast<const uint4*>(p.rotation)[1024 * half + at];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint32_t r[4];
+            ldmatrix_x4_trans(r, smem_u32(&a_s[16 * j + (lane & 15)][16 * warp + 8 * (lane >> 4)]));
+            bf[0][4 * half + j][0] = r[0]; bf[0][4 * half + j][1] = r[1];
+            bf[1][4 * half + j][0] = r[2]; bf[1][4 * half + j][1] = r[3];
+        }
+    }
+    const long long per_kind = (long long)p.T * p.Hkv, tiles = (per_kind + READ_VECTORS - 1) / READ_VECTORS;
+    for (long long tile = blockIdx.x; tile < 2 * tiles; tile += gridDim.x) {
+        const bool is_v = tile >= tiles;
+        const long long v0 = (is_v ? tile - tiles : tile) * READ_VECTORS;
+        __syncthreads();  // (table; the last tile's operand has been read)
+        {
+            const long long v = v0 + (tid >> 2), t = v / p.Hkv;  // four threads a vector, 32 coordinates each
+            const int h = (int)(v - t * p.Hkv), copy = tid & 7;
+            const long long row = v < per_kind ? p.slots[t] : -1;
+            const bool on = row >= 0 && row < p.total_rows;
+            uint32_t w[4] = {0u, 0u, 0u, 0u};
+            if (on) {
+                const uint8_t* const src = (is_v ? p.cv : p.ck) + ((size_t)row * p.Hkv + h) * BPH + (BPH / 4) * (tid & 3);
+                if (BITS == 4) {
+                    const uint4 u = *reinterpret_cast<const uint4*>(src);
+                    w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+                } else {
+                    const uint2 u = *reinterpret_cast<const uint2*>(src);
+                    w[0] = u.x & 0xffffu; w[1] = u.x >> 16; w[2] = u.y & 0xffffu; w[3] = u.y >> 16;
+                }
+            }
+            if ((tid & 3) == 0) norm_s[tid >> 2] = on ? __half2float((is_v ? p.vn : p.kn)[(size_t)row * p.Hkv + h]) : 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint4 u;
+                constexpr uint32_t M = ENTRIES - 1, W = BITS == 4 ? 8 : 4;
+                u.x = lut[(w[i] & M) * 8 + copy]; u.y = lut[((w[i] >> W) & M) * 8 + copy];
+                u.z = lut[((w[i] >> (2 * W)) & M) * 8 + copy]; u.w = lut[((w[i] >> (3 * W)) & M) * 8 + copy];
+                *reinterpret_cast<uint4*>(&a_s[tid >> 2][32 * (tid & 3) + 8 * i]) = u;
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int m = 0; m < READ_VECTORS / 16; ++m) {
+            float c[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                uint32_t a[4];
+                ldmatrix_x4(a, smem_u32(&a_s[16 * m + (lane & 15)][16 * j + 8 * (lane >> 4)]));
+#pragma unroll
+                for (int i = 0; i < 2; ++i) mma16816(c[i], a[0], a[1], a[2], a[3], bf[i][j][0], bf[i][j][1]);
+            }
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int at = 16 * m + gl + 8 * r;
+                const long long v = v0 + at, t = v / p.Hkv;
+                if (v >= per_kind) continue;
+                const float n = norm_s[at];
+                __half* const dst = (is_v ? p.v_out : p.k_out) + t * p.stride + (v - t * p.Hkv) * HEAD_DIM + 16 * warp + 2 * t4;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) *reinterpret_cast<__half2*>(dst + 8 * i) = __floats2half2_rn(c[i][2 * r] * n, c[i][2 * r + 1] * n);
+            }
+        }
+    }
+}
+
+}  // namespace tq

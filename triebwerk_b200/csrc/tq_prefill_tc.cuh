@@ -130,6 +130,7 @@ struct PrefillTcParams {
     __half* v16;
     float* norms;
     int norm_tiles;
+    long long total_rows;      // SLOTS: rows of the cache arrays
     __half* k_post;            // [vectors][128] like k_buf: receives the produced K vectors (what the reference's k buffer
                                // holds after its two kernels); the exact chains of near-bound coordinates re-read them
 };
@@ -289,7 +290,8 @@ __device__ __forceinline__ uint32_t tc_operand_addr(uint32_t tile, int row, int 
 // ROWS16: the prompt's rows as fp16 centroids and its norms as floats too, for the attention behind this launch: one launch and one
 // pass over the codes less where the prompt is short enough for those to count (whole prompts from position 0; Hkv divides 8, a
 // tile's tokens are of one prompt).
-template <bool PRODUCER, bool TMA_IN, bool ROWS16 = false>
+// SLOTS: every token is a "sequence" of its own (T = 1) and goes to row row_base[token]; one outside 0 .. total_rows - 1 is not stored.
+template <bool PRODUCER, bool TMA_IN, bool ROWS16 = false, bool SLOTS = false>
 __global__ void __launch_bounds__(TC_THREADS, PRODUCER || ROWS16 ? 2 : TC_CTAS_PER_SM)  // (these need more registers, shared memory)
 prefill_append_tc_kernel(const __grid_constant__ CUtensorMap tm_k_in, const __grid_constant__ CUtensorMap tm_v_in, const PrefillTcParams p) {
     static_assert(!ROWS16 || TMA_IN, "a tile of whole tokens");
@@ -409,7 +411,7 @@ prefill_append_tc_kernel(const __grid_constant__ CUtensorMap tm_k_in, const __gr
     // divisions and range checks of the general case once per tile and vector, a third of a CTA's time went into bookkeeping.)
     const int TPT = TMA_IN ? TC_TILE / p.Hkv : 0;
     const int dtok = TMA_IN && settle_v >= 0 ? settle_v / p.Hkv : 0, dhead = TMA_IN && settle_v >= 0 ? settle_v - dtok * p.Hkv : 0;
-    const bool plain_positions = TMA_IN && p.step_G == 0 && !p.positions;
+    const bool plain_positions = TMA_IN && !SLOTS && p.step_G == 0 && !p.positions;
 
     fence_proxy_async_smem();
     tc_fence_before();
@@ -599,6 +601,16 @@ prefill_append_tc_kernel(const __grid_constant__ CUtensorMap tm_k_in, const __gr
             const long long row = (p.row_base ? p.row_base[seq0] : p.token_row0 + (long long)seq0 * p.seq_stride_rows) + pos0 + dtok;
             my_norm = row * p.Hkv + dhead;
             my_dst = my_norm * bpv;
+        } else if (SLOTS) {
+            if (settle_v >= 0 && vec0 + settle_v < vec_per_kind) {
+                int tok, head;
+                split_vec(settle_v, tok, head);
+                const long long row = p.row_base[tok];
+                if (row >= 0 && row < p.total_rows) {
+                    my_norm = row * p.Hkv + head;
+                    my_dst = my_norm * bpv;
+                }
+            }
         } else if (settle_v >= 0 && vec0 + settle_v < vec_per_kind) {
             int tok, head, seq, t, layer = 0;
             split_vec(settle_v, tok, head);

@@ -131,3 +131,50 @@ def decode_attention(out, ck_q, cv_q, k_norms, v_norms, rotation, positions, max
 
 def workspace_status(workspace) -> int:
     return int(lib().tq_workspace_status(_ptr(workspace), _stream()))
+
+
+# ---- paged packed caches ---------------------------------------------------------------------------------------------
+# Cache arrays as above ([rows][...] with rows = pages * page_size), block tables int32 [requests, pages] (views of a wider one
+# too), tensors on the current device.  include/triebwerk_b200.h has the full contracts.
+def page_plan(block_table, free_pages, free_count, free_count_out, context_lens, new_tokens, finished, page_size, seq_lens,
+              query_start, slots, positions=None):
+    """Block tables and slot maps of one step: pages of `finished` requests back to the pool, pages for new tokens out of it.
+    Fills block_table, seq_lens, query_start, slots, positions, free_count_out; a request that was not admitted gets the
+    length ~(tokens held) and slots of -1."""
+    st = hostcall.page_plan(block_table, free_pages, free_count, free_count_out, context_lens, new_tokens, finished, page_size, seq_lens,
+                            query_start, slots, positions)
+    if st:
+        raise TqError(st, "tq_page_plan")
+
+
+def paged_append(ck_q, k_norms, cv_q, v_norms, k_buf, v_buf, rotation, slots, num_kv_heads, bits):
+    """Quantise k_buf, v_buf [T, num_kv_heads * 128] (rows of one stride) into the rows slots [T] (int64; -1: nowhere)."""
+    st = hostcall.paged_append(ck_q, k_norms, cv_q, v_norms, k_buf, v_buf, rotation, slots, num_kv_heads, bits)
+    if st:
+        raise TqError(st, "tq_paged_append")
+
+
+def paged_read(k_out, v_out, ck_q, k_norms, cv_q, v_norms, rotation, slots, num_kv_heads, bits):
+    """The K and V vectors that the rows slots [T] stand for, into k_out, v_out [T, num_kv_heads * 128]."""
+    st = hostcall.paged_read(k_out, v_out, ck_q, k_norms, cv_q, v_norms, rotation, slots, num_kv_heads, bits)
+    if st:
+        raise TqError(st, "tq_paged_read")
+
+
+def paged_workspace(T: int, G: int, num_heads: int, device="cuda") -> torch.Tensor:
+    """Workspace of the paged attentions for T query tokens of G requests; one per stream that they run on."""
+    return torch.empty(int(lib().tq_paged_workspace_bytes(T, G, num_heads)), dtype=torch.uint8, device=device)
+
+
+def paged_decode_attention(out, q, ck_q, cv_q, k_norms, v_norms, rotation, block_table, seq_lens, page_size, num_heads, num_kv_heads, bits,
+                           workspace):
+    """One query token per request, q and out [G, num_heads * 128], over its first seq_lens[g] tokens (none: zeros)."""
+    st = hostcall.paged_decode_attention(out, q, ck_q, cv_q, k_norms, v_norms, rotation, block_table, seq_lens, page_size, num_heads,
+                                         num_kv_heads, bits, workspace)
+    if st:
+        raise TqError(st, "tq_paged_decode_attention")
+
+
+def paged_status() -> int:
+    """Status word of the paged calls on the current device (0 = fine); reading clears it and synchronises the stream."""
+    return int(lib().tq_paged_status(_stream()))
