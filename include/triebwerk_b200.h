@@ -454,6 +454,16 @@ int tq_paged_decode_attention(void* out, const void* q, const uint8_t* ck_q, con
                               const int* seq_lens, int num_pages, int page_size, int G, int num_heads, int num_kv_heads, int head_dim,
                               int q_stride, int out_stride, int bits, void* workspace, size_t workspace_bytes, tq_stream_t s);
 
+/* Causal attention of several new tokens per request (prompts, chunks behind earlier tokens, drafted tokens): the query tokens
+ * query_start[g] .. query_start[g + 1] - 1 (device, [G + 1], ascending from 0, at most T) are the last ones of request g's seq_lens[g] tokens, whose
+ * rows are in the cache already; query i of n stands at position seq_lens[g] - n + i and attends to tokens 0 .. there (none: zeros, so
+ * also where seq_lens[g] is 0 or negative).  Rows of out behind query_start[G] are left as they are.  Up to 128 query heads per KV head. */
+int tq_paged_prefill_attention(void* out, const void* q, const uint8_t* ck_q, const uint8_t* cv_q, const void* k_norms,
+                               const void* v_norms, const void* rotation, const int* block_table, int table_stride, int table_width,
+                               const int* seq_lens, const int* query_start, int num_pages, int page_size, int T, int G, int num_heads,
+                               int num_kv_heads, int head_dim, int q_stride, int out_stride, int bits, void* workspace,
+                               size_t workspace_bytes, tq_stream_t s);
+
 /* Reads (and clears) the status word that all paged calls on the current device share: 0, or a code as tq_workspace_status gives.
  * Synchronises the stream. */
 int tq_paged_status(tq_stream_t s);

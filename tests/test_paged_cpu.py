@@ -55,6 +55,24 @@ def test_no_tokens_is_no_work(name):
     assert rows(name, T=0, k=None, v=None, slots=None) == 0
 
 
+def prefill(**kw):
+    a = dict(out=P, q=P, ck=P, cv=P, kn=P, vn=P, R=P, table=P, stride=8, width=8, lens=P, start=P, pages=16, page=32, T=7, G=4, H=16, Hkv=8, D=128, qs=2048,
+             os=2048, bits=4, ws=P, bytes=1 << 30)
+    a.update(kw)
+    return tq.lib().tq_paged_prefill_attention(*a.values(), None)
+
+
+@pytest.mark.parametrize("change, status", [
+    (dict(start=None), -1), (dict(T=-1), -1), (dict(H=258, Hkv=2, qs=258 * 128, os=258 * 128), -4), (dict(bytes=1000), -3), (dict(ws=None), -3), (dict(lens=None), -1),
+    (dict(table=None), -1), (dict(page=24), -4), (dict(G=0), -1), (dict(bits=0), -1), (dict(q=ODD), -1), (dict(qs=2044), -1)])
+def test_prefill_refuses(change, status):
+    assert prefill(**change) == status
+
+
+def test_prefill_of_no_tokens_is_no_work():
+    assert prefill(T=0) == 0
+
+
 @pytest.mark.parametrize("change, status", [
     (dict(page=16), -4), (dict(page=96), -4), (dict(D=64), -4), (dict(bits=0), -1), (dict(bits=8), -1), (dict(G=0), -1), (dict(H=15), -1), (dict(Hkv=0), -1),
     (dict(H=0), -1), (dict(qs=2040), -1), (dict(qs=2052), -1), (dict(os=2047), -1), (dict(stride=4), -1), (dict(width=0), -1), (dict(pages=0), -1),

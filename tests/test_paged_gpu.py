@@ -357,3 +357,168 @@ def test_python_refusals():
     for bad in ((k, k[:1], slots), (k, k.float(), slots), (k, k, slots.int()), (k, k, slots[:1]), (k, k.cpu(), slots), (k[:, :512], k[:, :512], slots)):
         with pytest.raises((AssertionError, TqError)):
             ops.paged_append(ck, kn, cv, vn, bad[0], bad[1], R, bad[2], 8, 4)
+
+
+# ---- prefill attention ----------------------------------------------------------------------------------------------------------
+def check_prefill(lens, new, H, Hkv, bits, page, seed, tail=3, narrow=False, strided=True):
+    rng = np.random.default_rng(seed)
+    start = [0] + np.cumsum(new).tolist()
+    T = start[-1] + tail
+    table, q, out, ck, cv, kn, vn, R, whole = attention_inputs(rng, lens, H, Hkv, bits, page, T=T, extra_columns=0 if narrow else 1, strided=strided)
+    ws = ops.paged_workspace(T, len(lens), H)
+    ops.paged_prefill_attention(out, q, ck, cv, kn, vn, R, table, i32(lens), i32(start), page, H, Hkv, bits, ws)
+    torch.cuda.synchronize()
+    want = pu.attention(q, ck, cv, kn, vn, R, table, lens, start, page, H, Hkv, bits)
+    pu.assert_attention(out[:start[-1]], (want[0][:start[-1]], want[1][:start[-1]]), f"{bits}-bit {H}/{Hkv} page {page}")
+    for g, n in enumerate(lens):  # queries with nothing in front of them
+        none = out[start[g]:start[g + 1]][:max(0, new[g] - max(n, 0))]
+        assert (none == 0).all()
+    assert (whole[:, H * 128:] == 7).all() and (whole[start[-1]:] == 7).all()
+
+
+@pytest.mark.parametrize("bits", [4, 2])
+@pytest.mark.parametrize("H, Hkv", [(16, 8), (32, 8), (4, 4), (40, 8), (14, 2), (16, 1), (9, 3)])
+@pytest.mark.parametrize("page", [32, 128])
+def test_prefill_small_batches(H, Hkv, bits, page):
+    new = [1, 0, 5, 33, 128, 1, 70, 0, 64]
+    lens = [1, 0, 5, 40, 128, 300, 71, 90, 1000]
+    check_prefill(lens, new, H, Hkv, bits, page, H + Hkv + bits + page)
+    check_prefill([77], [77], H, Hkv, bits, page, 1, tail=0)
+
+
+@pytest.mark.parametrize("bits", [4, 2])
+@pytest.mark.parametrize("H, Hkv", [(16, 8), (32, 8), (32, 4), (40, 8)])
+@pytest.mark.parametrize("page", [32, 64, 256])
+def test_prefill_two_blocks_a_cta(H, Hkv, bits, page):
+    rng = np.random.default_rng(page)
+    new = rng.integers(1, 700, 14).tolist() + [0, 1, 129, 512, 127]
+    lens = [n + c for n, c in zip(new, [0, 0, 1000, 31, 32, 33, 500, 1, 0, 7, 128, 127, 129, 900, 64, 2000, 0, 0, 1])]
+    check_prefill(lens, new, H, Hkv, bits, page, H + Hkv + bits + page)
+
+
+@pytest.mark.parametrize("bits", [4, 2])
+@pytest.mark.parametrize("H, Hkv, new, lens", [(16, 8, [4], [9000]), (32, 8, [1, 5], [5000, 700]), (16, 1, [8, 1, 3], [4000, 1, 3]), (14, 2, [40], [6000]),
+                                               (8, 1, [17], [16001])])
+def test_prefill_cut_along_the_context(H, Hkv, new, lens, bits):
+    check_prefill(lens, new, H, Hkv, bits, 64, sum(lens), tail=2)
+
+
+@pytest.mark.parametrize("bits", [4, 2])
+def test_prefill_rows_without_tokens(bits):
+    # requests not admitted, empty ones, more queries than tokens: zeros
+    check_prefill([-5, 0, 3, 200, -1, 10], [7, 2, 8, 200, 1, 140], 16, 8, bits, 32, 3)
+    check_prefill([0], [300], 16, 8, bits, 32, 4)
+    check_prefill([-9] * 40, [130] * 40, 16, 8, bits, 32, 5)
+    check_prefill([0, 5000], [3, 3], 16, 1, bits, 32, 6)
+
+
+def test_prefill_many_requests():
+    rng = np.random.default_rng(8)
+    new = rng.integers(0, 4, 900)
+    check_prefill((new + rng.integers(0, 60, 900)).tolist(), new.tolist(), 16, 8, 4, 32, 9)
+
+
+def test_prefill_single_tokens_are_a_decode_step():
+    rng = np.random.default_rng(10)
+    lens = rng.integers(1, 900, 20).tolist()
+    check_prefill(lens, [1] * 20, 32, 8, 4, 32, 11, tail=0)
+
+
+@pytest.mark.parametrize("H, Hkv, n, L", [(16, 8, 40, 900), (16, 1, 4, 5000), (16, 8, 600, 600)])
+def test_prefill_captured_on_another_stream(H, Hkv, n, L):
+    rng = np.random.default_rng(12)
+    G = 6
+    lens, start = [L] * G, [n * g for g in range(G + 1)]
+    table, q, out, ck, cv, kn, vn, R, _ = attention_inputs(rng, lens, H, Hkv, 4, 64, T=n * G)
+    d, st = i32(lens), i32(start)
+    ws = ops.paged_workspace(n * G, G, H)
+    call = lambda: ops.paged_prefill_attention(out, q, ck, cv, kn, vn, R, table, d, st, 64, H, Hkv, 4, ws)  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for cut in (lens, [n] * G, [0] * G, [L - 13 * g for g in range(G)]):
+        d.copy_(i32(cut))
+        out.fill_(9.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        pu.assert_attention(out, pu.attention(q, ck, cv, kn, vn, R, table, cut, start, 64, H, Hkv, 4))
+
+
+def test_prefill_norms_that_are_not_finite():
+    # of a later token: nothing of it reaches the earlier ones; of an earlier token: every query behind it
+    rng = np.random.default_rng(13)
+    lens, new, start = [300, 300], [300, 300], [0, 300, 600]
+    for name, value in (("v", float("nan")), ("v", float("inf")), ("k", float("nan"))):
+        table, q, out, ck, cv, kn, vn, R, _ = attention_inputs(rng, lens, 16, 8, 4, 32, T=600)
+        at = pu.rows_of(table[0], 300, 32)[150]
+        (vn if name == "v" else kn)[at, 3] = value
+        ws = ops.paged_workspace(600, 2, 16)
+        ops.paged_prefill_attention(out, q, ck, cv, kn, vn, R, table, i32(lens), i32(start), 32, 16, 8, 4, ws)
+        bad = ~out.isfinite().view(600, 8, 256).all(-1)
+        want = torch.zeros_like(bad)
+        want[150:300, 3] = True
+        assert torch.equal(bad, want)
+
+
+# ---- all together -----------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("bits, H, Hkv, page", [(4, 16, 8, 32), (2, 32, 8, 64), (4, 14, 2, 128)])
+def test_a_serving_loop(bits, H, Hkv, page):
+    """Requests come and go over ten steps: plan, append, attention of prompts and of single tokens, against vectors kept in 64 bits
+    (read back from the cache, whose rows are those of the plan)."""
+    rng = np.random.default_rng(bits + H)
+    G, width, pool = 5, 1024 // page, 4 * 1024 // page
+    R = pu.rotation(4).cuda()
+    (ck, kn), (cv, vn) = (pu.random_cache(rng, pool * page, Hkv, bits) for _ in range(2))
+    table = i32(np.full((G, width), -1))
+    stack, count = i32(rng.permutation(pool)), i32([pool])
+    lens = i32(np.zeros(G))
+    history = [[] for _ in range(G)]  # rows, in order, that each request's tokens went to
+    for step in range(10):
+        ended = np.array([len(h) > 0 and rng.random() < 0.25 for h in history], np.uint8)
+        for g in range(G):
+            if ended[g]:
+                history[g] = []
+        new = np.array([1 if h else int(rng.integers(0, 400)) for h in history])
+        if step % 3 == 1:
+            new = np.where(new == 1, rng.integers(0, 6, G), new)
+        T = int(new.sum()) + 2
+        start, slots, pos = i32(np.zeros(G + 1)), torch.zeros(T, dtype=torch.int64, device="cuda"), i32(np.zeros(T))
+        ops.page_plan(table, stack, count, count, lens, i32(new), torch.from_numpy(ended).cuda(), page, lens, start, slots, pos)
+        qkv = torch.from_numpy(rng.standard_normal((T, (H + 2 * Hkv) * 128)).astype(np.float16)).cuda()
+        q, k, v = qkv[:, :H * 128], qkv[:, H * 128:(H + Hkv) * 128], qkv[:, (H + Hkv) * 128:]
+        ops.paged_append(ck, kn, cv, vn, k, v, R, slots, Hkv, bits)
+        k_back, v_back = torch.empty(T, Hkv * 128, dtype=torch.float16, device="cuda"), torch.empty(T, Hkv * 128, dtype=torch.float16, device="cuda")
+        ops.paged_read(k_back, v_back, ck, kn, cv, vn, R, slots, Hkv, bits)
+        out = torch.full((T, H * 128), 7.0, dtype=torch.float16, device="cuda")
+        ws = ops.paged_workspace(T, G, H)
+        ops.paged_prefill_attention(out, q, ck, cv, kn, vn, R, table, lens, start, page, H, Hkv, bits, ws)
+        torch.cuda.synchronize()
+        at = 0
+        for g in range(G):
+            for t in range(new[g]):
+                assert pos[at] == len(history[g])
+                history[g].append(int(slots[at]))
+                at += 1
+        held = [len(h) for h in history]
+        assert lens.tolist() == held and (slots[at:] == -1).all()
+        rows = sum(history, [])
+        assert len(set(rows)) == len(rows) and int(count) == pool - sum(-(-n // page) for n in held)
+        # quantising keeps most of a vector: the error of the 4-bit code book is 0.0095 of the energy, of the 2-bit one 0.1175
+        if at:
+            for a, b in ((k, k_back), (v, v_back)):
+                off = (a[:at].double() - b[:at].double()).square().sum() / a[:at].double().square().sum()
+                assert off < {4: 0.012, 2: 0.13}[bits]
+        want = pu.attention(q, ck, cv, kn, vn, R, table, held, start.tolist(), page, H, Hkv, bits)
+        pu.assert_attention(out[:at], (want[0][:at], want[1][:at]), f"step {step}")
+        assert (out[at:] == 7).all()
+        if all(n <= 1 for n in new):  # a step of single tokens: the decode call gives the same
+            pick = [int(start[g]) for g in range(G)]
+            qd = q[[min(i, T - 1) for i in pick]].contiguous()
+            one = torch.empty(G, H * 128, dtype=torch.float16, device="cuda")
+            ops.paged_decode_attention(one, qd, ck, cv, kn, vn, R, table, lens, page, H, Hkv, bits, ws)
+            pu.assert_attention(one, pu.attention(qd, ck, cv, kn, vn, R, table, held, list(range(G + 1)), page, H, Hkv, bits))

@@ -28,7 +28,7 @@ SYMBOLS = [
     "tq_engine_output_f32", "tq_engine_read_output_f32", "tq_engine_decode_layers", "tq_static_status", "tq_selftest_bounded_wait",
     "tq_engine_sequence_blob_bytes", "tq_engine_export_sequence", "tq_engine_import_sequence", "tq_engine_sleep_keep", "tq_engine_prefill_shared", "tq_engine_decode_step_produce", "tq_fold_rotation_into_projection",
     "tq_engine_time_attention", "tq_engine_last_attention_ms", "tq_engine_prefill_layer", "tq_engine_prefill_layer_batch", "tq_engine_step_prepare", "tq_engine_step_attend_layers",
-    "tq_page_plan", "tq_paged_append", "tq_paged_read", "tq_paged_workspace_bytes", "tq_paged_decode_attention", "tq_paged_status",
+    "tq_page_plan", "tq_paged_append", "tq_paged_read", "tq_paged_workspace_bytes", "tq_paged_decode_attention", "tq_paged_prefill_attention", "tq_paged_status",
     "tq_peer_buffer_create", "tq_peer_buffer_open", "tq_peer_buffer_close", "tq_peer_buffer_destroy", "tq_peer_copy", "tq_peer_signal", "tq_peer_wait",
 ]
 
@@ -117,6 +117,7 @@ def lib() -> C.CDLL:
     sig("tq_paged_read", i, [vp, vp, vp, vp, vp, vp, vp, vp, ll, i, i, i, ll, i, vp])
     sig("tq_paged_workspace_bytes", sz, [i, i, i])
     sig("tq_paged_decode_attention", i, [vp, vp, vp, vp, vp, vp, vp, vp, i, i, vp, i, i, i, i, i, i, i, i, i, vp, sz, vp])
+    sig("tq_paged_prefill_attention", i, [vp, vp, vp, vp, vp, vp, vp, vp, i, i, vp, vp, i, i, i, i, i, i, i, i, i, i, vp, sz, vp])
     sig("tq_paged_status", i, [vp])
     sig("tq_peer_buffer_create", i, [sz, C.POINTER(vp), vp])
     sig("tq_peer_buffer_open", i, [vp, C.POINTER(vp)])

@@ -298,6 +298,17 @@ PyObject* paged_decode_attention(PyObject*, PyObject* const* args, Py_ssize_t n)
     });
 }
 
+PyObject* paged_prefill_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return paged_call(args, n, 15, [](const Args& a, tq_stream_t s) {
+        const AttentionArgs p = attention_args(a, 10);
+        const int* const start = a.flat(9, at::kInt, p.G + 1ll, "query_start: int32 [requests + 1]").data_ptr<int>();
+        return unlocked([&] {
+            return tq_paged_prefill_attention(p.out, p.q, p.c.ck, p.c.cv, p.c.kn, p.c.vn, p.R, p.table, p.stride, p.width, p.lens, start, p.pages, p.page, p.T,
+                                              p.G, p.H, p.Hkv, 128, p.q_stride, p.out_stride, p.bits, p.ws, p.ws_bytes, s);
+        });
+    });
+}
+
 #define TQ_CALL(name, need) {#name, (PyCFunction)(void (*)(void))Call<&name, need>::py, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {
     TQ_CALL(tq_engine_decode_layer, Need::Half),
@@ -318,6 +329,7 @@ PyMethodDef methods[] = {
     {"page_plan", (PyCFunction)(void (*)(void))page_plan, METH_FASTCALL, nullptr},
     {"paged_append", (PyCFunction)(void (*)(void))paged_rows<&tq_paged_append, 4, 0>, METH_FASTCALL, nullptr},
     {"paged_read", (PyCFunction)(void (*)(void))paged_rows<&tq_paged_read, 0, 2>, METH_FASTCALL, nullptr},
+    {"paged_prefill_attention", (PyCFunction)(void (*)(void))paged_prefill_attention, METH_FASTCALL, nullptr},
     {"paged_decode_attention", (PyCFunction)(void (*)(void))paged_decode_attention, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 

@@ -3,6 +3,7 @@
 
 #include "tq_host.cuh"
 #include "tq_paged.cuh"
+#include "tq_paged_prefill.cuh"
 
 using namespace tq;
 
@@ -144,9 +145,31 @@ int tq_paged_read(void* k_out, void* v_out, const uint8_t* ck_q, const void* k_n
                      : launch_kernel(paged_read_kernel<2>, grid, dim3(READ_THREADS), 0, cs(s), use_pdl(), p);
 }
 
+}  // extern "C"
+
+// How a prefill call's work is cut: blocks per CTA (MT) and parts of a block's tiles.  The host knows the tokens of all requests
+// together, so it goes by their mean.
+struct PrefillCut {
+    int mt, splits;
+};
+constexpr int SPLIT_SMS = 160, MAX_SPLITS = 16;
+static PrefillCut prefill_cut(int T, int G, int H, int Hkv, int most) {
+    const long long sms = std::min(device_props().sm_count, SPLIT_SMS), qt = PFT_ROWS / (H / Hkv), mean = (T + G - 1) / G;
+    const long long blocks1 = (long long)Hkv * G * ((mean + qt - 1) / qt), blocks2 = (long long)Hkv * G * ((mean + 2 * qt - 1) / (2 * qt));
+    if (mean > qt && 4 * blocks2 >= 5 * sms) return {2, 1};
+    const long long tiles = (most + PFT_KT - 1) / PFT_KT;
+    const long long splits = std::min({sms / std::max(blocks1, 1ll), tiles / 4, (long long)MAX_SPLITS});
+    return {1, (int)std::max(splits, 1ll)};
+}
+// Rows of partial sums that split calls write: splits * T * H, where splits * blocks1 <= the SMs and T * H <= 128 rows a block... and at
+// most MAX_SPLITS of T * H.
+static size_t split_rows(int T, int H) { return (size_t)std::min<long long>((long long)MAX_SPLITS * T * H, (long long)SPLIT_SMS * PFT_ROWS); }
+
+extern "C" {
+
 size_t tq_paged_workspace_bytes(int T, int G, int num_heads) {
     if (T < 0 || G <= 0 || num_heads <= 0) return 0;
-    return carve_full(nullptr, G, num_heads).bytes;
+    return std::max(carve_full(nullptr, G, num_heads).bytes, split_rows(T, num_heads) * PART_STRIDE * sizeof(float));
 }
 
 // What both attentions check of their arguments.
@@ -212,6 +235,73 @@ int tq_paged_decode_attention(void* out, const void* q, const uint8_t* ck_q, con
     m.partials = p.partials; m.positions = seq_lens; m.rotation_t = fw.rot_t; m.out = (__half*)out; m.G = G; m.H = H; m.q_dim = out_stride;
     m.workers = ctas * ATTN_GROUPS; m.most_tokens = most;
     return launch_merge_layer<true>(m, cs(s), use_pdl());
+}
+
+}  // extern "C"
+
+template <int BITS, int MT, bool SPLIT>
+static int launch_paged_prefill(const CUtensorMap& tmQ, const CUtensorMap& tmR, const PagedPrefillParams& p, dim3 grid, cudaStream_t s) {
+    auto kernel = paged_prefill_kernel<BITS, MT, SPLIT>;
+    int r = ensure_dynamic_smem((const void*)kernel, PpfSmem::BYTES);
+    if (r != TQ_OK) return r;
+    // the register split inside the kernel draws on what the launch brings: never launch with less
+    static const int regs = [] {
+        cudaFuncAttributes a{};
+        return cudaFuncGetAttributes(&a, (const void*)paged_prefill_kernel<BITS, MT, SPLIT>) == cudaSuccess ? a.numRegs : 0;
+    }();
+    if (regs < PPF_REGS_LAUNCH) return TQ_ERR_UNSUPPORTED;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(PPF_THREADS);
+    cfg.dynamicSmemBytes = PpfSmem::BYTES;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = use_pdl() ? 1 : 0;
+    return cuda_status(cudaLaunchKernelEx(&cfg, kernel, tmQ, tmR, p));
+}
+
+extern "C" {
+
+int tq_paged_prefill_attention(void* out, const void* q, const uint8_t* ck_q, const uint8_t* cv_q, const void* k_norms, const void* v_norms,
+                               const void* rotation, const int* block_table, int table_stride, int table_width, const int* seq_lens,
+                               const int* query_start, int num_pages, int page_size, int T, int G, int num_heads, int num_kv_heads, int head_dim,
+                               int q_stride, int out_stride, int bits, void* workspace, size_t workspace_bytes, tq_stream_t s) {
+    int r = check_attention(out, q, ck_q, cv_q, k_norms, v_norms, rotation, block_table, table_stride, table_width, seq_lens, num_pages, page_size, G,
+                            num_heads, num_kv_heads, head_dim, q_stride, out_stride, bits);
+    if (r != TQ_OK) return r;
+    if (T < 0 || !query_start) return TQ_ERR_ARG;
+    const int H = num_heads, Hkv = num_kv_heads, grp = H / Hkv, most = table_width * page_size;
+    if (!prefill_attn_shape(H, Hkv)) return TQ_ERR_UNSUPPORTED;
+    if (!workspace || workspace_bytes < tq_paged_workspace_bytes(T, G, H) || !aligned({workspace}, 256)) return TQ_ERR_WORKSPACE;
+    if (T == 0) return TQ_OK;
+    const PrefillCut cut = prefill_cut(T, G, H, Hkv, most);
+    const int qt = PFT_ROWS / grp, bt = cut.mt * qt;
+    const long long ctas = (long long)Hkv * (T / bt + (long long)G);
+    if (ctas >= (1ll << 31)) return TQ_ERR_UNSUPPORTED;
+    PagedPrefillParams p{};
+    p.ck = ck_q; p.cv = cv_q; p.kn = (const __half*)k_norms; p.vn = (const __half*)v_norms;
+    p.block_table = block_table; p.lens = seq_lens; p.start = query_start; p.out = (__half*)out; p.partials = (float*)workspace;
+    r = paged_status_word(&p.status);
+    if (r != TQ_OK) return r;
+    p.table_stride = table_stride; p.page_shift = log2_of(page_size); p.num_pages = num_pages; p.most_tokens = most;
+    p.T = T; p.G = G; p.H = H; p.Hkv = Hkv; p.grp = grp; p.out_stride = out_stride;
+    CUtensorMap tmQ, tmR;
+    r = make_prefill_query_map(&tmQ, q, T, H, grp, qt, q_stride);
+    if (r == TQ_OK) r = make_prefill_rows_map(&tmR, rotation, HEAD_DIM, HEAD_DIM);
+    if (r != TQ_OK) return r;
+    const dim3 grid((unsigned)ctas, 1, (unsigned)cut.splits);
+    if (cut.mt == 2) return bits == 4 ? launch_paged_prefill<4, 2, false>(tmQ, tmR, p, grid, cs(s)) : launch_paged_prefill<2, 2, false>(tmQ, tmR, p, grid, cs(s));
+    if (cut.splits == 1) return bits == 4 ? launch_paged_prefill<4, 1, false>(tmQ, tmR, p, grid, cs(s)) : launch_paged_prefill<2, 1, false>(tmQ, tmR, p, grid, cs(s));
+    r = bits == 4 ? launch_paged_prefill<4, 1, true>(tmQ, tmR, p, grid, cs(s)) : launch_paged_prefill<2, 1, true>(tmQ, tmR, p, grid, cs(s));
+    if (r != TQ_OK) return r;
+    PagedMergeParams m{};
+    m.partials = p.partials; m.rotation = (const __half*)rotation; m.start = query_start; m.out = p.out; m.splits = cut.splits;
+    m.T = T; m.G = G; m.H = H; m.out_stride = out_stride;
+    const long long pieces = ((long long)T * H + 15) / 16;
+    return launch_kernel(paged_merge_kernel, dim3((unsigned)std::min<long long>(pieces, 4ll * device_props().sm_count)), dim3(256), 0, cs(s), use_pdl(), m);
 }
 
 }  // extern "C"

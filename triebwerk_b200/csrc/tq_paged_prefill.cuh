@@ -1,0 +1,716 @@
+// Causal attention of several new tokens per request over paged packed caches (tcgen05 + tensor memory), sm_100a.
+//
+// Query i of request g, of its n new tokens, stands at position p = L - n + i of its L tokens and attends to tokens 0 .. p:
+//   out = R (softmax_t((R^T-rotated q . centroids_K[t]) norm_K[t] / sqrt(128)) . (norm_V[t] centroids_V[t]))
+// with q rotated by R first and one R product at the end (tq_prefill_fa.cuh has the mathematics; the slots, the softmax and the order of
+// products are that kernel's).  What differs: the batch is ragged, requests have earlier tokens, rows come by way of block tables, and the
+// codes become fp16 centroids INSIDE the kernel, so that a call needs no scratch for the contexts, whose lengths the host does not know
+// (16384 tokens and 8 KV heads as fp16 are 64 MB a request), and reads the packed bytes alone.
+//   * A block = 128 score rows = 128 / GRP query tokens x the GRP query heads of a KV head.  MT = 2: a CTA has two blocks, which share
+//     every K and V tile; MT = 1: one block, whose two slots take the even and the odd tiles and are combined at the end.
+//   * The 16 softmax warps are the producers too: a thread fetches 16 (2-bit: 8) bytes of one row of the next K and V tile into registers a
+//     tile ahead (its page's number another tile ahead), and turns them into centroids through a shared-memory table with a column
+//     per lane: K of tile j + 1 before it waits for S(j), V of tile j + 1 after its weights P(j) are out.  So the table look-ups and
+//     operand stores fill the time in which the tensor core works on the slot's own products.
+//   * MT = 2: all 16 warps make a share of every tile.  MT = 1: a slot's warps make that slot's tiles, and nothing ties the slots.
+//   * SPLIT (MT = 1): few query rows, long contexts: the tiles of a block are cut into gridDim.z parts, whose sums meet in
+//     paged_merge_kernel.
+// Blocks are found without a table: request g's blocks begin at floor(start[g] / BT) + g (BT query tokens a CTA), which leaves room for
+// them all; a CTA counts the requests that begin at or before its own number, and one whose block does not exist ends at once.
+// Every wait on a barrier is bounded, as there.
+#pragma once
+
+#include "tq_prefill_fa.cuh"
+
+namespace tq {
+
+struct PagedPrefillParams {
+    const uint8_t* ck;
+    const uint8_t* cv;
+    const __half* kn;
+    const __half* vn;
+    const int* block_table;
+    const int* lens;          // [G]; 0 and less: no token
+    const int* start;         // [G + 1]
+    __half* out;
+    float* partials;          // SPLIT: [splits][T][H][PART_STRIDE]
+    int* status;
+    int table_stride, page_shift, num_pages, most_tokens;
+    int T, G, H, Hkv, grp, out_stride;
+};
+
+constexpr int PPF_THREADS = 32 * PFT_SOFT_WARPS + 128;  // softmax and operands; one warp for the products, three idle (a full warpgroup)
+constexpr int PPF_MEET = 32 * PFT_SOFT_WARPS + 32;      // those that work
+// Registers per thread of the softmax warpgroups and of the last one after the split, out of what the launch brings (the host checks it):
+// 640 x 96 = 512 x 104 + 128 x 64.
+constexpr int PPF_REGS_SOFT = 104, PPF_REGS_REST = 64;
+constexpr int PPF_REGS_LAUNCH = (32 * PFT_SOFT_WARPS * PPF_REGS_SOFT + 128 * PPF_REGS_REST + PPF_THREADS - 1) / PPF_THREADS;
+constexpr int PPF_NSTAGES = 4;                          // of norms: the slots may be that far apart
+struct PpfSmem {
+    static constexpr uint32_t Q = 0;                       // 2 tiles; at the end: high parts of the results
+    static constexpr uint32_t K = 2 * PFT_TILE;            // 2 stages; at the start R in the second; at the end: low parts
+    static constexpr uint32_t V = K + 2 * PFT_TILE;        // 2 stages; at the end R in the first
+    static constexpr uint32_t LUT = V + 2 * PFT_TILE;      // byte (4-bit) or nibble -> two centroids, a column per lane
+    static constexpr uint32_t LUT_BYTES = 32768u;
+    static constexpr uint32_t NORM = LUT + LUT_BYTES;      // [stage]: K norms, V norms as halves, 16 warps' largest V norm; MT = 1, at the end: the slots' maxima and sums
+    static constexpr uint32_t NORM_BYTES = 2u * PFT_KT * 2u + 32u;
+    static constexpr uint32_t CTRL = NORM + PPF_NSTAGES * NORM_BYTES;
+    static constexpr uint32_t BYTES = CTRL + 192u;
+};
+static_assert(PpfSmem::BYTES <= 227 * 1024, "one CTA's shared memory");
+static_assert(PPF_NSTAGES * PpfSmem::NORM_BYTES >= 2 * 128 * 8, "the slots' maxima and sums");
+
+template <int BITS, int MT, bool SPLIT>
+__global__ void __launch_bounds__(PPF_THREADS, 1)
+paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmR, const PagedPrefillParams p) {
+    static_assert(!SPLIT || MT == 1, "few rows");
+    extern __shared__ __align__(1024) uint8_t ppf_smem[];
+    const uint32_t sb = smem_u32(ppf_smem);
+    uint8_t* const gb = ppf_smem;
+    if ((sb & 1023u) != 0u) {
+        if (threadIdx.x == 0) atomicMax(p.status, ST_SMEM_LAYOUT);
+        return;
+    }
+    constexpr int MMA_WARP = PFT_SOFT_WARPS;
+    constexpr int BPH = HEAD_DIM * BITS / 8;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int GRP = p.grp, QT = PFT_ROWS / GRP, BT = MT * QT;
+
+    pdl_launch_dependents();
+    pdl_wait();  // (lengths, tables, caches, queries: all of earlier launches)
+    // ---- the request and the block of this CTA ----
+    const int ny = (int)(gridDim.x / (unsigned)p.Hkv);
+    const int kvh = (int)blockIdx.x % p.Hkv, y = ny - 1 - (int)blockIdx.x / p.Hkv;  // the longest causal prefixes of a request first
+    int g = -1;
+    for (int base = 0; base < p.G; base += PPF_THREADS) {
+        const int i = base + tid;
+        g += __syncthreads_count(i < p.G && p.start[i] / BT + i <= y);
+    }
+    if (g < 0) return;  // (never: request 0 begins at block 0)
+    const int s0 = max(p.start[g], 0), n = min(p.start[g + 1], p.T) - s0, q0 = (y - (s0 / BT + g)) * BT;
+    if (q0 >= n) return;
+    const int L = min(max(p.lens[g], 0), p.most_tokens), pos0 = L - n;  // position of the request's first new token
+    // tiles that the block whose first query is `first` reads
+    auto tiles_to = [&](int first) { return first < n ? max(pos0 + min(first + QT, n) - 1 + PFT_KT, 0) / PFT_KT : 0; };
+    const int t_lo = SPLIT ? (int)((long long)tiles_to(q0) * blockIdx.z / gridDim.z) : 0;
+    const int n_all = (SPLIT ? (int)((long long)tiles_to(q0) * (blockIdx.z + 1) / gridDim.z) : tiles_to(q0)) - t_lo;
+    const int n0 = MT == 2 ? n_all : (n_all + 1) / 2, n1 = MT == 2 ? tiles_to(q0 + QT) : n_all / 2;
+    const int n_tiles = MT == 2 ? max(n0, n1) : n_all;
+    auto tile_of = [&](int s, int i) { return MT == 2 ? i : 2 * i + s; };  // (behind t_lo)
+
+    const uint32_t ctrl = sb + PpfSmem::CTRL;
+    const uint32_t bar_kfull = ctrl, bar_vfull = ctrl + 16u, bar_kfree = ctrl + 32u, bar_vfree = ctrl + 48u;  // [2] each
+    const uint32_t bar_sfull = ctrl + 64u, bar_pfull = ctrl + 80u;                                            // [2 slots] each
+    const uint32_t bar_rot = ctrl + 96u, bar_done = ctrl + 104u, bar_q = ctrl + 112u, bar_r = ctrl + 120u;
+    volatile uint32_t* const tmem_slot = reinterpret_cast<volatile uint32_t*>(gb + PpfSmem::CTRL + 128);
+    bool dead = false;
+    auto wait_bar = [&](uint32_t bar, uint32_t parity) {
+        if (!dead && !mbar_try_wait(bar, parity) && !mbar_wait_bounded_hint(bar, parity, 1u << 17, 2000u)) {
+            dead = true;
+            atomicMax(p.status, ST_TMA_WAIT_TIMEOUT);
+        }
+    };
+    constexpr int MAKERS = MT == 2 ? PFT_SOFT_WARPS : PFT_SOFT_WARPS / 2;  // warps that make a tile
+    if (warp == 0) {
+        tmem_alloc(ctrl + 128u, 512u);
+        tmem_relinquish();
+    }
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(bar_kfull + 8u * i, MAKERS);
+            mbar_init(bar_vfull + 8u * i, MAKERS);
+            mbar_init(bar_kfree + 8u * i, 1);
+            mbar_init(bar_vfree + 8u * i, 1);
+            mbar_init(bar_sfull + 8u * i, 1);
+            mbar_init(bar_pfull + 8u * i, 16 * PFT_SOFT_WARPS);
+        }
+        mbar_init(bar_rot, 1);
+        mbar_init(bar_done, 1);
+        mbar_init(bar_q, 1);
+        mbar_init(bar_r, 1);
+        fence_mbar_init();
+    }
+    {
+        constexpr int ENTRIES = BITS == 4 ? 256 : 16;
+        for (int i = tid; i < ENTRIES * 8; i += PPF_THREADS) {  // four lanes' columns at a time
+            const int e = i >> 3;
+            const uint32_t u = BITS == 4 ? pack_half2(kCent4[e & 15], kCent4[(e >> 4) & 15]) : pack_half2(kCent2[e & 3], kCent2[(e >> 2) & 3]);
+            *reinterpret_cast<uint4*>(gb + PpfSmem::LUT + 16u * (uint32_t)i) = make_uint4(u, u, u, u);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (tid == 32 * MMA_WARP) {
+        mbar_arrive_expect_tx(bar_q, (uint32_t)(MT * QT * GRP) * 256u + PFT_TILE);
+        for (int m = 0; m < MT; ++m) {  // (rows of other requests or past the end: a row's garbage stays in that row and is never stored)
+            tma_load_4d(sb + PpfSmem::Q + m * PFT_TILE, &tmQ, bar_q, 0, kvh * GRP, s0 + q0 + m * QT, 0);
+            tma_load_4d(sb + PpfSmem::Q + m * PFT_TILE + PFT_TILE / 2, &tmQ, bar_q, 0, kvh * GRP, s0 + q0 + m * QT, 1);
+        }
+        tma_load_3d(sb + PpfSmem::K + PFT_TILE, &tmR, bar_q, 0, 0, 0);
+    }
+    const uint32_t tmem = *tmem_slot;
+    const int slot = (warp >> 2) & 1, row0 = 32 * (warp & 3) + 16 * (warp >> 3), gl = lane >> 2, t4 = lane & 3;
+    const int my_first = q0 + (MT == 2 ? slot * QT : 0);
+    auto make_by_grp = [&]() {  // row / GRP by a multiplication, exact below 128
+        uint32_t d = (uint32_t)GRP;
+        asm volatile("" : "+r"(d));
+        return (65536u + d - 1u) / d;
+    };
+    auto token_in = [&](int row, uint32_t by_grp) { return (int)(((uint32_t)row * by_grp) >> 16); };
+    auto token_of = [&](int row, uint32_t by_grp) { return token_in(row, by_grp) < QT ? my_first + token_in(row, by_grp) : n; };  // (n: a row of no query)
+    const uint32_t my_lanes = tmem + ((uint32_t)row0 << 16);
+    auto put_frag = [&](uint32_t tile, int c0, const float (&v)[32]) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < 8; j += 4) {
+                auto two = [&](int b) { return pack_half2(v[4 * b + 2 * h], v[4 * b + 2 * h + 1]); };
+                stmatrix_x4(sb + tile + pft_chunk(row0 + 8 * h + (lane & 7), (c0 >> 3) + j + (lane >> 3)), two(j), two(j + 1), two(j + 2), two(j + 3));
+            }
+    };
+    constexpr int PCOLS = MT == 2 ? 128 : 64;
+    const int pcol0 = MT == 2 ? 0 : 64 * slot;
+    const uint32_t pslot = MT == 2 ? (uint32_t)slot : 0u;
+
+    if (warp >= MMA_WARP) {
+      regs_dec<PPF_REGS_REST>();
+      if (warp == MMA_WARP) {
+        // ================= one thread issues every product =================
+        if (lane == 0) {
+            wait_bar(bar_q, 0u);
+            tc_fence_after();
+            if (!dead) {
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int ks = 0; ks < 8; ++ks)
+                        umma_lo(tmem + 128u * m, pft_lo_k(sb + PpfSmem::Q + m * PFT_TILE) + pft_kstep(ks), pft_lo_k(sb + PpfSmem::K + PFT_TILE) + pft_kstep(ks), PFT_IDESC_K, ks != 0);
+            }
+            umma_commit(bar_rot);
+        }
+        __syncwarp();
+        named_barrier(1, PPF_MEET);  // the rotated queries are in place
+        tc_fence_after();
+        if (lane == 0) {
+            auto issue_scores = [&](int s, int i) {
+                const int j = tile_of(s, i), st = j & 1;
+                wait_bar(bar_kfull + 8u * st, (uint32_t)((j >> 1) & 1));
+                tc_fence_after();
+                if (dead) return;
+                const uint32_t a = pft_lo_k(sb + PpfSmem::Q + (MT == 2 ? s * PFT_TILE : 0u)), b = pft_lo_k(sb + PpfSmem::K + st * PFT_TILE);
+#pragma unroll
+                for (int ks = 0; ks < 8; ++ks) umma_lo(tmem + 128u * s, a + pft_kstep(ks), b + pft_kstep(ks), PFT_IDESC_K, ks != 0);
+                umma_commit(bar_sfull + 8u * s);
+                if (MT == 1 || s == (j < n1 ? 1 : 0)) umma_commit(bar_kfree + 8u * st);  // its last reader
+            };
+            auto issue_values = [&](int s, int i) {
+                const int j = tile_of(s, i), st = j & 1;
+                wait_bar(bar_vfull + 8u * st, (uint32_t)((j >> 1) & 1));
+                wait_bar(bar_pfull + 8u * s, (uint32_t)(i & 1));
+                tc_fence_after();
+                if (dead) return;
+                const uint32_t b = pft_lo_mn(sb + PpfSmem::V + st * PFT_TILE);
+#pragma unroll
+                for (int ks = 0; ks < 8; ++ks)
+                    umma_lo_ta(tmem + 256u + 128u * s, tmem + 128u * s + 8u * ks, b + 128u * ks, PFT_IDESC_MN, ks == 0 ? (uint32_t)(i != 0) : 1u);
+                if (MT == 1 || s == (j < n1 ? 1 : 0)) umma_commit(bar_vfree + 8u * st);
+            };
+            if (n0 > 0) issue_scores(0, 0);
+            if (n1 > 0) issue_scores(1, 0);
+            for (int i = 0; i < max(n0, n1); ++i) {
+                if (i < n0) {
+                    issue_values(0, i);
+                    if (i + 1 < n0) issue_scores(0, i + 1);
+                }
+                if (i < n1) {
+                    issue_values(1, i);
+                    if (i + 1 < n1) issue_scores(1, i + 1);
+                }
+            }
+            umma_commit(bar_done);
+            if (!SPLIT) {
+                wait_bar(bar_done, 0u);
+                if (!dead) {
+                    mbar_arrive_expect_tx(bar_r, PFT_TILE);
+                    tma_load_3d(sb + PpfSmem::V, &tmR, bar_r, 0, 0, 0);
+                }
+            }
+        }
+        __syncwarp();
+        if (!SPLIT) {
+            // out[d] = sum_k R[k][d] * acc[k]: the results' high and low parts times R
+            named_barrier(1, PPF_MEET);
+            if (lane == 0) {
+                wait_bar(bar_r, 0u);
+                tc_fence_after();
+                if (!dead) {
+#pragma unroll
+                    for (int m = 0; m < MT; ++m)
+#pragma unroll
+                        for (int part = 0; part < 2; ++part)
+#pragma unroll
+                            for (int ks = 0; ks < 8; ++ks)
+                                umma_lo(tmem + 128u * m, pft_lo_k(sb + (part ? PpfSmem::K : PpfSmem::Q) + m * PFT_TILE) + pft_kstep(ks),
+                                        pft_lo_mn(sb + PpfSmem::V) + 128u * ks, PFT_IDESC_MN, (part | ks) != 0);
+                }
+                umma_commit(bar_rot);
+            }
+            __syncwarp();
+        }
+      }
+    } else {
+        // ================= operands and softmax =================
+        regs_inc<PPF_REGS_SOFT>();
+        // ---- a thread's rows of the tiles: piece mk & 3 of row (mk >> 2) (MT = 1: and of the row 64 further on) ----
+        constexpr int ROWS = MT == 2 ? 1 : 2;
+        const int mk = MT == 2 ? tid : 128 * (warp >> 3) + 32 * (warp & 3) + lane;  // (MT = 1: number among the slot's 256 threads)
+        const int mrow = mk >> 2, piece = mk & 3;
+        const int my_tiles = MT == 2 ? n_tiles : (slot ? n1 : n0);  // tiles that this thread has a share in
+        constexpr int FORMS = 4;                                    // 16-byte pieces of fp16 per share
+        uint4 kc[ROWS], vc[ROWS];                                   // codes of the next tile (2-bit: x, y)
+        unsigned short nrm[ROWS];                                   // piece 0: K norm, piece 1: V norm of the row
+        uint32_t page[ROWS];                                        // of the tile after it
+        const int* const my_pages = p.block_table + (size_t)g * p.table_stride;
+        auto first_token = [&](int i) { return (t_lo + (MT == 2 ? i : 2 * i + slot)) * PFT_KT; };
+        auto fetch_pages = [&](int i) {
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+                const int t = first_token(i) + mrow + 64 * r;
+                page[r] = 0u;
+                if (i < my_tiles && t < L) page[r] = min((uint32_t)__ldg(my_pages + (t >> p.page_shift)), (uint32_t)p.num_pages - 1u);
+            }
+        };
+        auto fetch_codes = [&](int i) {  // (rows behind the request's last: zeros, so that nothing of them counts)
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+                const int t = first_token(i) + mrow + 64 * r;
+                kc[r] = vc[r] = make_uint4(0u, 0u, 0u, 0u);
+                nrm[r] = 0;
+                if (i < my_tiles && t < L) {
+                    const size_t at = ((((size_t)page[r] << p.page_shift) + (size_t)(t & ((1 << p.page_shift) - 1))) * p.Hkv + kvh);
+                    if (BITS == 4) {
+                        kc[r] = __ldg(reinterpret_cast<const uint4*>(p.ck + at * BPH) + piece);
+                        vc[r] = __ldg(reinterpret_cast<const uint4*>(p.cv + at * BPH) + piece);
+                    } else {
+                        const uint2 a = __ldg(reinterpret_cast<const uint2*>(p.ck + at * BPH) + piece), b = __ldg(reinterpret_cast<const uint2*>(p.cv + at * BPH) + piece);
+                        kc[r].x = a.x; kc[r].y = a.y;
+                        vc[r].x = b.x; vc[r].y = b.y;
+                    }
+                    if (piece < 2) nrm[r] = __ldg(reinterpret_cast<const unsigned short*>(piece ? p.vn : p.kn) + at);
+                }
+            }
+        };
+        uint32_t lut;  // (made here, behind the barrier that the table waits for: the look-ups take it into their address)
+        asm volatile("mov.u32 %0, %1;" : "=r"(lut) : "r"(sb + PpfSmem::LUT + 4u * (uint32_t)lane) : "memory");
+        // 32 codes as centroids into the row's 16-byte pieces 4 piece .. + 3 (in an order in which a quarter-warp's stores meet no bank twice)
+        auto put_codes = [&](uint32_t tile, int row, const uint4 c) {
+#pragma unroll
+            for (int f = 0; f < FORMS; ++f) {
+                const int i = f ^ (piece & 2);
+                const uint32_t w = BITS == 4 ? ((f & 2) ? ((f & 1) ? ((piece & 2) ? c.y : c.w) : ((piece & 2) ? c.x : c.z))
+                                                        : ((f & 1) ? ((piece & 2) ? c.w : c.y) : ((piece & 2) ? c.z : c.x)))
+                                             : ((i & 2) ? c.y : c.x) >> ((f & 1) * 16);
+                uint32_t u[4];
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    const uint32_t at = BITS == 4 ? (b == 0 ? (w << 7) & 0x7f80u : (w >> (8 * b - 7)) & 0x7f80u)
+                                                  : (b < 2 ? (w << (7 - 4 * b)) & 0x780u : (w >> (4 * b - 7)) & 0x780u);
+                    u[b] = ldsp32(lut + at);
+                }
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(sb + tile + pft_chunk(row, 4 * piece + i)), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]) : "memory");
+            }
+        };
+        auto handed = [&](uint32_t bar) {  // this warp's stores are in place
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
+        };
+        const int maker = MT == 2 ? warp : 4 * (warp >> 3) + (warp & 3);
+        auto make_k = [&](int i) {  // the share's K codes and norms of tile i (among this thread's tiles)
+            if (i >= my_tiles) return;
+            const int j = MT == 2 ? i : 2 * i + slot, st = j & 1;
+            if (j >= 2) wait_bar(bar_kfree + 8u * st, (uint32_t)(((j >> 1) - 1) & 1));
+            uint8_t* const norms = gb + PpfSmem::NORM + (uint32_t)(j & (PPF_NSTAGES - 1)) * PpfSmem::NORM_BYTES;
+            uint32_t top = 0u;
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+                put_codes(PpfSmem::K + st * PFT_TILE, mrow + 64 * r, kc[r]);
+                if (piece < 2) reinterpret_cast<unsigned short*>(norms)[PFT_KT * piece + mrow + 64 * r] = nrm[r];
+                top = max(top, piece == 1 ? (uint32_t)nrm[r] : 0u);
+            }
+            top = __reduce_max_sync(0xffffffffu, top);
+            if (lane == 0) reinterpret_cast<unsigned short*>(norms + 4 * PFT_KT)[maker] = (unsigned short)top;
+            handed(bar_kfull + 8u * st);
+        };
+        auto make_v = [&](int i) {  // ... its V codes; then the next tile's are requested
+            if (i >= my_tiles) return;
+            const int j = MT == 2 ? i : 2 * i + slot, st = j & 1;
+            if (j >= 2) wait_bar(bar_vfree + 8u * st, (uint32_t)(((j >> 1) - 1) & 1));
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) put_codes(PpfSmem::V + st * PFT_TILE, mrow + 64 * r, vc[r]);
+            handed(bar_vfull + 8u * st);
+            fetch_codes(i + 1);
+            fetch_pages(i + 2);
+        };
+        fetch_pages(0);
+        fetch_codes(0);
+        fetch_pages(1);
+        const bool k_waits = MT == 1 && slot == 1;  // (its first K tile goes where R is)
+        if (!k_waits) make_k(0);
+        if (!k_waits) make_v(0);
+        // ---- q_rot = Q . R^T, scaled by log2(e) / sqrt(128), back into the Q tiles ----
+        wait_bar(bar_rot, 0u);
+        tc_fence_after();
+#pragma unroll 1
+        for (int c0 = pcol0; c0 < pcol0 + PCOLS; c0 += 64) {
+            uint32_t r[32];
+            tmem_ld_frag64(my_lanes + 128u * pslot + (uint32_t)c0, r);
+            tmem_ld_wait();
+            float v[32];
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(r[e]) * PFT_SCALE;
+            put_frag(PpfSmem::Q + pslot * PFT_TILE, c0, v);
+        }
+        fence_proxy_async_smem();
+        tc_fence_before();
+        named_barrier(1, PPF_MEET);
+        tc_fence_after();
+        if (k_waits) {
+            make_k(0);
+            make_v(0);
+        }
+
+        // ---- softmax of slot `slot`, rows row0 + gl and row0 + gl + 8 ----
+        const uint32_t s_col = my_lanes + 128u * slot, o_col = my_lanes + 256u + 128u * slot;
+        const int nt = slot ? n1 : n0;
+        const uint32_t by_grp0 = make_by_grp();
+        const int tok0 = token_of(row0 + gl, by_grp0), tok1 = token_of(row0 + gl + 8, by_grp0);
+        const bool some_row = token_in(row0, by_grp0) < QT && my_first + token_in(row0, by_grp0) < n;  // (uniform for the warp)
+        // last token of a row of no query: none
+        const int last0 = tok0 < n ? pos0 + tok0 : -1, last1 = tok1 < n ? pos0 + tok1 : -1;
+        float m_run[2] = {-1e30f, -1e30f}, l_run[2] = {0.0f, 0.0f};  // (sums: of this thread's columns)
+        for (int i = 0; i < (MT == 2 ? n_tiles : nt); ++i) {
+            // (the tile's norms.  MT = 1: asked for before the slot's next tile, which uses the same barrier, is made)
+            const int j = tile_of(slot, i), col0 = (t_lo + j) * PFT_KT;
+            if (MT == 1 || i < nt) wait_bar(bar_kfull + 8u * (j & 1), (uint32_t)((j >> 1) & 1));
+            make_k(i + 1);
+            if (MT == 1 || i < nt) {
+                wait_bar(bar_sfull + 8u * slot, (uint32_t)(i & 1));
+                tc_fence_after();
+                if (some_row) {
+                    const bool diagonal = col0 + PFT_KT - 1 > pos0 + my_first;  // (uniform for the slot)
+                    const uint8_t* const norms = gb + PpfSmem::NORM + (uint32_t)(j & (PPF_NSTAGES - 1)) * PpfSmem::NORM_BYTES;
+                    const __half2* const nrm2 = reinterpret_cast<const __half2*>(norms) + t4;
+                    float v_top;  // the tile's largest V norm
+                    {
+                        uint4 u = *reinterpret_cast<const uint4*>(norms + 4 * PFT_KT);
+                        uint32_t m = __vmaxu2(__vmaxu2(u.x, u.y), __vmaxu2(u.z, u.w));
+                        if (MT == 2) {
+                            u = *reinterpret_cast<const uint4*>(norms + 4 * PFT_KT + 16);
+                            m = __vmaxu2(m, __vmaxu2(__vmaxu2(u.x, u.y), __vmaxu2(u.z, u.w)));
+                        }
+                        v_top = __half2float(__ushort_as_half((unsigned short)max(m & 0xffffu, m >> 16)));
+                    }
+                    uint32_t sr[2][32];
+                    tmem_ld_frag64(s_col, sr[0]);
+                    tmem_ld_frag64(s_col + 64u, sr[1]);
+                    tmem_ld_wait();
+                    float2 x[2][16];  // [row][column block]
+                    float mx[2] = {-1e30f, -1e30f};
+#pragma unroll
+                    for (int b = 0; b < 16; ++b) {
+                        const float2 k2 = __half22float2(nrm2[4 * b]);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+                            x[h][b] = mul2(make_float2(__uint_as_float(sr[b >> 3][4 * (b & 7) + 2 * h]), __uint_as_float(sr[b >> 3][4 * (b & 7) + 2 * h + 1])), k2);
+                    }
+                    if (diagonal) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int lim = (h ? last1 : last0) - col0 - 2 * t4;  // columns up to here count
+#pragma unroll
+                            for (int b = 0; b < 16; ++b) {
+                                if (8 * b > lim) x[h][b].x = -1e30f;
+                                if (8 * b + 1 > lim) x[h][b].y = -1e30f;
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float m2 = -1e30f;
+#pragma unroll
+                        for (int b = 0; b < 16; b += 2) {
+                            mx[h] = fmaxf(mx[h], fmaxf(x[h][b].x, x[h][b].y));
+                            m2 = fmaxf(m2, fmaxf(x[h][b + 1].x, x[h][b + 1].y));
+                        }
+                        mx[h] = fmaxf(mx[h], m2);
+                        mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
+                        mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
+                    }
+                    // (weights of up to 2^PFT_SLACK times a norm of 4094 still fit fp16; a tile with a larger one keeps its weights below 1)
+                    const float slack = v_top <= 65504.0f / (float)(1 << (int)PFT_SLACK) ? PFT_SLACK : 0.0f;
+                    const bool grew0 = mx[0] > m_run[0] + slack, grew1 = mx[1] > m_run[1] + slack;
+                    if (__any_sync(0xffffffffu, grew0 || grew1)) {
+                        const float mn0 = grew0 ? mx[0] : m_run[0], mn1 = grew1 ? mx[1] : m_run[1];
+                        const float corr0 = ex2_approx(m_run[0] - mn0), corr1 = ex2_approx(m_run[1] - mn1);
+                        m_run[0] = mn0; m_run[1] = mn1;
+                        l_run[0] *= corr0; l_run[1] *= corr1;
+                        if (i > 0) {  // S(i) is there, so P(i - 1) V has finished: O is at rest
+#pragma unroll 1
+                            for (int c = 0; c < 4; ++c) {
+                                uint32_t r[16];
+                                tmem_ld_frag32(o_col + 32u * c, r);
+                                tmem_ld_wait();
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * ((e & 2) ? corr1 : corr0));
+                                tmem_st_frag32(o_col + 32u * c, r);
+                            }
+                        }
+                    }
+                    // ---- P (times the V norm) as fp16 over S ----
+                    float2 lsum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+                    float2 minus[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)  // (no column counts yet: all weights 0)
+                        minus[h] = m_run[h] <= -1e29f ? make_float2(0.0f, 0.0f) : make_float2(-m_run[h], -m_run[h]);
+                    auto weights = [&](auto masked_is_zero) {
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            uint32_t pr[16];
+#pragma unroll
+                            for (int b = 0; b < 8; ++b) {
+                                const float2 v2 = __half22float2(nrm2[64 + 32 * c + 4 * b]);
+#pragma unroll
+                                for (int h = 0; h < 2; ++h) {
+                                    float2 a = add2(x[h][8 * c + b], minus[h]);
+                                    a = make_float2(ex2_approx(a.x), ex2_approx(a.y));
+                                    lsum[h] = add2(lsum[h], a);
+                                    if constexpr (decltype(masked_is_zero)::value)
+                                        a = make_float2(x[h][8 * c + b].x <= -1e30f ? 0.0f : a.x * v2.x, x[h][8 * c + b].y <= -1e30f ? 0.0f : a.y * v2.y);
+                                    else
+                                        a = mul2(a, v2);
+                                    pr[2 * b + h] = pack_half2(a.x, a.y);
+                                }
+                            }
+                            tmem_st_pack32(s_col + 32u * c, pr);
+                        }
+                    };
+                    // a masked weight is 0, and 0 times a V norm that is not finite is not: a tile with such a norm selects instead
+                    if (diagonal && !(v_top < INFINITY)) weights(std::true_type{});
+                    else weights(std::false_type{});
+                    l_run[0] += lsum[0].x + lsum[0].y;
+                    l_run[1] += lsum[1].x + lsum[1].y;
+                    tmem_st_wait();
+                }
+                tc_fence_before();
+                mbar_arrive(bar_pfull + 8u * slot);
+            }
+            make_v(i + 1);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 1);
+            l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 2);
+        }
+        wait_bar(bar_done, 0u);  // every product has completed (and nobody reads the norms any more)
+        tc_fence_after();
+
+        // ================= results =================
+        float w0[2], w1[2] = {0.0f, 0.0f};  // by row: weights of the slots' sums, normalised (MT = 2: of its own; SPLIT: not normalised)
+        float M_all[2], Z_all[2];
+        if constexpr (MT == 1) {
+            named_barrier(2, 32 * PFT_SOFT_WARPS);  // (the other slot's last norms have been read)
+            float2* const xch = reinterpret_cast<float2*>(gb + PpfSmem::NORM);
+            if (t4 == 0) {
+                xch[slot * 128 + row0 + gl] = make_float2(m_run[0], l_run[0]);
+                xch[slot * 128 + row0 + gl + 8] = make_float2(m_run[1], l_run[1]);
+            }
+            named_barrier(2, 32 * PFT_SOFT_WARPS);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float2 a = xch[row0 + gl + 8 * h], b = xch[128 + row0 + gl + 8 * h];
+                const float M = fmaxf(a.x, b.x), e0 = n0 > 0 ? ex2_approx(a.x - M) : 0.0f, e1 = n1 > 0 ? ex2_approx(b.x - M) : 0.0f;
+                M_all[h] = M;
+                Z_all[h] = a.y * e0 + b.y * e1;
+                const float inv = SPLIT ? 1.0f : 1.0f / (Z_all[h] + 1e-8f);
+                w0[h] = e0 * inv;
+                w1[h] = e1 * inv;
+            }
+        } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) w0[h] = 1.0f / (l_run[h] + 1e-8f);
+        }
+        // rows that attend to nothing (no tile at all, or none up to their position) give zeros whatever tensor memory holds
+        const bool on[2] = {last0 >= 0 && (MT == 1 || nt > 0), last1 >= 0 && (MT == 1 || nt > 0)};
+        auto result = [&](int c0, float (&v)[32]) {  // columns c0 .. c0 + 63 in fragment order
+            uint32_t r[32];
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = 0.0f;
+            if (MT == 2 ? nt > 0 : n0 > 0) {
+                tmem_ld_frag64((MT == 2 ? o_col : my_lanes + 256u) + (uint32_t)c0, r);
+                tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 32; ++e) v[e] = on[(e >> 1) & 1] ? __uint_as_float(r[e]) * w0[(e >> 1) & 1] : 0.0f;
+            }
+            if (MT == 1 && n1 > 0) {
+                tmem_ld_frag64(my_lanes + 384u + (uint32_t)c0, r);
+                tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 32; ++e) v[e] = on[(e >> 1) & 1] ? fmaf(__uint_as_float(r[e]), w1[(e >> 1) & 1], v[e]) : 0.0f;
+            }
+        };
+        if constexpr (SPLIT) {
+            // the sums as they are, with maximum and sum of weights behind them
+            const uint32_t by_grp = make_by_grp();
+            const int c0 = pcol0;
+            float v[32];
+            result(c0, v);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int row = row0 + gl + 8 * h, tok = h ? tok1 : tok0;
+                if (tok >= n) continue;
+                float* const dst = p.partials + (((size_t)blockIdx.z * p.T + s0 + tok) * p.H + (size_t)(kvh * GRP + row - token_in(row, by_grp) * GRP)) * PART_STRIDE;
+#pragma unroll
+                for (int b = 0; b < 8; ++b) *reinterpret_cast<float2*>(dst + c0 + 8 * b + 2 * t4) = make_float2(v[4 * b + 2 * h], v[4 * b + 2 * h + 1]);
+                if (slot == 0 && t4 == 0) *reinterpret_cast<float2*>(dst + HEAD_DIM) = on[h] ? make_float2(M_all[h], Z_all[h]) : make_float2(-1e30f, 0.0f);
+            }
+        } else {
+            const uint32_t qtile = PpfSmem::Q + pslot * PFT_TILE, ktile = PpfSmem::K + pslot * PFT_TILE;
+            // the normalised rows, split into fp16 high and low parts, over the Q and K tiles
+#pragma unroll 1
+            for (int c0 = pcol0; c0 < pcol0 + PCOLS; c0 += 64) {
+                float v[32];
+                result(c0, v);
+                put_frag(qtile, c0, v);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) v[e] = low_part(v[e]);
+                put_frag(ktile, c0, v);
+            }
+            fence_proxy_async_smem();
+            tc_fence_before();
+            named_barrier(1, PPF_MEET);
+            wait_bar(bar_rot, 1u);
+            tc_fence_after();
+            // the finished values as fp16 through the (consumed) query tile, so that 16 lanes store 256 contiguous bytes of a row
+#pragma unroll 1
+            for (int c0 = pcol0; c0 < pcol0 + PCOLS; c0 += 64) {
+                float v[32];
+                uint32_t r[32];
+                tmem_ld_frag64(my_lanes + 128u * pslot + (uint32_t)c0, r);
+                tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(r[e]);
+                put_frag(qtile, c0, v);
+            }
+            __syncwarp();
+            constexpr int CH = PCOLS / 8;  // 16-byte pieces per row
+            const uint32_t by_grp = make_by_grp();
+            __half* const out_seq = p.out + (size_t)s0 * p.out_stride;
+#pragma unroll
+            for (int k = 0; k < CH / 2; ++k) {
+                const int at = 32 * k + lane, row = row0 + at / CH, ch = (pcol0 >> 3) + at % CH, tok = token_of(row, by_grp);
+                if (tok < n) {
+                    const uint4 u = *reinterpret_cast<const uint4*>(gb + qtile + pft_chunk(row, ch));
+                    *(reinterpret_cast<uint4*>(out_seq + (size_t)tok * p.out_stride + (size_t)(kvh * GRP + row - token_in(row, by_grp) * GRP) * HEAD_DIM) + ch) = u;
+                }
+            }
+        }
+        tc_fence_before();
+    }
+    if (dead) {  // copies and products may still be in flight: a bounded chance to land before shared and tensor memory go away
+        mbar_wait_bounded_hint(bar_q, 0u, 1u << 10, 2000u);
+        mbar_wait_bounded_hint(bar_r, 0u, 1u << 10, 2000u);
+        mbar_wait_bounded_hint(bar_done, 0u, 1u << 10, 2000u);
+    }
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 0) tmem_dealloc(tmem, 512u);
+}
+
+// The parts of a split call: out[tok][h] = R (sum_z 2^(m_z - M) acc_z / sum_z 2^(m_z - M) l_z).  16 (token, head) rows per CTA, two a warp;
+// fp16 high and low parts of the sums times R on mma.sync, a warp 16 output coordinates.
+struct PagedMergeParams {
+    const float* partials;   // [splits][T][H][PART_STRIDE]
+    const __half* rotation;  // R row-major
+    const int* start;        // [G + 1]
+    __half* out;
+    int splits, T, G, H, out_stride;
+};
+static __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedMergeParams p) {
+    __shared__ __align__(16) __half r_s[HEAD_DIM / 2][HEAD_DIM + 8];
+    __shared__ __align__(16) __half a_s[2][16][HEAD_DIM + 8];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gl = lane >> 2, t4 = lane & 3;
+    pdl_launch_dependents();
+    pdl_wait();
+    uint32_t bf[2][8][2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int at = tid + 256 * i;
+            *reinterpret_cast<uint4*>(&r_s[at >> 4][8 * (at & 15)]) = reinterpret_cast<const uint4*>(p.rotation)[1024 * half + at];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint32_t r[4];
+            ldmatrix_x4_trans(r, smem_u32(&r_s[16 * j + (lane & 15)][16 * warp + 8 * (lane >> 4)]));
+            bf[0][4 * half + j][0] = r[0]; bf[0][4 * half + j][1] = r[1];
+            bf[1][4 * half + j][0] = r[2]; bf[1][4 * half + j][1] = r[3];
+        }
+    }
+    const long long rows = (long long)min(p.start[p.G], p.T) * p.H;  // (tokens behind the last request have no sums)
+    const size_t part = (size_t)p.T * p.H * PART_STRIDE;
+    for (long long row0 = 16ll * blockIdx.x; row0 < rows; row0 += 16ll * gridDim.x) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int rr = 2 * warp + k;
+            const float* const src = p.partials + (size_t)(row0 + rr) * PART_STRIDE;
+            float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (row0 + rr < rows) {
+                float2 ml = make_float2(-1e30f, 0.0f);
+                if (lane < p.splits) ml = __ldcg(reinterpret_cast<const float2*>(src + lane * part + HEAD_DIM));
+                float M = ml.x;
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+                const float e = lane < p.splits ? ex2_approx(ml.x - M) : 0.0f;
+                float Z = ml.y * e;
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) Z += __shfl_xor_sync(0xffffffffu, Z, o);
+                const float sc = e / (Z + 1e-8f);
+#pragma unroll 4
+                for (int z = 0; z < p.splits; ++z) {
+                    const float4 v = __ldcg(reinterpret_cast<const float4*>(src + z * part) + lane);
+                    const float w = __shfl_sync(0xffffffffu, sc, z);
+                    a.x = fmaf(w, v.x, a.x); a.y = fmaf(w, v.y, a.y); a.z = fmaf(w, v.z, a.z); a.w = fmaf(w, v.w, a.w);
+                }
+            }
+            *reinterpret_cast<uint2*>(&a_s[0][rr][4 * lane]) = make_uint2(pack_half2(a.x, a.y), pack_half2(a.z, a.w));
+            *reinterpret_cast<uint2*>(&a_s[1][rr][4 * lane]) = make_uint2(pack_low_half2(a.x, a.y), pack_low_half2(a.z, a.w));
+        }
+        __syncthreads();
+        float c[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int part2 = 0; part2 < 2; ++part2)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                uint32_t a[4];
+                ldmatrix_x4(a, smem_u32(&a_s[part2][lane & 15][16 * j + 8 * (lane >> 4)]));
+#pragma unroll
+                for (int i = 0; i < 2; ++i) mma16816(c[i], a[0], a[1], a[2], a[3], bf[i][j][0], bf[i][j][1]);
+            }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const long long row = row0 + gl + 8 * r, tok = row / p.H;
+            if (row >= rows) continue;
+            __half* const dst = p.out + tok * p.out_stride + (row - tok * p.H) * HEAD_DIM + 16 * warp + 2 * t4;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) *reinterpret_cast<__half2*>(dst + 8 * i) = __floats2half2_rn(c[i][2 * r], c[i][2 * r + 1]);
+        }
+        __syncthreads();  // (the next rows)
+    }
+}
+
+}  // namespace tq

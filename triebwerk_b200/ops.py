@@ -175,6 +175,16 @@ def paged_decode_attention(out, q, ck_q, cv_q, k_norms, v_norms, rotation, block
         raise TqError(st, "tq_paged_decode_attention")
 
 
+def paged_prefill_attention(out, q, ck_q, cv_q, k_norms, v_norms, rotation, block_table, seq_lens, query_start, page_size, num_heads,
+                            num_kv_heads, bits, workspace):
+    """Causal attention of a ragged batch: the queries query_start[g] .. query_start[g + 1] - 1 of q [T, num_heads * 128] are the
+    last of request g's seq_lens[g] tokens."""
+    st = hostcall.paged_prefill_attention(out, q, ck_q, cv_q, k_norms, v_norms, rotation, block_table, seq_lens, query_start, page_size,
+                                          num_heads, num_kv_heads, bits, workspace)
+    if st:
+        raise TqError(st, "tq_paged_prefill_attention")
+
+
 def paged_status() -> int:
     """Status word of the paged calls on the current device (0 = fine); reading clears it and synchronises the stream."""
     return int(lib().tq_paged_status(_stream()))
