@@ -8,8 +8,8 @@
 // (16384 tokens and 8 KV heads as fp16 are 64 MB a request), and reads the packed bytes alone.
 //   * A block = 128 score rows = 128 / GRP query tokens x the GRP query heads of a KV head.  MT = 2: a CTA has two blocks, which share
 //     every K and V tile; MT = 1: one block, whose two slots take the even and the odd tiles and are combined at the end.
-//   * The 16 softmax warps are the producers too: a thread fetches 16 (2-bit: 8) bytes of one row of the next K and V tile into registers a
-//     tile ahead (its page's number another tile ahead), and turns them into centroids through a shared-memory table with a column
+//   * The 16 softmax warps are the producers too: a thread fetches 16 (2-bit: 8) bytes of one row of the next K and V tile into registers
+//     as soon as it has made the present one (their page's number before that), and turns them into centroids through a shared-memory table with a column
 //     per lane: K of tile j + 1 before it waits for S(j), V of tile j + 1 after its weights P(j) are out.  So the table look-ups and
 //     operand stores fill the time in which the tensor core works on the slot's own products.
 //   * MT = 2: all 16 warps make a share of every tile.  MT = 1: a slot's warps make that slot's tiles, and nothing ties the slots.
@@ -281,26 +281,27 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                 if (i < my_tiles && t < L) page[r] = min((uint32_t)__ldg(my_pages + (t >> p.page_shift)), (uint32_t)p.num_pages - 1u);
             }
         };
-        auto fetch_codes = [&](int i) {  // (rows behind the request's last: zeros, so that nothing of them counts)
+        // (rows behind the request's last: zeros, so that nothing of them counts)
+        auto fetch_codes = [&](int i, const uint8_t* codes, uint4 (&c)[ROWS], bool norms) {
 #pragma unroll
             for (int r = 0; r < ROWS; ++r) {
                 const int t = first_token(i) + mrow + 64 * r;
-                kc[r] = vc[r] = make_uint4(0u, 0u, 0u, 0u);
-                nrm[r] = 0;
+                c[r] = make_uint4(0u, 0u, 0u, 0u);
+                if (norms) nrm[r] = 0;
                 if (i < my_tiles && t < L) {
                     const size_t at = ((((size_t)page[r] << p.page_shift) + (size_t)(t & ((1 << p.page_shift) - 1))) * p.Hkv + kvh);
                     if (BITS == 4) {
-                        kc[r] = __ldg(reinterpret_cast<const uint4*>(p.ck + at * BPH) + piece);
-                        vc[r] = __ldg(reinterpret_cast<const uint4*>(p.cv + at * BPH) + piece);
+                        c[r] = __ldg(reinterpret_cast<const uint4*>(codes + at * BPH) + piece);
                     } else {
-                        const uint2 a = __ldg(reinterpret_cast<const uint2*>(p.ck + at * BPH) + piece), b = __ldg(reinterpret_cast<const uint2*>(p.cv + at * BPH) + piece);
-                        kc[r].x = a.x; kc[r].y = a.y;
-                        vc[r].x = b.x; vc[r].y = b.y;
+                        const uint2 a = __ldg(reinterpret_cast<const uint2*>(codes + at * BPH) + piece);
+                        c[r].x = a.x; c[r].y = a.y;
                     }
-                    if (piece < 2) nrm[r] = __ldg(reinterpret_cast<const unsigned short*>(piece ? p.vn : p.kn) + at);
+                    if (norms && piece < 2) nrm[r] = __ldg(reinterpret_cast<const unsigned short*>(piece ? p.vn : p.kn) + at);
                 }
             }
         };
+        auto fetch_k = [&](int i) { fetch_codes(i, p.ck, kc, true); };
+        auto fetch_v = [&](int i) { fetch_codes(i, p.cv, vc, false); };
         uint32_t lut;  // (made here, behind the barrier that the table waits for: the look-ups take it into their address)
         asm volatile("mov.u32 %0, %1;" : "=r"(lut) : "r"(sb + PpfSmem::LUT + 4u * (uint32_t)lane) : "memory");
         // 32 codes as centroids into the row's 16-byte pieces 4 piece .. + 3 (in an order in which a quarter-warp's stores meet no bank twice)
@@ -327,7 +328,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             if (lane == 0) mbar_arrive(bar);
         };
         const int maker = MT == 2 ? warp : 4 * (warp >> 3) + (warp & 3);
-        auto make_k = [&](int i) {  // the share's K codes and norms of tile i (among this thread's tiles)
+        auto make_k = [&](int i) {  // the share's K codes and norms of tile i (among this thread's tiles); then the next tile's are requested
             if (i >= my_tiles) return;
             const int j = MT == 2 ? i : 2 * i + slot, st = j & 1;
             if (j >= 2) wait_bar(bar_kfree + 8u * st, (uint32_t)(((j >> 1) - 1) & 1));
@@ -342,19 +343,21 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             top = __reduce_max_sync(0xffffffffu, top);
             if (lane == 0) reinterpret_cast<unsigned short*>(norms + 4 * PFT_KT)[maker] = (unsigned short)top;
             handed(bar_kfull + 8u * st);
+            fetch_k(i + 1);
         };
-        auto make_v = [&](int i) {  // ... its V codes; then the next tile's are requested
+        auto make_v = [&](int i) {  // ... its V codes; then the next tile's, and the pages of the one after it
             if (i >= my_tiles) return;
             const int j = MT == 2 ? i : 2 * i + slot, st = j & 1;
             if (j >= 2) wait_bar(bar_vfree + 8u * st, (uint32_t)(((j >> 1) - 1) & 1));
 #pragma unroll
             for (int r = 0; r < ROWS; ++r) put_codes(PpfSmem::V + st * PFT_TILE, mrow + 64 * r, vc[r]);
             handed(bar_vfull + 8u * st);
-            fetch_codes(i + 1);
+            fetch_v(i + 1);
             fetch_pages(i + 2);
         };
         fetch_pages(0);
-        fetch_codes(0);
+        fetch_k(0);
+        fetch_v(0);
         fetch_pages(1);
         const bool k_waits = MT == 1 && slot == 1;  // (its first K tile goes where R is)
         if (!k_waits) make_k(0);
@@ -412,39 +415,51 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                         }
                         v_top = __half2float(__ushort_as_half((unsigned short)max(m & 0xffffu, m >> 16)));
                     }
-                    uint32_t sr[2][32];
-                    tmem_ld_frag64(s_col, sr[0]);
-                    tmem_ld_frag64(s_col + 64u, sr[1]);
-                    tmem_ld_wait();
-                    float2 x[2][16];  // [row][column block]
-                    float mx[2] = {-1e30f, -1e30f};
+                    // Scores of 64 columns at a time, scaled by the K norms and masked: [row][column block].  The second half is read once for the
+                    // row maxima and once more for its weights: with all 128 in registers the compiler spilled, and what is spilled comes back
+                    // from L2 (shared memory leaves no L1): 4 x 1024 tokens behind 8192 took 990 us, 60 % of them waits for such loads.
+                    auto scores = [&](int c, float2 (&x)[2][8]) {
+                        uint32_t r[32];
+                        tmem_ld_frag64(s_col + 64u * c, r);
+                        tmem_ld_wait();
 #pragma unroll
-                    for (int b = 0; b < 16; ++b) {
-                        const float2 k2 = __half22float2(nrm2[4 * b]);
+                        for (int b = 0; b < 8; ++b) {
+                            const float2 k2 = __half22float2(nrm2[32 * c + 4 * b]);
 #pragma unroll
-                        for (int h = 0; h < 2; ++h)
-                            x[h][b] = mul2(make_float2(__uint_as_float(sr[b >> 3][4 * (b & 7) + 2 * h]), __uint_as_float(sr[b >> 3][4 * (b & 7) + 2 * h + 1])), k2);
-                    }
-                    if (diagonal) {
+                            for (int h = 0; h < 2; ++h) x[h][b] = mul2(make_float2(__uint_as_float(r[4 * b + 2 * h]), __uint_as_float(r[4 * b + 2 * h + 1])), k2);
+                        }
+                        if (diagonal) {
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const int lim = (h ? last1 : last0) - col0 - 2 * t4;  // columns up to here count
+                            for (int h = 0; h < 2; ++h) {
+                                const int lim = (h ? last1 : last0) - col0 - 64 * c - 2 * t4;  // columns up to here count
 #pragma unroll
-                            for (int b = 0; b < 16; ++b) {
-                                if (8 * b > lim) x[h][b].x = -1e30f;
-                                if (8 * b + 1 > lim) x[h][b].y = -1e30f;
+                                for (int b = 0; b < 8; ++b) {
+                                    if (8 * b > lim) x[h][b].x = -1e30f;
+                                    if (8 * b + 1 > lim) x[h][b].y = -1e30f;
+                                }
                             }
                         }
-                    }
+                    };
+                    float mx[2] = {-1e30f, -1e30f};
+                    auto largest = [&](const float2 (&x)[2][8]) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            float m2 = -1e30f;
+#pragma unroll
+                            for (int b = 0; b < 8; b += 2) {
+                                mx[h] = fmaxf(mx[h], fmaxf(x[h][b].x, x[h][b].y));
+                                m2 = fmaxf(m2, fmaxf(x[h][b + 1].x, x[h][b + 1].y));
+                            }
+                            mx[h] = fmaxf(mx[h], m2);
+                        }
+                    };
+                    float2 x[2][8];
+                    scores(1, x);
+                    largest(x);
+                    scores(0, x);
+                    largest(x);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        float m2 = -1e30f;
-#pragma unroll
-                        for (int b = 0; b < 16; b += 2) {
-                            mx[h] = fmaxf(mx[h], fmaxf(x[h][b].x, x[h][b].y));
-                            m2 = fmaxf(m2, fmaxf(x[h][b + 1].x, x[h][b + 1].y));
-                        }
-                        mx[h] = fmaxf(mx[h], m2);
                         mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
                         mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
                     }
@@ -474,31 +489,33 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 #pragma unroll
                     for (int h = 0; h < 2; ++h)  // (no column counts yet: all weights 0)
                         minus[h] = m_run[h] <= -1e29f ? make_float2(0.0f, 0.0f) : make_float2(-m_run[h], -m_run[h]);
-                    auto weights = [&](auto masked_is_zero) {
+                    auto weights = [&](int c, auto masked_is_zero) {
+                        uint32_t pr[16];
 #pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            uint32_t pr[16];
+                        for (int b = 0; b < 8; ++b) {
+                            const float2 v2 = __half22float2(nrm2[64 + 32 * c + 4 * b]);
 #pragma unroll
-                            for (int b = 0; b < 8; ++b) {
-                                const float2 v2 = __half22float2(nrm2[64 + 32 * c + 4 * b]);
-#pragma unroll
-                                for (int h = 0; h < 2; ++h) {
-                                    float2 a = add2(x[h][8 * c + b], minus[h]);
-                                    a = make_float2(ex2_approx(a.x), ex2_approx(a.y));
-                                    lsum[h] = add2(lsum[h], a);
-                                    if constexpr (decltype(masked_is_zero)::value)
-                                        a = make_float2(x[h][8 * c + b].x <= -1e30f ? 0.0f : a.x * v2.x, x[h][8 * c + b].y <= -1e30f ? 0.0f : a.y * v2.y);
-                                    else
-                                        a = mul2(a, v2);
-                                    pr[2 * b + h] = pack_half2(a.x, a.y);
-                                }
+                            for (int h = 0; h < 2; ++h) {
+                                float2 a = add2(x[h][b], minus[h]);
+                                a = make_float2(ex2_approx(a.x), ex2_approx(a.y));
+                                lsum[h] = add2(lsum[h], a);
+                                if constexpr (decltype(masked_is_zero)::value)
+                                    a = make_float2(x[h][b].x <= -1e30f ? 0.0f : a.x * v2.x, x[h][b].y <= -1e30f ? 0.0f : a.y * v2.y);
+                                else
+                                    a = mul2(a, v2);
+                                pr[2 * b + h] = pack_half2(a.x, a.y);
                             }
-                            tmem_st_pack32(s_col + 32u * c, pr);
                         }
+                        tmem_st_pack32(s_col + 32u * c, pr);
                     };
                     // a masked weight is 0, and 0 times a V norm that is not finite is not: a tile with such a norm selects instead
-                    if (diagonal && !(v_top < INFINITY)) weights(std::true_type{});
-                    else weights(std::false_type{});
+                    const bool select = diagonal && !(v_top < INFINITY);
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        if (c) scores(1, x);
+                        if (select) weights(c, std::true_type{});
+                        else weights(c, std::false_type{});
+                    }
                     l_run[0] += lsum[0].x + lsum[0].y;
                     l_run[1] += lsum[1].x + lsum[1].y;
                     tmem_st_wait();
