@@ -1,8 +1,8 @@
 // Causal attention of several new tokens per request over paged packed caches (tcgen05 + tensor memory), sm_100a.
 //
 // Query i of request g, of its n new tokens, stands at position p = L - n + i of its L tokens and attends to tokens 0 .. p:
-//   out = R (softmax_t((R^T-rotated q . centroids_K[t]) norm_K[t] / sqrt(128)) . (norm_V[t] centroids_V[t]))
-// with q rotated by R first and one R product at the end (tq_prefill_fa.cuh has the mathematics; the slots, the softmax and the order of
+//   out = R (softmax_t(R q . norm_K[t] centroids_K[t] / sqrt(128)) . norm_V[t] centroids_V[t])
+// with q rotated once and one R product at the end (tq_prefill_fa.cuh has the mathematics; the slots, the softmax and the order of
 // products are that kernel's).  What differs: the batch is ragged, requests have earlier tokens, rows come by way of block tables, and the
 // codes become fp16 centroids INSIDE the kernel, so that a call needs no scratch for the contexts, whose lengths the host does not know
 // (16384 tokens and 8 KV heads as fp16 are 64 MB a request), and reads the packed bytes alone.
@@ -50,15 +50,19 @@ struct PpfSmem {
     static constexpr uint32_t Q = 0;                       // 2 tiles; at the end: high parts of the results
     static constexpr uint32_t K = 2 * PFT_TILE;            // 2 stages; at the start R in the second; at the end: low parts
     static constexpr uint32_t V = K + 2 * PFT_TILE;        // 2 stages; at the end R in the first
-    static constexpr uint32_t LUT = V + 2 * PFT_TILE;      // byte (4-bit) or nibble -> two centroids, a column per lane
+    static constexpr uint32_t LUT = V + 2 * PFT_TILE;      // byte (4-bit) or nibble -> two centroids, a column per lane; at the end (MT = 1) the slots' maxima and sums
     static constexpr uint32_t LUT_BYTES = 32768u;
-    static constexpr uint32_t NORM = LUT + LUT_BYTES;      // [stage]: K norms, V norms as halves, 16 warps' largest V norm; MT = 1, at the end: the slots' maxima and sums
-    static constexpr uint32_t NORM_BYTES = 2u * PFT_KT * 2u + 32u;
+    static constexpr uint32_t NORM = LUT + LUT_BYTES;      // [stage]: V's factors as halves, 16 warps' words: one that is not finite
+    static constexpr uint32_t NORM_BYTES = 2u * PFT_KT + 32u;
     static constexpr uint32_t CTRL = NORM + PPF_NSTAGES * NORM_BYTES;
     static constexpr uint32_t BYTES = CTRL + 192u;
 };
 static_assert(PpfSmem::BYTES <= 227 * 1024, "one CTA's shared memory");
-static_assert(PPF_NSTAGES * PpfSmem::NORM_BYTES >= 2 * 128 * 8, "the slots' maxima and sums");
+constexpr uint32_t PPF_XCH = PpfSmem::LUT;  // (the table is no longer needed then)
+// The centroids times these have fp16 neighbours 3.4 times (2-bit: over 1000 times) as close as the centroids themselves (2^-11 x 0.22 and 0.0004
+// against 0.73 and 0.54, relative): the table holds them scaled, the queries and the results carry the inverse.
+template <int BITS>
+constexpr float PPF_CENT = BITS == 4 ? 1.211955f : 1.591824f;
 
 template <int BITS, int MT, bool SPLIT>
 __global__ void __launch_bounds__(PPF_THREADS, 1)
@@ -134,7 +138,8 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         constexpr int ENTRIES = BITS == 4 ? 256 : 16;
         for (int i = tid; i < ENTRIES * 8; i += PPF_THREADS) {  // four lanes' columns at a time
             const int e = i >> 3;
-            const uint32_t u = BITS == 4 ? pack_half2(kCent4[e & 15], kCent4[(e >> 4) & 15]) : pack_half2(kCent2[e & 3], kCent2[(e >> 2) & 3]);
+            constexpr float c = PPF_CENT<BITS>;
+            const uint32_t u = BITS == 4 ? pack_half2(c * kCent4[e & 15], c * kCent4[(e >> 4) & 15]) : pack_half2(c * kCent2[e & 3], c * kCent2[(e >> 2) & 3]);
             *reinterpret_cast<uint4*>(gb + PpfSmem::LUT + 16u * (uint32_t)i) = make_uint4(u, u, u, u);
         }
     }
@@ -270,6 +275,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         constexpr int FORMS = 4;                                    // 16-byte pieces of fp16 per share
         uint4 kc[ROWS], vc[ROWS];                                   // codes of the next tile (2-bit: x, y)
         unsigned short nrm[ROWS];                                   // piece 0: K norm, piece 1: V norm of the row
+        uint32_t vn[ROWS];                                          // the factor of V's row, from make_k to make_v of a tile
         uint32_t page[ROWS];                                        // of the tile after it
         const int* const my_pages = p.block_table + (size_t)g * p.table_stride;
         auto first_token = [&](int i) { return (t_lo + (MT == 2 ? i : 2 * i + slot)) * PFT_KT; };
@@ -304,8 +310,11 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         auto fetch_v = [&](int i) { fetch_codes(i, p.cv, vc, false); };
         uint32_t lut;  // (made here, behind the barrier that the table waits for: the look-ups take it into their address)
         asm volatile("mov.u32 %0, %1;" : "=r"(lut) : "r"(sb + PpfSmem::LUT + 4u * (uint32_t)lane) : "memory");
-        // 32 codes as centroids into the row's 16-byte pieces 4 piece .. + 3 (in an order in which a quarter-warp's stores meet no bank twice)
-        auto put_codes = [&](uint32_t tile, int row, const uint4 c) {
+        // 32 codes as centroids times a norm into the row's 16-byte pieces 4 piece .. + 3 (in an order in which a quarter-warp's stores meet no
+        // bank twice).  The norm is in the operands, rounded to fp16 once more: for each score and weight, 64 a thread and tile, it cost a
+        // fifth of all instructions.
+        auto put_codes = [&](uint32_t tile, int row, const uint4 c, uint32_t norm) {
+            const __half2 n2 = __half2half2(__ushort_as_half((unsigned short)norm));
 #pragma unroll
             for (int f = 0; f < FORMS; ++f) {
                 const int i = f ^ (piece & 2);
@@ -318,6 +327,8 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                     const uint32_t at = BITS == 4 ? (b == 0 ? (w << 7) & 0x7f80u : (w >> (8 * b - 7)) & 0x7f80u)
                                                   : (b < 2 ? (w << (7 - 4 * b)) & 0x780u : (w >> (4 * b - 7)) & 0x780u);
                     u[b] = ldsp32(lut + at);
+                    const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&u[b]), n2);
+                    u[b] = *reinterpret_cast<const uint32_t*>(&v);
                 }
                 asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(sb + tile + pft_chunk(row, 4 * piece + i)), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]) : "memory");
             }
@@ -336,12 +347,19 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             uint32_t top = 0u;
 #pragma unroll
             for (int r = 0; r < ROWS; ++r) {
-                put_codes(PpfSmem::K + st * PFT_TILE, mrow + 64 * r, kc[r]);
-                if (piece < 2) reinterpret_cast<unsigned short*>(norms)[PFT_KT * piece + mrow + 64 * r] = nrm[r];
-                top = max(top, piece == 1 ? (uint32_t)nrm[r] : 0u);
+                put_codes(PpfSmem::K + st * PFT_TILE, mrow + 64 * r, kc[r], __shfl_sync(0xffffffffu, (uint32_t)nrm[r], lane & ~3));
+                // V's norm goes into V too, unless it is not finite: it would reach queries that the token is hidden from (0 x inf).  Then the
+                // weights take it, those that count (below).
+                vn[r] = __shfl_sync(0xffffffffu, (uint32_t)nrm[r], (lane & ~3) | 1);
+                const bool odd = (vn[r] & 0x7fffu) >= 0x7c00u;
+                if (piece == 0) reinterpret_cast<unsigned short*>(norms)[mrow + 64 * r] = odd ? (unsigned short)vn[r] : (unsigned short)0x3c00u;
+                if (odd) {
+                    vn[r] = 0x3c00u;
+                    top = 1u;
+                }
             }
             top = __reduce_max_sync(0xffffffffu, top);
-            if (lane == 0) reinterpret_cast<unsigned short*>(norms + 4 * PFT_KT)[maker] = (unsigned short)top;
+            if (lane == 0) reinterpret_cast<unsigned short*>(norms + 2 * PFT_KT)[maker] = (unsigned short)top;
             handed(bar_kfull + 8u * st);
             fetch_k(i + 1);
         };
@@ -350,7 +368,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             const int j = MT == 2 ? i : 2 * i + slot, st = j & 1;
             if (j >= 2) wait_bar(bar_vfree + 8u * st, (uint32_t)(((j >> 1) - 1) & 1));
 #pragma unroll
-            for (int r = 0; r < ROWS; ++r) put_codes(PpfSmem::V + st * PFT_TILE, mrow + 64 * r, vc[r]);
+            for (int r = 0; r < ROWS; ++r) put_codes(PpfSmem::V + st * PFT_TILE, mrow + 64 * r, vc[r], vn[r]);
             handed(bar_vfull + 8u * st);
             fetch_v(i + 1);
             fetch_pages(i + 2);
@@ -372,7 +390,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             tmem_ld_wait();
             float v[32];
 #pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(r[e]) * PFT_SCALE;
+            for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(r[e]) * (PFT_SCALE / PPF_CENT<BITS>);
             put_frag(PpfSmem::Q + pslot * PFT_TILE, c0, v);
         }
         fence_proxy_async_smem();
@@ -405,17 +423,17 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                     const bool diagonal = col0 + PFT_KT - 1 > pos0 + my_first;  // (uniform for the slot)
                     const uint8_t* const norms = gb + PpfSmem::NORM + (uint32_t)(j & (PPF_NSTAGES - 1)) * PpfSmem::NORM_BYTES;
                     const __half2* const nrm2 = reinterpret_cast<const __half2*>(norms) + t4;
-                    float v_top;  // the tile's largest V norm
+                    bool select;  // a norm of V that is not finite in the tile
                     {
-                        uint4 u = *reinterpret_cast<const uint4*>(norms + 4 * PFT_KT);
-                        uint32_t m = __vmaxu2(__vmaxu2(u.x, u.y), __vmaxu2(u.z, u.w));
+                        const uint4 u = *reinterpret_cast<const uint4*>(norms + 2 * PFT_KT);
+                        uint32_t any = u.x | u.y | u.z | u.w;
                         if (MT == 2) {
-                            u = *reinterpret_cast<const uint4*>(norms + 4 * PFT_KT + 16);
-                            m = __vmaxu2(m, __vmaxu2(__vmaxu2(u.x, u.y), __vmaxu2(u.z, u.w)));
+                            const uint4 w = *reinterpret_cast<const uint4*>(norms + 2 * PFT_KT + 16);
+                            any |= w.x | w.y | w.z | w.w;
                         }
-                        v_top = __half2float(__ushort_as_half((unsigned short)max(m & 0xffffu, m >> 16)));
+                        select = any != 0u;
                     }
-                    // Scores of 64 columns at a time, scaled by the K norms and masked: [row][column block].  The second half is read once for the
+                    // Scores of 64 columns at a time, masked: [row][column block].  The second half is read once for the
                     // row maxima and once more for its weights: with all 128 in registers the compiler spilled, and what is spilled comes back
                     // from L2 (shared memory leaves no L1): 4 x 1024 tokens behind 8192 took 990 us, 60 % of them waits for such loads.
                     auto scores = [&](int c, float2 (&x)[2][8]) {
@@ -423,11 +441,9 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                         tmem_ld_frag64(s_col + 64u * c, r);
                         tmem_ld_wait();
 #pragma unroll
-                        for (int b = 0; b < 8; ++b) {
-                            const float2 k2 = __half22float2(nrm2[32 * c + 4 * b]);
+                        for (int b = 0; b < 8; ++b)
 #pragma unroll
-                            for (int h = 0; h < 2; ++h) x[h][b] = mul2(make_float2(__uint_as_float(r[4 * b + 2 * h]), __uint_as_float(r[4 * b + 2 * h + 1])), k2);
-                        }
+                            for (int h = 0; h < 2; ++h) x[h][b] = make_float2(__uint_as_float(r[4 * b + 2 * h]), __uint_as_float(r[4 * b + 2 * h + 1]));
                         if (diagonal) {
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
@@ -463,9 +479,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                         mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
                         mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
                     }
-                    // (weights of up to 2^PFT_SLACK times a norm of 4094 still fit fp16; a tile with a larger one keeps its weights below 1)
-                    const float slack = v_top <= 65504.0f / (float)(1 << (int)PFT_SLACK) ? PFT_SLACK : 0.0f;
-                    const bool grew0 = mx[0] > m_run[0] + slack, grew1 = mx[1] > m_run[1] + slack;
+                    const bool grew0 = mx[0] > m_run[0] + PFT_SLACK, grew1 = mx[1] > m_run[1] + PFT_SLACK;
                     if (__any_sync(0xffffffffu, grew0 || grew1)) {
                         const float mn0 = grew0 ? mx[0] : m_run[0], mn1 = grew1 ? mx[1] : m_run[1];
                         const float corr0 = ex2_approx(m_run[0] - mn0), corr1 = ex2_approx(m_run[1] - mn1);
@@ -483,7 +497,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                             }
                         }
                     }
-                    // ---- P (times the V norm) as fp16 over S ----
+                    // ---- P as fp16 over S ----
                     float2 lsum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
                     float2 minus[2];
 #pragma unroll
@@ -493,7 +507,8 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                         uint32_t pr[16];
 #pragma unroll
                         for (int b = 0; b < 8; ++b) {
-                            const float2 v2 = __half22float2(nrm2[64 + 32 * c + 4 * b]);
+                            float2 v2;
+                            if constexpr (decltype(masked_is_zero)::value) v2 = __half22float2(nrm2[32 * c + 4 * b]);
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
                                 float2 a = add2(x[h][b], minus[h]);
@@ -501,15 +516,11 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                                 lsum[h] = add2(lsum[h], a);
                                 if constexpr (decltype(masked_is_zero)::value)
                                     a = make_float2(x[h][b].x <= -1e30f ? 0.0f : a.x * v2.x, x[h][b].y <= -1e30f ? 0.0f : a.y * v2.y);
-                                else
-                                    a = mul2(a, v2);
                                 pr[2 * b + h] = pack_half2(a.x, a.y);
                             }
                         }
                         tmem_st_pack32(s_col + 32u * c, pr);
                     };
-                    // a masked weight is 0, and 0 times a V norm that is not finite is not: a tile with such a norm selects instead
-                    const bool select = diagonal && !(v_top < INFINITY);
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
                         if (c) scores(1, x);
@@ -537,8 +548,8 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         float w0[2], w1[2] = {0.0f, 0.0f};  // by row: weights of the slots' sums, normalised (MT = 2: of its own; SPLIT: not normalised)
         float M_all[2], Z_all[2];
         if constexpr (MT == 1) {
-            named_barrier(2, 32 * PFT_SOFT_WARPS);  // (the other slot's last norms have been read)
-            float2* const xch = reinterpret_cast<float2*>(gb + PpfSmem::NORM);
+            named_barrier(2, 32 * PFT_SOFT_WARPS);  // (every warp has made its last tile)
+            float2* const xch = reinterpret_cast<float2*>(gb + PPF_XCH);
             if (t4 == 0) {
                 xch[slot * 128 + row0 + gl] = make_float2(m_run[0], l_run[0]);
                 xch[slot * 128 + row0 + gl + 8] = make_float2(m_run[1], l_run[1]);
@@ -550,13 +561,13 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                 const float M = fmaxf(a.x, b.x), e0 = n0 > 0 ? ex2_approx(a.x - M) : 0.0f, e1 = n1 > 0 ? ex2_approx(b.x - M) : 0.0f;
                 M_all[h] = M;
                 Z_all[h] = a.y * e0 + b.y * e1;
-                const float inv = SPLIT ? 1.0f : 1.0f / (Z_all[h] + 1e-8f);
+                const float inv = (1.0f / PPF_CENT<BITS>) * (SPLIT ? 1.0f : 1.0f / (Z_all[h] + 1e-8f));
                 w0[h] = e0 * inv;
                 w1[h] = e1 * inv;
             }
         } else {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) w0[h] = 1.0f / (l_run[h] + 1e-8f);
+            for (int h = 0; h < 2; ++h) w0[h] = (1.0f / PPF_CENT<BITS>) / (l_run[h] + 1e-8f);
         }
         // rows that attend to nothing (no tile at all, or none up to their position) give zeros whatever tensor memory holds
         const bool on[2] = {last0 >= 0 && (MT == 1 || nt > 0), last1 >= 0 && (MT == 1 || nt > 0)};
