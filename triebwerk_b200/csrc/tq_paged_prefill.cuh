@@ -10,9 +10,9 @@
 //     every K and V tile; MT = 1: one block, whose two slots take the even and the odd tiles and are combined at the end.
 //   * The 16 softmax warps are the producers too: a thread fetches 16 (2-bit: 8) bytes of one row of the next K and V tile into registers
 //     as soon as it has made the present one (their page's number before that), and turns them into centroids through a shared-memory table with a column
-//     per lane: K of tile j + 1 before it waits for S(j), V of tile j + 1 after its weights P(j) are out.  So the table look-ups and
-//     operand stores fill the time in which the tensor core works on the slot's own products.
-//   * MT = 2: all 16 warps make a share of every tile.  MT = 1: a slot's warps make that slot's tiles, and nothing ties the slots.
+//     per lane.  So the table look-ups and operand stores fill the time in which the tensor core works on the slot's own products.
+//   * All 16 warps make a share of every tile.  MT = 2: K of tile j + 1 before the softmax of tile j, V behind it.  MT = 1: after tile j, which is
+//     one slot's, K of tile j + 2 and V of tile j + 1, so that the other slot's warps need not wait for tile j's products.
 //   * SPLIT (MT = 1): few query rows, long contexts: the tiles of a block are cut into gridDim.z parts, whose sums meet in
 //     paged_merge_kernel.
 // Blocks are found without a table: request g's blocks begin at floor(start[g] / BT) + g (BT query tokens a CTA), which leaves room for
@@ -114,15 +114,14 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             atomicMax(p.status, ST_TMA_WAIT_TIMEOUT);
         }
     };
-    constexpr int MAKERS = MT == 2 ? PFT_SOFT_WARPS : PFT_SOFT_WARPS / 2;  // warps that make a tile
     if (warp == 0) {
         tmem_alloc(ctrl + 128u, 512u);
         tmem_relinquish();
     }
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(bar_kfull + 8u * i, MAKERS);
-            mbar_init(bar_vfull + 8u * i, MAKERS);
+            mbar_init(bar_kfull + 8u * i, PFT_SOFT_WARPS);
+            mbar_init(bar_vfull + 8u * i, PFT_SOFT_WARPS);
             mbar_init(bar_kfree + 8u * i, 1);
             mbar_init(bar_vfree + 8u * i, 1);
             mbar_init(bar_sfull + 8u * i, 1);
@@ -267,47 +266,42 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     } else {
         // ================= operands and softmax =================
         regs_inc<PPF_REGS_SOFT>();
-        // ---- a thread's rows of the tiles: piece mk & 3 of row (mk >> 2) (MT = 1: and of the row 64 further on) ----
-        constexpr int ROWS = MT == 2 ? 1 : 2;
-        const int mk = MT == 2 ? tid : 128 * (warp >> 3) + 32 * (warp & 3) + lane;  // (MT = 1: number among the slot's 256 threads)
-        const int mrow = mk >> 2, piece = mk & 3;
-        const int my_tiles = MT == 2 ? n_tiles : (slot ? n1 : n0);  // tiles that this thread has a share in
-        constexpr int FORMS = 4;                                    // 16-byte pieces of fp16 per share
-        uint4 kc[ROWS], vc[ROWS];                                   // codes of the next tile (2-bit: x, y)
-        unsigned short nrm[ROWS];                                   // piece 0: K norm, piece 1: V norm of the row
-        uint32_t vn[ROWS];                                          // the factor of V's row, from make_k to make_v of a tile
-        uint32_t page[ROWS];                                        // of the tile after it
+        // ---- a thread's share of every tile: piece tid & 3 of row tid >> 2 ----
+        const int mrow = tid >> 2, piece = tid & 3;
+        constexpr int FORMS = 4;        // 16-byte pieces of fp16 per share
+        uint4 kc, vc;                   // codes of the next tile (2-bit: x, y)
+        unsigned short nrm;             // piece 0: K norm, piece 1: V norm of the row
+        uint32_t vn = 0u, vn_next = 0u; // the factor of V's row, from make_k to make_v of a tile
+        uint32_t page, page_v;          // of the tile whose K (V) codes come next
         const int* const my_pages = p.block_table + (size_t)g * p.table_stride;
-        auto first_token = [&](int i) { return (t_lo + (MT == 2 ? i : 2 * i + slot)) * PFT_KT; };
-        auto fetch_pages = [&](int i) {
-#pragma unroll
-            for (int r = 0; r < ROWS; ++r) {
-                const int t = first_token(i) + mrow + 64 * r;
-                page[r] = 0u;
-                if (i < my_tiles && t < L) page[r] = min((uint32_t)__ldg(my_pages + (t >> p.page_shift)), (uint32_t)p.num_pages - 1u);
-            }
+        auto token = [&](int j) { return (t_lo + j) * PFT_KT + mrow; };
+        auto fetch_page = [&](int j) {
+            const int t = token(j);
+            page = 0u;
+            if (j < n_tiles && t < L) page = min((uint32_t)__ldg(my_pages + (t >> p.page_shift)), (uint32_t)p.num_pages - 1u);
         };
         // (rows behind the request's last: zeros, so that nothing of them counts)
-        auto fetch_codes = [&](int i, const uint8_t* codes, uint4 (&c)[ROWS], bool norms) {
-#pragma unroll
-            for (int r = 0; r < ROWS; ++r) {
-                const int t = first_token(i) + mrow + 64 * r;
-                c[r] = make_uint4(0u, 0u, 0u, 0u);
-                if (norms) nrm[r] = 0;
-                if (i < my_tiles && t < L) {
-                    const size_t at = ((((size_t)page[r] << p.page_shift) + (size_t)(t & ((1 << p.page_shift) - 1))) * p.Hkv + kvh);
-                    if (BITS == 4) {
-                        c[r] = __ldg(reinterpret_cast<const uint4*>(codes + at * BPH) + piece);
-                    } else {
-                        const uint2 a = __ldg(reinterpret_cast<const uint2*>(codes + at * BPH) + piece);
-                        c[r].x = a.x; c[r].y = a.y;
-                    }
-                    if (norms && piece < 2) nrm[r] = __ldg(reinterpret_cast<const unsigned short*>(piece ? p.vn : p.kn) + at);
-                }
+        auto row_at = [&](uint32_t pg, int t) { return (((size_t)pg << p.page_shift) + (size_t)(t & ((1 << p.page_shift) - 1))) * p.Hkv + kvh; };
+        auto codes_at = [&](const uint8_t* codes, size_t at) {
+            if (BITS == 4) return __ldg(reinterpret_cast<const uint4*>(codes + at * BPH) + piece);
+            const uint2 a = __ldg(reinterpret_cast<const uint2*>(codes + at * BPH) + piece);
+            return make_uint4(a.x, a.y, 0u, 0u);
+        };
+        auto fetch_k = [&](int j) {
+            const int t = token(j);
+            kc = make_uint4(0u, 0u, 0u, 0u);
+            nrm = 0;
+            if (j < n_tiles && t < L) {
+                const size_t at = row_at(page, t);
+                kc = codes_at(p.ck, at);
+                if (piece < 2) nrm = __ldg(reinterpret_cast<const unsigned short*>(piece ? p.vn : p.kn) + at);
             }
         };
-        auto fetch_k = [&](int i) { fetch_codes(i, p.ck, kc, true); };
-        auto fetch_v = [&](int i) { fetch_codes(i, p.cv, vc, false); };
+        auto fetch_v = [&](int j) {
+            const int t = token(j);
+            vc = make_uint4(0u, 0u, 0u, 0u);
+            if (j < n_tiles && t < L) vc = codes_at(p.cv, row_at(page_v, t));
+        };
         uint32_t lut;  // (made here, behind the barrier that the table waits for: the look-ups take it into their address)
         asm volatile("mov.u32 %0, %1;" : "=r"(lut) : "r"(sb + PpfSmem::LUT + 4u * (uint32_t)lane) : "memory");
         // 32 codes as centroids times a norm into the row's 16-byte pieces 4 piece .. + 3 (in an order in which a quarter-warp's stores meet no
@@ -338,48 +332,47 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             __syncwarp();
             if (lane == 0) mbar_arrive(bar);
         };
-        const int maker = MT == 2 ? warp : 4 * (warp >> 3) + (warp & 3);
-        auto make_k = [&](int i) {  // the share's K codes and norms of tile i (among this thread's tiles); then the next tile's are requested
-            if (i >= my_tiles) return;
-            const int j = MT == 2 ? i : 2 * i + slot, st = j & 1;
+        // The share's K codes and norms of tile j; then the next tile's are requested.  K is made a tile ahead of V (MT = 1), or both are made of one
+        // tile.
+        auto make_k = [&](int j) {
+            if (j >= n_tiles) return;
+            const int st = j & 1;
             if (j >= 2) wait_bar(bar_kfree + 8u * st, (uint32_t)(((j >> 1) - 1) & 1));
             uint8_t* const norms = gb + PpfSmem::NORM + (uint32_t)(j & (PPF_NSTAGES - 1)) * PpfSmem::NORM_BYTES;
-            uint32_t top = 0u;
-#pragma unroll
-            for (int r = 0; r < ROWS; ++r) {
-                put_codes(PpfSmem::K + st * PFT_TILE, mrow + 64 * r, kc[r], __shfl_sync(0xffffffffu, (uint32_t)nrm[r], lane & ~3));
-                // V's norm goes into V too, unless it is not finite: it would reach queries that the token is hidden from (0 x inf).  Then the
-                // weights take it, those that count (below).
-                vn[r] = __shfl_sync(0xffffffffu, (uint32_t)nrm[r], (lane & ~3) | 1);
-                const bool odd = (vn[r] & 0x7fffu) >= 0x7c00u;
-                if (piece == 0) reinterpret_cast<unsigned short*>(norms)[mrow + 64 * r] = odd ? (unsigned short)vn[r] : (unsigned short)0x3c00u;
-                if (odd) {
-                    vn[r] = 0x3c00u;
-                    top = 1u;
-                }
-            }
-            top = __reduce_max_sync(0xffffffffu, top);
-            if (lane == 0) reinterpret_cast<unsigned short*>(norms + 2 * PFT_KT)[maker] = (unsigned short)top;
+            put_codes(PpfSmem::K + st * PFT_TILE, mrow, kc, __shfl_sync(0xffffffffu, (uint32_t)nrm, lane & ~3));
+            // V's norm goes into V too, unless it is not finite: it would reach queries that the token is hidden from (0 x inf).  Then the
+            // weights take it, those that count (below).
+            const uint32_t n_v = __shfl_sync(0xffffffffu, (uint32_t)nrm, (lane & ~3) | 1);
+            const bool odd = (n_v & 0x7fffu) >= 0x7c00u;
+            if (piece == 0) reinterpret_cast<unsigned short*>(norms)[mrow] = odd ? (unsigned short)n_v : (unsigned short)0x3c00u;
+            vn = vn_next;
+            vn_next = odd ? 0x3c00u : n_v;
+            if (MT == 2) vn = vn_next;
+            const bool any = __any_sync(0xffffffffu, odd);
+            if (lane == 0) reinterpret_cast<unsigned short*>(norms + 2 * PFT_KT)[warp] = any ? 1 : 0;
             handed(bar_kfull + 8u * st);
-            fetch_k(i + 1);
+            if (MT == 2) page_v = page;
+            fetch_k(j + 1);
         };
-        auto make_v = [&](int i) {  // ... its V codes; then the next tile's, and the pages of the one after it
-            if (i >= my_tiles) return;
-            const int j = MT == 2 ? i : 2 * i + slot, st = j & 1;
+        auto make_v = [&](int j) {  // ... its V codes; then the next tile's, and the page of the one whose K codes come next
+            if (j >= n_tiles) return;
+            const int st = j & 1;
             if (j >= 2) wait_bar(bar_vfree + 8u * st, (uint32_t)(((j >> 1) - 1) & 1));
-#pragma unroll
-            for (int r = 0; r < ROWS; ++r) put_codes(PpfSmem::V + st * PFT_TILE, mrow + 64 * r, vc[r], vn[r]);
+            put_codes(PpfSmem::V + st * PFT_TILE, mrow, vc, MT == 1 && j == n_tiles - 1 ? vn_next : vn);
             handed(bar_vfull + 8u * st);
-            fetch_v(i + 1);
-            fetch_pages(i + 2);
+            fetch_v(j + 1);
+            page_v = page;
+            fetch_page(MT == 1 && j > 0 ? j + 3 : j + 2);
         };
-        fetch_pages(0);
+        fetch_page(0);
+        page_v = page;
         fetch_k(0);
         fetch_v(0);
-        fetch_pages(1);
-        const bool k_waits = MT == 1 && slot == 1;  // (its first K tile goes where R is)
-        if (!k_waits) make_k(0);
-        if (!k_waits) make_v(0);
+        fetch_page(1);
+        make_k(0);
+        vn = vn_next;
+        page_v = page;
+        make_v(0);
         // ---- q_rot = Q . R^T, scaled by log2(e) / sqrt(128), back into the Q tiles ----
         wait_bar(bar_rot, 0u);
         tc_fence_after();
@@ -397,9 +390,10 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         tc_fence_before();
         named_barrier(1, PPF_MEET);
         tc_fence_after();
-        if (k_waits) {
-            make_k(0);
-            make_v(0);
+        if (MT == 1) {
+            make_k(1);  // (goes where R was)
+            page_v = page;
+            fetch_page(3);
         }
 
         // ---- softmax of slot `slot`, rows row0 + gl and row0 + gl + 8 ----
@@ -411,12 +405,11 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         // last token of a row of no query: none
         const int last0 = tok0 < n ? pos0 + tok0 : -1, last1 = tok1 < n ? pos0 + tok1 : -1;
         float m_run[2] = {-1e30f, -1e30f}, l_run[2] = {0.0f, 0.0f};  // (sums: of this thread's columns)
-        for (int i = 0; i < (MT == 2 ? n_tiles : nt); ++i) {
-            // (the tile's norms.  MT = 1: asked for before the slot's next tile, which uses the same barrier, is made)
-            const int j = tile_of(slot, i), col0 = (t_lo + j) * PFT_KT;
-            if (MT == 1 || i < nt) wait_bar(bar_kfull + 8u * (j & 1), (uint32_t)((j >> 1) & 1));
-            make_k(i + 1);
-            if (MT == 1 || i < nt) {
+        for (int j = 0; j < n_tiles; ++j) {
+            if (MT == 2) make_k(j + 1);
+            if (MT == 2 ? j < nt : (j & 1) == slot) {
+                const int i = MT == 2 ? j : j >> 1, col0 = (t_lo + j) * PFT_KT;
+                wait_bar(bar_kfull + 8u * (j & 1), (uint32_t)((j >> 1) & 1));  // (the tile's norms)
                 wait_bar(bar_sfull + 8u * slot, (uint32_t)(i & 1));
                 tc_fence_after();
                 if (some_row) {
@@ -534,7 +527,8 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                 tc_fence_before();
                 mbar_arrive(bar_pfull + 8u * slot);
             }
-            make_v(i + 1);
+            if (MT == 1) make_k(j + 2);
+            make_v(j + 1);
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
