@@ -244,12 +244,6 @@ static int launch_paged_prefill(const CUtensorMap& tmQ, const CUtensorMap& tmR, 
     auto kernel = paged_prefill_kernel<BITS, MT, SPLIT>;
     int r = ensure_dynamic_smem((const void*)kernel, PpfSmem::BYTES);
     if (r != TQ_OK) return r;
-    // the register split inside the kernel draws on what the launch brings: never launch with less
-    static const int regs = [] {
-        cudaFuncAttributes a{};
-        return cudaFuncGetAttributes(&a, (const void*)paged_prefill_kernel<BITS, MT, SPLIT>) == cudaSuccess ? a.numRegs : 0;
-    }();
-    if (regs < PPF_REGS_LAUNCH) return TQ_ERR_UNSUPPORTED;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(PPF_THREADS);

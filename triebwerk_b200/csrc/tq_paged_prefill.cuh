@@ -9,10 +9,11 @@
 //   * A block = 128 score rows = 128 / GRP query tokens x the GRP query heads of a KV head.  MT = 2: a CTA has two blocks, which share
 //     every K and V tile; MT = 1: one block, whose two slots take the even and the odd tiles and are combined at the end.
 //   * The 16 softmax warps are the producers too: a thread fetches 16 (2-bit: 8) bytes of one row of the next K and V tile into registers
-//     as soon as it has made the present one (their page's number before that), and turns them into centroids through a shared-memory table with a column
+//     as soon as it has made the present one, and turns them into centroids through a shared-memory table with a column
 //     per lane.  So the table look-ups and operand stores fill the time in which the tensor core works on the slot's own products.
 //   * All 16 warps make a share of every tile.  MT = 2: K of tile j + 1 before the softmax of tile j, V behind it.  MT = 1: after tile j, which is
 //     one slot's, K of tile j + 2 and V of tile j + 1, so that the other slot's warps need not wait for tile j's products.
+//   * Three warps fetch the tiles' rows (one page number for each 32 tokens) and norms ahead, into a ring in shared memory.
 //   * SPLIT (MT = 1): few query rows, long contexts: the tiles of a block are cut into gridDim.z parts, whose sums meet in
 //     paged_merge_kernel.
 // Blocks are found without a table: request g's blocks begin at floor(start[g] / BT) + g (BT query tokens a CTA), which leaves room for
@@ -39,23 +40,21 @@ struct PagedPrefillParams {
     int T, G, H, Hkv, grp, out_stride;
 };
 
-constexpr int PPF_THREADS = 32 * PFT_SOFT_WARPS + 128;  // softmax and operands; one warp for the products, three idle (a full warpgroup)
-constexpr int PPF_MEET = 32 * PFT_SOFT_WARPS + 32;      // those that work
-// Registers per thread of the softmax warpgroups and of the last one after the split, out of what the launch brings (the host checks it):
-// 640 x 96 = 512 x 104 + 128 x 64.
-constexpr int PPF_REGS_SOFT = 104, PPF_REGS_REST = 64;
-constexpr int PPF_REGS_LAUNCH = (32 * PFT_SOFT_WARPS * PPF_REGS_SOFT + 128 * PPF_REGS_REST + PPF_THREADS - 1) / PPF_THREADS;
-constexpr int PPF_NSTAGES = 4;                          // of norms: the slots may be that far apart
+constexpr int PPF_THREADS = 32 * PFT_SOFT_WARPS + 128;  // softmax and operands; one warp for the products, three for rows and norms
+constexpr int PPF_MEET = 32 * PFT_SOFT_WARPS + 32;      // all but those
+// (No register split: 96 each are enough, and the thread that issues the products spilled with fewer -- 64 for it, 104 for the rest, 4 x 1024 tokens
+// behind 8192 took 618 us, with 32 and 112 1072.)
+constexpr int PPF_STAGES = 4;                          // of a tile's norms and rows: fetched ahead, and the slots may be far apart
 struct PpfSmem {
     static constexpr uint32_t Q = 0;                       // 2 tiles; at the end: high parts of the results
     static constexpr uint32_t K = 2 * PFT_TILE;            // 2 stages; at the start R in the second; at the end: low parts
-    static constexpr uint32_t V = K + 2 * PFT_TILE;        // 2 stages; at the end R in the first
+    static constexpr uint32_t V = K + 2 * PFT_TILE;        // 2 stages; at the end R in the free one
     static constexpr uint32_t LUT = V + 2 * PFT_TILE;      // byte (4-bit) or nibble -> two centroids, a column per lane; at the end (MT = 1) the slots' maxima and sums
     static constexpr uint32_t LUT_BYTES = 32768u;
-    static constexpr uint32_t NORM = LUT + LUT_BYTES;      // [stage]: V's factors as halves, 16 warps' words: one that is not finite
-    static constexpr uint32_t NORM_BYTES = 2u * PFT_KT + 32u;
-    static constexpr uint32_t CTRL = NORM + PPF_NSTAGES * NORM_BYTES;
-    static constexpr uint32_t BYTES = CTRL + 192u;
+    static constexpr uint32_t INFO = LUT + LUT_BYTES;      // [stage]: K norms, V norms as halves, first row of each 32 tokens, a V norm that is not finite
+    static constexpr uint32_t INFO_ROWS = 4u * PFT_KT, INFO_ODD = INFO_ROWS + 16u, INFO_BYTES = INFO_ODD + 16u;
+    static constexpr uint32_t CTRL = INFO + PPF_STAGES * INFO_BYTES;
+    static constexpr uint32_t BYTES = CTRL + 256u;
 };
 static_assert(PpfSmem::BYTES <= 227 * 1024, "one CTA's shared memory");
 constexpr uint32_t PPF_XCH = PpfSmem::LUT;  // (the table is no longer needed then)
@@ -80,45 +79,18 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int GRP = p.grp, QT = PFT_ROWS / GRP, BT = MT * QT;
 
-    pdl_launch_dependents();
-    pdl_wait();  // (lengths, tables, caches, queries: all of earlier launches)
-    // ---- the request and the block of this CTA ----
-    const int ny = (int)(gridDim.x / (unsigned)p.Hkv);
-    const int kvh = (int)blockIdx.x % p.Hkv, y = ny - 1 - (int)blockIdx.x / p.Hkv;  // the longest causal prefixes of a request first
-    int g = -1;
-    for (int base = 0; base < p.G; base += PPF_THREADS) {
-        const int i = base + tid;
-        g += __syncthreads_count(i < p.G && p.start[i] / BT + i <= y);
-    }
-    if (g < 0) return;  // (never: request 0 begins at block 0)
-    const int s0 = max(p.start[g], 0), n = min(p.start[g + 1], p.T) - s0, q0 = (y - (s0 / BT + g)) * BT;
-    if (q0 >= n) return;
-    const int L = min(max(p.lens[g], 0), p.most_tokens), pos0 = L - n;  // position of the request's first new token
-    // tiles that the block whose first query is `first` reads
-    auto tiles_to = [&](int first) { return first < n ? max(pos0 + min(first + QT, n) - 1 + PFT_KT, 0) / PFT_KT : 0; };
-    const int t_lo = SPLIT ? (int)((long long)tiles_to(q0) * blockIdx.z / gridDim.z) : 0;
-    const int n_all = (SPLIT ? (int)((long long)tiles_to(q0) * (blockIdx.z + 1) / gridDim.z) : tiles_to(q0)) - t_lo;
-    const int n0 = MT == 2 ? n_all : (n_all + 1) / 2, n1 = MT == 2 ? tiles_to(q0 + QT) : n_all / 2;
-    const int n_tiles = MT == 2 ? max(n0, n1) : n_all;
-    auto tile_of = [&](int s, int i) { return MT == 2 ? i : 2 * i + s; };  // (behind t_lo)
-
+    // ---- once: tensor memory, barriers, table ----
     const uint32_t ctrl = sb + PpfSmem::CTRL;
     const uint32_t bar_kfull = ctrl, bar_vfull = ctrl + 16u, bar_kfree = ctrl + 32u, bar_vfree = ctrl + 48u;  // [2] each
     const uint32_t bar_sfull = ctrl + 64u, bar_pfull = ctrl + 80u;                                            // [2 slots] each
     const uint32_t bar_rot = ctrl + 96u, bar_done = ctrl + 104u, bar_q = ctrl + 112u, bar_r = ctrl + 120u;
-    volatile uint32_t* const tmem_slot = reinterpret_cast<volatile uint32_t*>(gb + PpfSmem::CTRL + 128);
-    bool dead = false;
-    auto wait_bar = [&](uint32_t bar, uint32_t parity) {
-        if (!dead && !mbar_try_wait(bar, parity) && !mbar_wait_bounded_hint(bar, parity, 1u << 17, 2000u)) {
-            dead = true;
-            atomicMax(p.status, ST_TMA_WAIT_TIMEOUT);
-        }
-    };
+    const uint32_t bar_rows = ctrl + 128u, bar_norms = ctrl + 160u, bar_used = ctrl + 192u;                   // [PPF_STAGES] each
+    volatile uint32_t* const tmem_slot = reinterpret_cast<volatile uint32_t*>(gb + PpfSmem::CTRL + 224);
     if (warp == 0) {
-        tmem_alloc(ctrl + 128u, 512u);
+        tmem_alloc(ctrl + 224u, 512u);
         tmem_relinquish();
     }
-    if (tid == 0) {
+    if (tid == 32 * MMA_WARP) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(bar_kfull + 8u * i, PFT_SOFT_WARPS);
             mbar_init(bar_vfull + 8u * i, PFT_SOFT_WARPS);
@@ -126,6 +98,11 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             mbar_init(bar_vfree + 8u * i, 1);
             mbar_init(bar_sfull + 8u * i, 1);
             mbar_init(bar_pfull + 8u * i, 16 * PFT_SOFT_WARPS);
+        }
+        for (int i = 0; i < PPF_STAGES; ++i) {
+            mbar_init(bar_rows + 8u * i, 1);
+            mbar_init(bar_norms + 8u * i, 1);
+            mbar_init(bar_used + 8u * i, PFT_SOFT_WARPS);
         }
         mbar_init(bar_rot, 1);
         mbar_init(bar_done, 1);
@@ -142,10 +119,31 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             *reinterpret_cast<uint4*>(gb + PpfSmem::LUT + 16u * (uint32_t)i) = make_uint4(u, u, u, u);
         }
     }
+    pdl_launch_dependents();
+    pdl_wait();  // (lengths, tables, caches, queries: all of earlier launches)
+    // ---- the request and the block of this CTA ----
+    const int ny = (int)(gridDim.x / (unsigned)p.Hkv);
+    const int kvh = (int)blockIdx.x % p.Hkv, y = ny - 1 - (int)blockIdx.x / p.Hkv;  // the longest causal prefixes of a request first
+    int g = -1;
     tc_fence_before();
-    __syncthreads();
+    for (int base = 0; base < p.G; base += PPF_THREADS) {  // (at least once: what was made above is in place)
+        const int i = base + tid;
+        g += __syncthreads_count(i < p.G && p.start[i] / BT + i <= y);
+    }
     tc_fence_after();
+    g = max(g, 0);  // (request 0 begins at block 0)
+    const uint32_t tmem = *tmem_slot;
+    const int s0 = max(p.start[g], 0), n = min(p.start[g + 1], p.T) - s0, q0 = (y - (s0 / BT + g)) * BT;
+    if (q0 >= n) {  // no such block
+        __syncthreads();
+        if (warp == 0) tmem_dealloc(tmem, 512u);
+        return;
+    }
+    volatile int* const kept = reinterpret_cast<volatile int*>(gb + PpfSmem::CTRL + 232);
     if (tid == 32 * MMA_WARP) {
+        kept[0] = s0;
+        kept[1] = n;
+        kept[2] = q0;
         mbar_arrive_expect_tx(bar_q, (uint32_t)(MT * QT * GRP) * 256u + PFT_TILE);
         for (int m = 0; m < MT; ++m) {  // (rows of other requests or past the end: a row's garbage stays in that row and is never stored)
             tma_load_4d(sb + PpfSmem::Q + m * PFT_TILE, &tmQ, bar_q, 0, kvh * GRP, s0 + q0 + m * QT, 0);
@@ -153,7 +151,22 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         }
         tma_load_3d(sb + PpfSmem::K + PFT_TILE, &tmR, bar_q, 0, 0, 0);
     }
-    const uint32_t tmem = *tmem_slot;
+    const int L = min(max(p.lens[g], 0), p.most_tokens), pos0 = L - n;  // position of the request's first new token
+    // tiles that the block whose first query is `first` reads
+    auto tiles_to = [&](int first) { return first < n ? max(pos0 + min(first + QT, n) - 1 + PFT_KT, 0) / PFT_KT : 0; };
+    const int t_lo = SPLIT ? (int)((long long)tiles_to(q0) * blockIdx.z / gridDim.z) : 0;
+    const int n_all = (SPLIT ? (int)((long long)tiles_to(q0) * (blockIdx.z + 1) / gridDim.z) : tiles_to(q0)) - t_lo;
+    const int n0 = MT == 2 ? n_all : (n_all + 1) / 2, n1 = MT == 2 ? tiles_to(q0 + QT) : n_all / 2;
+    const int n_tiles = MT == 2 ? max(n0, n1) : n_all;
+    auto tile_of = [&](int s, int i) { return MT == 2 ? i : 2 * i + s; };  // (behind t_lo)
+
+    bool dead = false;
+    auto wait_bar = [&](uint32_t bar, uint32_t parity) {
+        if (!dead && !mbar_try_wait(bar, parity) && !mbar_wait_bounded_hint(bar, parity, 1u << 17, 2000u)) {
+            dead = true;
+            atomicMax(p.status, ST_TMA_WAIT_TIMEOUT);
+        }
+    };
     const int slot = (warp >> 2) & 1, row0 = 32 * (warp & 3) + 16 * (warp >> 3), gl = lane >> 2, t4 = lane & 3;
     const int my_first = q0 + (MT == 2 ? slot * QT : 0);
     auto make_by_grp = [&]() {  // row / GRP by a multiplication, exact below 128
@@ -178,7 +191,6 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     const uint32_t pslot = MT == 2 ? (uint32_t)slot : 0u;
 
     if (warp >= MMA_WARP) {
-      regs_dec<PPF_REGS_REST>();
       if (warp == MMA_WARP) {
         // ================= one thread issues every product =================
         if (lane == 0) {
@@ -222,6 +234,14 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             };
             if (n0 > 0) issue_scores(0, 0);
             if (n1 > 0) issue_scores(1, 0);
+            // R again, for the results, where V of the tile in front of the last was: as soon as its products are done
+            auto fetch_rotation = [&]() {
+                if (SPLIT) return;
+                if (n_tiles >= 2) wait_bar(bar_vfree + 8u * (n_tiles & 1), (uint32_t)(((n_tiles - 2) >> 1) & 1));
+                if (dead) return;
+                mbar_arrive_expect_tx(bar_r, PFT_TILE);
+                tma_load_3d(sb + PpfSmem::V + (uint32_t)(n_tiles & 1) * PFT_TILE, &tmR, bar_r, 0, 0, 0);
+            };
             for (int i = 0; i < max(n0, n1); ++i) {
                 if (i < n0) {
                     issue_values(0, i);
@@ -233,13 +253,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                 }
             }
             umma_commit(bar_done);
-            if (!SPLIT) {
-                wait_bar(bar_done, 0u);
-                if (!dead) {
-                    mbar_arrive_expect_tx(bar_r, PFT_TILE);
-                    tma_load_3d(sb + PpfSmem::V, &tmR, bar_r, 0, 0, 0);
-                }
-            }
+            fetch_rotation();
         }
         __syncwarp();
         if (!SPLIT) {
@@ -256,51 +270,69 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 #pragma unroll
                             for (int ks = 0; ks < 8; ++ks)
                                 umma_lo(tmem + 128u * m, pft_lo_k(sb + (part ? PpfSmem::K : PpfSmem::Q) + m * PFT_TILE) + pft_kstep(ks),
-                                        pft_lo_mn(sb + PpfSmem::V) + 128u * ks, PFT_IDESC_MN, (part | ks) != 0);
+                                        pft_lo_mn(sb + PpfSmem::V + (uint32_t)(n_tiles & 1) * PFT_TILE) + 128u * ks, PFT_IDESC_MN, (part | ks) != 0);
                 }
                 umma_commit(bar_rot);
             }
             __syncwarp();
         }
+      } else {
+        // ================= rows and norms of the tiles, three warps in turn =================
+        const int* const my_pages = p.block_table + (size_t)g * p.table_stride;
+        for (int j = warp - MMA_WARP - 1; j < n_tiles; j += 3) {
+            const int st = j & (PPF_STAGES - 1), t0 = (t_lo + j) * PFT_KT;
+            if (j >= PPF_STAGES) wait_bar(bar_used + 8u * st, (uint32_t)((j / PPF_STAGES - 1) & 1));
+            uint8_t* const info = gb + PpfSmem::INFO + (uint32_t)st * PpfSmem::INFO_BYTES;
+            // pages hold 32 tokens at least.  (Behind the request's last token: some row of the cache; its norm counts as zero.)
+            uint32_t row = 0u;
+            if (lane < 4 && t0 + 32 * lane < L)
+                row = (min((uint32_t)__ldg(my_pages + ((t0 + 32 * lane) >> p.page_shift)), (uint32_t)p.num_pages - 1u) << p.page_shift) + (uint32_t)((t0 + 32 * lane) & ((1 << p.page_shift) - 1));
+            if (lane < 4) reinterpret_cast<uint32_t*>(info + PpfSmem::INFO_ROWS)[lane] = row;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_rows + 8u * st);
+            unsigned short kn[4], vn[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const size_t at = (size_t)(__shfl_sync(0xffffffffu, row, k) + (uint32_t)lane) * p.Hkv + kvh;
+                kn[k] = vn[k] = 0;
+                if (t0 + 32 * k + lane < L) {
+                    kn[k] = __ldg(reinterpret_cast<const unsigned short*>(p.kn) + at);
+                    vn[k] = __ldg(reinterpret_cast<const unsigned short*>(p.vn) + at);
+                }
+            }
+            bool odd = false;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                reinterpret_cast<unsigned short*>(info)[32 * k + lane] = kn[k];
+                reinterpret_cast<unsigned short*>(info)[PFT_KT + 32 * k + lane] = vn[k];
+                odd = odd || (vn[k] & 0x7fffu) >= 0x7c00u;
+            }
+            odd = __any_sync(0xffffffffu, odd);
+            __syncwarp();
+            if (lane == 0) {
+                *reinterpret_cast<uint32_t*>(info + PpfSmem::INFO_ODD) = odd ? 1u : 0u;
+                mbar_arrive(bar_norms + 8u * st);
+            }
+        }
       }
     } else {
         // ================= operands and softmax =================
-        regs_inc<PPF_REGS_SOFT>();
         // ---- a thread's share of every tile: piece tid & 3 of row tid >> 2 ----
         const int mrow = tid >> 2, piece = tid & 3;
         constexpr int FORMS = 4;        // 16-byte pieces of fp16 per share
         uint4 kc, vc;                   // codes of the next tile (2-bit: x, y)
-        unsigned short nrm;             // piece 0: K norm, piece 1: V norm of the row
-        uint32_t vn = 0u, vn_next = 0u; // the factor of V's row, from make_k to make_v of a tile
-        uint32_t page, page_v;          // of the tile whose K (V) codes come next
-        const int* const my_pages = p.block_table + (size_t)g * p.table_stride;
-        auto token = [&](int j) { return (t_lo + j) * PFT_KT + mrow; };
-        auto fetch_page = [&](int j) {
-            const int t = token(j);
-            page = 0u;
-            if (j < n_tiles && t < L) page = min((uint32_t)__ldg(my_pages + (t >> p.page_shift)), (uint32_t)p.num_pages - 1u);
-        };
-        // (rows behind the request's last: zeros, so that nothing of them counts)
-        auto row_at = [&](uint32_t pg, int t) { return (((size_t)pg << p.page_shift) + (size_t)(t & ((1 << p.page_shift) - 1))) * p.Hkv + kvh; };
-        auto codes_at = [&](const uint8_t* codes, size_t at) {
-            if (BITS == 4) return __ldg(reinterpret_cast<const uint4*>(codes + at * BPH) + piece);
-            const uint2 a = __ldg(reinterpret_cast<const uint2*>(codes + at * BPH) + piece);
-            return make_uint4(a.x, a.y, 0u, 0u);
-        };
-        auto fetch_k = [&](int j) {
-            const int t = token(j);
-            kc = make_uint4(0u, 0u, 0u, 0u);
-            nrm = 0;
-            if (j < n_tiles && t < L) {
-                const size_t at = row_at(page, t);
-                kc = codes_at(p.ck, at);
-                if (piece < 2) nrm = __ldg(reinterpret_cast<const unsigned short*>(piece ? p.vn : p.kn) + at);
+        auto info_of = [&](int j) { return gb + PpfSmem::INFO + (uint32_t)(j & (PPF_STAGES - 1)) * PpfSmem::INFO_BYTES; };
+        auto fetch = [&](int j, const uint8_t* codes, uint4& c) {
+            if (j >= n_tiles) return;
+            wait_bar(bar_rows + 8u * (j & (PPF_STAGES - 1)), (uint32_t)((j / PPF_STAGES) & 1));
+            const uint32_t row = reinterpret_cast<const uint32_t*>(info_of(j) + PpfSmem::INFO_ROWS)[mrow >> 5] + (uint32_t)(mrow & 31);
+            const uint8_t* const src = codes + ((size_t)row * (uint32_t)p.Hkv + (uint32_t)kvh) * BPH;
+            if (BITS == 4) {
+                c = __ldg(reinterpret_cast<const uint4*>(src) + piece);
+            } else {
+                const uint2 a = __ldg(reinterpret_cast<const uint2*>(src) + piece);
+                c.x = a.x; c.y = a.y;
             }
-        };
-        auto fetch_v = [&](int j) {
-            const int t = token(j);
-            vc = make_uint4(0u, 0u, 0u, 0u);
-            if (j < n_tiles && t < L) vc = codes_at(p.cv, row_at(page_v, t));
         };
         uint32_t lut;  // (made here, behind the barrier that the table waits for: the look-ups take it into their address)
         asm volatile("mov.u32 %0, %1;" : "=r"(lut) : "r"(sb + PpfSmem::LUT + 4u * (uint32_t)lane) : "memory");
@@ -332,46 +364,31 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             __syncwarp();
             if (lane == 0) mbar_arrive(bar);
         };
-        // The share's K codes and norms of tile j; then the next tile's are requested.  K is made a tile ahead of V (MT = 1), or both are made of one
-        // tile.
+        // The share's K codes of tile j; then the next tile's are requested.
         auto make_k = [&](int j) {
             if (j >= n_tiles) return;
             const int st = j & 1;
+            wait_bar(bar_norms + 8u * (j & (PPF_STAGES - 1)), (uint32_t)((j / PPF_STAGES) & 1));
             if (j >= 2) wait_bar(bar_kfree + 8u * st, (uint32_t)(((j >> 1) - 1) & 1));
-            uint8_t* const norms = gb + PpfSmem::NORM + (uint32_t)(j & (PPF_NSTAGES - 1)) * PpfSmem::NORM_BYTES;
-            put_codes(PpfSmem::K + st * PFT_TILE, mrow, kc, __shfl_sync(0xffffffffu, (uint32_t)nrm, lane & ~3));
-            // V's norm goes into V too, unless it is not finite: it would reach queries that the token is hidden from (0 x inf).  Then the
-            // weights take it, those that count (below).
-            const uint32_t n_v = __shfl_sync(0xffffffffu, (uint32_t)nrm, (lane & ~3) | 1);
-            const bool odd = (n_v & 0x7fffu) >= 0x7c00u;
-            if (piece == 0) reinterpret_cast<unsigned short*>(norms)[mrow] = odd ? (unsigned short)n_v : (unsigned short)0x3c00u;
-            vn = vn_next;
-            vn_next = odd ? 0x3c00u : n_v;
-            if (MT == 2) vn = vn_next;
-            const bool any = __any_sync(0xffffffffu, odd);
-            if (lane == 0) reinterpret_cast<unsigned short*>(norms + 2 * PFT_KT)[warp] = any ? 1 : 0;
+            put_codes(PpfSmem::K + st * PFT_TILE, mrow, kc, reinterpret_cast<const unsigned short*>(info_of(j))[mrow]);
             handed(bar_kfull + 8u * st);
-            if (MT == 2) page_v = page;
-            fetch_k(j + 1);
+            fetch(j + 1, p.ck, kc);
         };
-        auto make_v = [&](int j) {  // ... its V codes; then the next tile's, and the page of the one whose K codes come next
+        // ... its V codes.  V's norm goes into V too, unless it is not finite: it would reach queries that the token is hidden from (0 x inf).
+        // Then the weights take it, those that count (below).
+        auto make_v = [&](int j) {
             if (j >= n_tiles) return;
             const int st = j & 1;
             if (j >= 2) wait_bar(bar_vfree + 8u * st, (uint32_t)(((j >> 1) - 1) & 1));
-            put_codes(PpfSmem::V + st * PFT_TILE, mrow, vc, MT == 1 && j == n_tiles - 1 ? vn_next : vn);
+            const uint32_t norm = reinterpret_cast<const unsigned short*>(info_of(j))[PFT_KT + mrow];
+            put_codes(PpfSmem::V + st * PFT_TILE, mrow, vc, (norm & 0x7fffu) >= 0x7c00u ? 0x3c00u : norm);
             handed(bar_vfull + 8u * st);
-            fetch_v(j + 1);
-            page_v = page;
-            fetch_page(MT == 1 && j > 0 ? j + 3 : j + 2);
+            fetch(j + 1, p.cv, vc);
         };
-        fetch_page(0);
-        page_v = page;
-        fetch_k(0);
-        fetch_v(0);
-        fetch_page(1);
+        kc = vc = make_uint4(0u, 0u, 0u, 0u);
+        fetch(0, p.ck, kc);
+        fetch(0, p.cv, vc);
         make_k(0);
-        vn = vn_next;
-        page_v = page;
         make_v(0);
         // ---- q_rot = Q . R^T, scaled by log2(e) / sqrt(128), back into the Q tiles ----
         wait_bar(bar_rot, 0u);
@@ -390,14 +407,10 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         tc_fence_before();
         named_barrier(1, PPF_MEET);
         tc_fence_after();
-        if (MT == 1) {
-            make_k(1);  // (goes where R was)
-            page_v = page;
-            fetch_page(3);
-        }
+        if (MT == 1) make_k(1);  // (goes where R was)
 
         // ---- softmax of slot `slot`, rows row0 + gl and row0 + gl + 8 ----
-        const uint32_t s_col = my_lanes + 128u * slot, o_col = my_lanes + 256u + 128u * slot;
+        const uint32_t s_col = my_lanes + 128u * slot, o_col = s_col + 256u;
         const int nt = slot ? n1 : n0;
         const uint32_t by_grp0 = make_by_grp();
         const int tok0 = token_of(row0 + gl, by_grp0), tok1 = token_of(row0 + gl + 8, by_grp0);
@@ -409,23 +422,12 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             if (MT == 2) make_k(j + 1);
             if (MT == 2 ? j < nt : (j & 1) == slot) {
                 const int i = MT == 2 ? j : j >> 1, col0 = (t_lo + j) * PFT_KT;
-                wait_bar(bar_kfull + 8u * (j & 1), (uint32_t)((j >> 1) & 1));  // (the tile's norms)
                 wait_bar(bar_sfull + 8u * slot, (uint32_t)(i & 1));
                 tc_fence_after();
                 if (some_row) {
                     const bool diagonal = col0 + PFT_KT - 1 > pos0 + my_first;  // (uniform for the slot)
-                    const uint8_t* const norms = gb + PpfSmem::NORM + (uint32_t)(j & (PPF_NSTAGES - 1)) * PpfSmem::NORM_BYTES;
-                    const __half2* const nrm2 = reinterpret_cast<const __half2*>(norms) + t4;
-                    bool select;  // a norm of V that is not finite in the tile
-                    {
-                        const uint4 u = *reinterpret_cast<const uint4*>(norms + 2 * PFT_KT);
-                        uint32_t any = u.x | u.y | u.z | u.w;
-                        if (MT == 2) {
-                            const uint4 w = *reinterpret_cast<const uint4*>(norms + 2 * PFT_KT + 16);
-                            any |= w.x | w.y | w.z | w.w;
-                        }
-                        select = any != 0u;
-                    }
+                    const uint8_t* const info = info_of(j);
+                    const bool select = *reinterpret_cast<const uint32_t*>(info + PpfSmem::INFO_ODD) != 0u;  // a norm of V that is not finite
                     // Scores of 64 columns at a time, masked: [row][column block].  The second half is read once for the
                     // row maxima and once more for its weights: with all 128 in registers the compiler spilled, and what is spilled comes back
                     // from L2 (shared memory leaves no L1): 4 x 1024 tokens behind 8192 took 990 us, 60 % of them waits for such loads.
@@ -501,7 +503,11 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 #pragma unroll
                         for (int b = 0; b < 8; ++b) {
                             float2 v2;
-                            if constexpr (decltype(masked_is_zero)::value) v2 = __half22float2(nrm2[32 * c + 4 * b]);
+                            if constexpr (decltype(masked_is_zero)::value) {
+                                v2 = __half22float2(reinterpret_cast<const __half2*>(info + 2 * PFT_KT)[32 * c + 4 * b + t4]);
+                                if (fabsf(v2.x) < INFINITY) v2.x = 1.0f;
+                                if (fabsf(v2.y) < INFINITY) v2.y = 1.0f;
+                            }
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
                                 float2 a = add2(x[h][b], minus[h]);
@@ -527,6 +533,8 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                 tc_fence_before();
                 mbar_arrive(bar_pfull + 8u * slot);
             }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_used + 8u * (j & (PPF_STAGES - 1)));
             if (MT == 1) make_k(j + 2);
             make_v(j + 1);
         }
@@ -537,6 +545,10 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         }
         wait_bar(bar_done, 0u);  // every product has completed (and nobody reads the norms any more)
         tc_fence_after();
+        // (what only the end needs waits in shared memory: kept in registers it was spilled, see above)
+        const int s0_e = kept[0], n_e = kept[1], first_e = kept[2] + (MT == 2 ? slot * QT : 0);
+        const uint32_t lanes_e = *tmem_slot + ((uint32_t)row0 << 16);
+        auto token_e = [&](int row, uint32_t by_grp) { return token_in(row, by_grp) < QT ? first_e + token_in(row, by_grp) : n_e; };
 
         // ================= results =================
         float w0[2], w1[2] = {0.0f, 0.0f};  // by row: weights of the slots' sums, normalised (MT = 2: of its own; SPLIT: not normalised)
@@ -570,13 +582,13 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 #pragma unroll
             for (int e = 0; e < 32; ++e) v[e] = 0.0f;
             if (MT == 2 ? nt > 0 : n0 > 0) {
-                tmem_ld_frag64((MT == 2 ? o_col : my_lanes + 256u) + (uint32_t)c0, r);
+                tmem_ld_frag64((MT == 2 ? o_col : lanes_e + 256u) + (uint32_t)c0, r);
                 tmem_ld_wait();
 #pragma unroll
                 for (int e = 0; e < 32; ++e) v[e] = on[(e >> 1) & 1] ? __uint_as_float(r[e]) * w0[(e >> 1) & 1] : 0.0f;
             }
             if (MT == 1 && n1 > 0) {
-                tmem_ld_frag64(my_lanes + 384u + (uint32_t)c0, r);
+                tmem_ld_frag64(lanes_e + 384u + (uint32_t)c0, r);
                 tmem_ld_wait();
 #pragma unroll
                 for (int e = 0; e < 32; ++e) v[e] = on[(e >> 1) & 1] ? fmaf(__uint_as_float(r[e]), w1[(e >> 1) & 1], v[e]) : 0.0f;
@@ -590,9 +602,9 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             result(c0, v);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int row = row0 + gl + 8 * h, tok = h ? tok1 : tok0;
-                if (tok >= n) continue;
-                float* const dst = p.partials + (((size_t)blockIdx.z * p.T + s0 + tok) * p.H + (size_t)(kvh * GRP + row - token_in(row, by_grp) * GRP)) * PART_STRIDE;
+                const int row = row0 + gl + 8 * h, tok = token_e(row, by_grp);
+                if (tok >= n_e) continue;
+                float* const dst = p.partials + (((size_t)blockIdx.z * p.T + s0_e + tok) * p.H + (size_t)(kvh * GRP + row - token_in(row, by_grp) * GRP)) * PART_STRIDE;
 #pragma unroll
                 for (int b = 0; b < 8; ++b) *reinterpret_cast<float2*>(dst + c0 + 8 * b + 2 * t4) = make_float2(v[4 * b + 2 * h], v[4 * b + 2 * h + 1]);
                 if (slot == 0 && t4 == 0) *reinterpret_cast<float2*>(dst + HEAD_DIM) = on[h] ? make_float2(M_all[h], Z_all[h]) : make_float2(-1e30f, 0.0f);
@@ -619,7 +631,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             for (int c0 = pcol0; c0 < pcol0 + PCOLS; c0 += 64) {
                 float v[32];
                 uint32_t r[32];
-                tmem_ld_frag64(my_lanes + 128u * pslot + (uint32_t)c0, r);
+                tmem_ld_frag64(lanes_e + 128u * pslot + (uint32_t)c0, r);
                 tmem_ld_wait();
 #pragma unroll
                 for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(r[e]);
@@ -628,11 +640,11 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             __syncwarp();
             constexpr int CH = PCOLS / 8;  // 16-byte pieces per row
             const uint32_t by_grp = make_by_grp();
-            __half* const out_seq = p.out + (size_t)s0 * p.out_stride;
+            __half* const out_seq = p.out + (size_t)s0_e * p.out_stride;
 #pragma unroll
             for (int k = 0; k < CH / 2; ++k) {
-                const int at = 32 * k + lane, row = row0 + at / CH, ch = (pcol0 >> 3) + at % CH, tok = token_of(row, by_grp);
-                if (tok < n) {
+                const int at = 32 * k + lane, row = row0 + at / CH, ch = (pcol0 >> 3) + at % CH, tok = token_e(row, by_grp);
+                if (tok < n_e) {
                     const uint4 u = *reinterpret_cast<const uint4*>(gb + qtile + pft_chunk(row, ch));
                     *(reinterpret_cast<uint4*>(out_seq + (size_t)tok * p.out_stride + (size_t)(kvh * GRP + row - token_in(row, by_grp) * GRP) * HEAD_DIM) + ch) = u;
                 }
