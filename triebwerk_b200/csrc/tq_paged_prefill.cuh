@@ -97,7 +97,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             mbar_init(bar_kfree + 8u * i, 1);
             mbar_init(bar_vfree + 8u * i, 1);
             mbar_init(bar_sfull + 8u * i, 1);
-            mbar_init(bar_pfull + 8u * i, 16 * PFT_SOFT_WARPS);
+            mbar_init(bar_pfull + 8u * i, PFT_SOFT_WARPS / 2);
         }
         for (int i = 0; i < PPF_STAGES; ++i) {
             mbar_init(bar_rows + 8u * i, 1);
@@ -322,31 +322,38 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         constexpr int FORMS = 4;        // 16-byte pieces of fp16 per share
         uint4 kc, vc;                   // codes of the next tile (2-bit: x, y)
         auto info_of = [&](int j) { return gb + PpfSmem::INFO + (uint32_t)(j & (PPF_STAGES - 1)) * PpfSmem::INFO_BYTES; };
+        // (four words in the order in which put_codes takes them)
         auto fetch = [&](int j, const uint8_t* codes, uint4& c) {
-            if (j >= n_tiles) return;
-            wait_bar(bar_rows + 8u * (j & (PPF_STAGES - 1)), (uint32_t)((j / PPF_STAGES) & 1));
             const uint32_t row = reinterpret_cast<const uint32_t*>(info_of(j) + PpfSmem::INFO_ROWS)[mrow >> 5] + (uint32_t)(mrow & 31);
             const uint8_t* const src = codes + ((size_t)row * (uint32_t)p.Hkv + (uint32_t)kvh) * BPH;
             if (BITS == 4) {
-                c = __ldg(reinterpret_cast<const uint4*>(src) + piece);
+                const uint2 a = __ldg(reinterpret_cast<const uint2*>(src + 16 * piece + 4 * (piece & 2))), b = __ldg(reinterpret_cast<const uint2*>(src + 16 * piece + 8 - 4 * (piece & 2)));
+                c = make_uint4(a.x, a.y, b.x, b.y);
             } else {
                 const uint2 a = __ldg(reinterpret_cast<const uint2*>(src) + piece);
                 c.x = a.x; c.y = a.y;
             }
         };
+        auto fetch_k = [&](int j) {  // (the norms' barrier: rows come before them)
+            if (j >= n_tiles) return;
+            wait_bar(bar_norms + 8u * (j & (PPF_STAGES - 1)), (uint32_t)((j / PPF_STAGES) & 1));
+            fetch(j, p.ck, kc);
+        };
+        auto fetch_v = [&](int j) {  // (K's fetch of that tile came before)
+            if (j < n_tiles) fetch(j, p.cv, vc);
+        };
         uint32_t lut;  // (made here, behind the barrier that the table waits for: the look-ups take it into their address)
         asm volatile("mov.u32 %0, %1;" : "=r"(lut) : "r"(sb + PpfSmem::LUT + 4u * (uint32_t)lane) : "memory");
-        // 32 codes as centroids times a norm into the row's 16-byte pieces 4 piece .. + 3 (in an order in which a quarter-warp's stores meet no
-        // bank twice).  The norm is in the operands, rounded to fp16 once more: for each score and weight, 64 a thread and tile, it cost a
-        // fifth of all instructions.
-        auto put_codes = [&](uint32_t tile, int row, const uint4 c, uint32_t norm) {
+        // 32 codes as centroids times a norm into the row's 16-byte pieces 4 piece .. + 3, in an order in which a quarter-warp's stores meet no
+        // bank twice: the f-th is piece f ^ (piece & 2) of the four.  The norm is in the operands, rounded to fp16 once more: for each score and
+        // weight, 64 a thread and tile, it cost a fifth of all instructions.
+        const uint32_t my_at = sb + (uint32_t)(piece >> 1) * (PFT_TILE / 2) + (uint32_t)mrow * 128u + (uint32_t)(((4 * (piece & 1)) ^ (piece & 2) ^ (mrow & 7)) << 4);
+        auto put_codes = [&](uint32_t tile, const uint4 c, uint32_t norm) {
             const __half2 n2 = __half2half2(__ushort_as_half((unsigned short)norm));
 #pragma unroll
-            for (int f = 0; f < FORMS; ++f) {
-                const int i = f ^ (piece & 2);
-                const uint32_t w = BITS == 4 ? ((f & 2) ? ((f & 1) ? ((piece & 2) ? c.y : c.w) : ((piece & 2) ? c.x : c.z))
-                                                        : ((f & 1) ? ((piece & 2) ? c.w : c.y) : ((piece & 2) ? c.z : c.x)))
-                                             : ((i & 2) ? c.y : c.x) >> ((f & 1) * 16);
+            for (int f = 0; f < 4; ++f) {
+                const uint32_t first = (piece & 2) ? c.y : c.x, second = (piece & 2) ? c.x : c.y;  // (2-bit: 16 bits a piece)
+                const uint32_t w = BITS == 4 ? (f == 0 ? c.x : f == 1 ? c.y : f == 2 ? c.z : c.w) : (f & 2 ? second : first) >> ((f & 1) * 16);
                 uint32_t u[4];
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
@@ -356,7 +363,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                     const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&u[b]), n2);
                     u[b] = *reinterpret_cast<const uint32_t*>(&v);
                 }
-                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(sb + tile + pft_chunk(row, 4 * piece + i)), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]) : "memory");
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"((my_at ^ (uint32_t)(f << 4)) + tile), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]) : "memory");
             }
         };
         auto handed = [&](uint32_t bar) {  // this warp's stores are in place
@@ -368,11 +375,10 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         auto make_k = [&](int j) {
             if (j >= n_tiles) return;
             const int st = j & 1;
-            wait_bar(bar_norms + 8u * (j & (PPF_STAGES - 1)), (uint32_t)((j / PPF_STAGES) & 1));
             if (j >= 2) wait_bar(bar_kfree + 8u * st, (uint32_t)(((j >> 1) - 1) & 1));
-            put_codes(PpfSmem::K + st * PFT_TILE, mrow, kc, reinterpret_cast<const unsigned short*>(info_of(j))[mrow]);
+            put_codes(PpfSmem::K + st * PFT_TILE, kc, reinterpret_cast<const unsigned short*>(info_of(j))[mrow]);
             handed(bar_kfull + 8u * st);
-            fetch(j + 1, p.ck, kc);
+            fetch_k(j + 1);
         };
         // ... its V codes.  V's norm goes into V too, unless it is not finite: it would reach queries that the token is hidden from (0 x inf).
         // Then the weights take it, those that count (below).
@@ -381,15 +387,18 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             const int st = j & 1;
             if (j >= 2) wait_bar(bar_vfree + 8u * st, (uint32_t)(((j >> 1) - 1) & 1));
             const uint32_t norm = reinterpret_cast<const unsigned short*>(info_of(j))[PFT_KT + mrow];
-            put_codes(PpfSmem::V + st * PFT_TILE, mrow, vc, (norm & 0x7fffu) >= 0x7c00u ? 0x3c00u : norm);
+            put_codes(PpfSmem::V + st * PFT_TILE, vc, (norm & 0x7fffu) >= 0x7c00u ? 0x3c00u : norm);
             handed(bar_vfull + 8u * st);
-            fetch(j + 1, p.cv, vc);
+            fetch_v(j + 1);
         };
         kc = vc = make_uint4(0u, 0u, 0u, 0u);
-        fetch(0, p.ck, kc);
-        fetch(0, p.cv, vc);
+        if (n_tiles > 0) {  // (the first tile's norms are on their way while its codes are)
+            wait_bar(bar_rows, 0u);
+            fetch(0, p.ck, kc);
+            fetch(0, p.cv, vc);
+            wait_bar(bar_norms, 0u);
+        }
         make_k(0);
-        make_v(0);
         // ---- q_rot = Q . R^T, scaled by log2(e) / sqrt(128), back into the Q tiles ----
         wait_bar(bar_rot, 0u);
         tc_fence_after();
@@ -407,6 +416,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         tc_fence_before();
         named_barrier(1, PPF_MEET);
         tc_fence_after();
+        make_v(0);
         if (MT == 1) make_k(1);  // (goes where R was)
 
         // ---- softmax of slot `slot`, rows row0 + gl and row0 + gl + 8 ----
@@ -465,10 +475,11 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                         }
                     };
                     float2 x[2][8];
-                    scores(1, x);
-                    largest(x);
-                    scores(0, x);
-                    largest(x);
+#pragma unroll
+                    for (int c = 1; c >= 0; --c) {
+                        scores(c, x);
+                        largest(x);
+                    }
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
@@ -531,9 +542,9 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                     tmem_st_wait();
                 }
                 tc_fence_before();
-                mbar_arrive(bar_pfull + 8u * slot);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar_pfull + 8u * slot);
             }
-            __syncwarp();
             if (lane == 0) mbar_arrive(bar_used + 8u * (j & (PPF_STAGES - 1)));
             if (MT == 1) make_k(j + 2);
             make_v(j + 1);
