@@ -4,6 +4,7 @@
 #include "tq_host.cuh"
 #include "tq_paged.cuh"
 #include "tq_paged_prefill.cuh"
+#include "tq_paged_rows.cuh"
 
 using namespace tq;
 
@@ -147,29 +148,40 @@ int tq_paged_read(void* k_out, void* v_out, const uint8_t* ck_q, const void* k_n
 
 }  // extern "C"
 
-// How a prefill call's work is cut: blocks per CTA (MT) and parts of a block's tiles.  The host knows the tokens of all requests
-// together, so it goes by their mean.
+// How a prefill call's work is cut.  The host knows the tokens of all requests together, so it goes by their mean.
 struct PrefillCut {
-    int mt, splits;
+    bool small, large;   // whether there may be requests of up to, of more than ROWS_MOST score rows
+    int ncb, parts;      // small ones: row blocks of 8 per CTA, parts of a request's tokens
+    int mt, splits;      // large ones: blocks of 128 rows per CTA, parts of a block's tiles
 };
 constexpr int SPLIT_SMS = 160, MAX_SPLITS = 16;
 static PrefillCut prefill_cut(int T, int G, int H, int Hkv, int most) {
-    const long long sms = std::min(device_props().sm_count, SPLIT_SMS), qt = PFT_ROWS / (H / Hkv), mean = (T + G - 1) / G;
-    const long long blocks1 = (long long)Hkv * G * ((mean + qt - 1) / qt), blocks2 = (long long)Hkv * G * ((mean + 2 * qt - 1) / (2 * qt));
-    if (mean > qt && 4 * blocks2 >= 5 * sms) return {2, 1};
-    const long long tiles = (most + PFT_KT - 1) / PFT_KT;
-    const long long splits = std::min({sms / std::max(blocks1, 1ll), tiles / 4, (long long)MAX_SPLITS});
-    return {1, (int)std::max(splits, 1ll)};
+    const long long sms = std::min(device_props().sm_count, SPLIT_SMS), grp = H / Hkv, qt = PFT_ROWS / grp, mean = (T + G - 1) / G;
+    PrefillCut c{};
+    c.small = grp <= ROWS_MOST && (G > 1 || T * grp <= ROWS_MOST);
+    c.large = grp > ROWS_MOST || T * grp > ROWS_MOST;
+    c.ncb = mean * grp <= 8 ? 1 : 2;
+    // One and a half turns of two CTAs per SM, four tiles of 16 tokens a warp at least.  (us by parts 1, 2, 3, 4, 8: 2-bit 32/8 heads 32 x 5 behind 4000 97 / 88 / 91 / 96 /
+    // 121; 4-bit 64 x 1 behind 2000 66 / 75 / 86 / 96 / 141; 16/8 heads 3 x 4 behind 9000 94 / 59 / 47 / 39 / 28.)
+    const long long ctas = (long long)Hkv * std::min((long long)G, (long long)T), room = 2 * sms;
+    c.parts = (int)std::max(1ll, std::min({(3 * room + ctas) / (2 * ctas), (long long)most / (16 * ROWS_WARPS * 4), (long long)MAX_SPLITS}));
+    const long long blocks1 = Hkv * G * ((mean + qt - 1) / qt), blocks2 = Hkv * G * ((mean + 2 * qt - 1) / (2 * qt));
+    c.mt = mean > qt && 4 * blocks2 >= 5 * sms ? 2 : 1;
+    c.splits = c.mt == 2 ? 1 : (int)std::max(1ll, std::min({sms / std::max(blocks1, 1ll), (long long)most / (4 * PFT_KT), (long long)MAX_SPLITS}));
+    return c;
 }
-// Rows of partial sums that split calls write: splits * T * H, where splits * blocks1 <= the SMs and T * H <= 128 rows a block... and at
-// most MAX_SPLITS of T * H.
-static size_t split_rows(int T, int H) { return (size_t)std::min<long long>((long long)MAX_SPLITS * T * H, (long long)SPLIT_SMS * PFT_ROWS); }
+// Rows of partial sums that those calls write.  Large requests are cut only while splits * blocks of 128 rows <= the SMs; small ones, of which a
+// request has 32 rows per KV head at most, only while parts * CTAs < 4 * 2 SMs.
+static size_t large_rows(long long T, long long H) { return (size_t)std::min<long long>(MAX_SPLITS * T * H, (long long)SPLIT_SMS * PFT_ROWS); }
+static size_t small_rows(long long T, long long G, long long H) {
+    return (size_t)std::max(std::min(T, (long long)ROWS_MOST * G) * H, std::min<long long>(MAX_SPLITS * T * H, 8ll * SPLIT_SMS * ROWS_MOST));
+}
 
 extern "C" {
 
 size_t tq_paged_workspace_bytes(int T, int G, int num_heads) {
     if (T < 0 || G <= 0 || num_heads <= 0) return 0;
-    return std::max(carve_full(nullptr, G, num_heads).bytes, split_rows(T, num_heads) * PART_STRIDE * sizeof(float));
+    return std::max(carve_full(nullptr, G, num_heads).bytes, (large_rows(T, num_heads) + small_rows(T, G, num_heads)) * PART_STRIDE * sizeof(float));
 }
 
 // What both attentions check of their arguments.
@@ -257,6 +269,13 @@ static int launch_paged_prefill(const CUtensorMap& tmQ, const CUtensorMap& tmR, 
     return cuda_status(cudaLaunchKernelEx(&cfg, kernel, tmQ, tmR, p));
 }
 
+template <int BITS, int NCB>
+static int launch_rows(const PagedRowsParams& p, dim3 grid, cudaStream_t s) {
+    constexpr size_t smem = rows_smem_bytes<BITS, NCB>();
+    const int r = ensure_dynamic_smem((const void*)paged_rows_kernel<BITS, NCB>, smem);
+    return r != TQ_OK ? r : launch_kernel(paged_rows_kernel<BITS, NCB>, grid, dim3(ROWS_THREADS), smem, s, use_pdl(), p);
+}
+
 extern "C" {
 
 int tq_paged_prefill_attention(void* out, const void* q, const uint8_t* ck_q, const uint8_t* cv_q, const void* k_norms, const void* v_norms,
@@ -271,31 +290,57 @@ int tq_paged_prefill_attention(void* out, const void* q, const uint8_t* ck_q, co
     if (!prefill_attn_shape(H, Hkv)) return TQ_ERR_UNSUPPORTED;
     if (!workspace || workspace_bytes < tq_paged_workspace_bytes(T, G, H) || !aligned({workspace}, 256)) return TQ_ERR_WORKSPACE;
     if (T == 0) return TQ_OK;
+    if ((long long)T * H >= (1ll << 31) || G > 65535) return TQ_ERR_UNSUPPORTED;
+    int* status = nullptr;
+    r = paged_status_word(&status);
+    if (r != TQ_OK) return r;
     const PrefillCut cut = prefill_cut(T, G, H, Hkv, most);
-    const int qt = PFT_ROWS / grp, bt = cut.mt * qt;
-    const long long ctas = (long long)Hkv * (T / bt + (long long)G);
-    if (ctas >= (1ll << 31)) return TQ_ERR_UNSUPPORTED;
-    PagedPrefillParams p{};
-    p.ck = ck_q; p.cv = cv_q; p.kn = (const __half*)k_norms; p.vn = (const __half*)v_norms;
-    p.block_table = block_table; p.lens = seq_lens; p.start = query_start; p.out = (__half*)out; p.partials = (float*)workspace;
-    r = paged_status_word(&p.status);
-    if (r != TQ_OK) return r;
-    p.table_stride = table_stride; p.page_shift = log2_of(page_size); p.num_pages = num_pages; p.most_tokens = most;
-    p.T = T; p.G = G; p.H = H; p.Hkv = Hkv; p.grp = grp; p.out_stride = out_stride;
-    CUtensorMap tmQ, tmR;
-    r = make_prefill_query_map(&tmQ, q, T, H, grp, qt, q_stride);
-    if (r == TQ_OK) r = make_prefill_rows_map(&tmR, rotation, HEAD_DIM, HEAD_DIM);
-    if (r != TQ_OK) return r;
-    const dim3 grid((unsigned)ctas, 1, (unsigned)cut.splits);
-    if (cut.mt == 2) return bits == 4 ? launch_paged_prefill<4, 2, false>(tmQ, tmR, p, grid, cs(s)) : launch_paged_prefill<2, 2, false>(tmQ, tmR, p, grid, cs(s));
-    if (cut.splits == 1) return bits == 4 ? launch_paged_prefill<4, 1, false>(tmQ, tmR, p, grid, cs(s)) : launch_paged_prefill<2, 1, false>(tmQ, tmR, p, grid, cs(s));
-    r = bits == 4 ? launch_paged_prefill<4, 1, true>(tmQ, tmR, p, grid, cs(s)) : launch_paged_prefill<2, 1, true>(tmQ, tmR, p, grid, cs(s));
-    if (r != TQ_OK) return r;
+    const int shift = log2_of(page_size), most_small = ROWS_MOST / grp;  // new tokens of a small request
+    float* const small_sums = (float*)workspace + large_rows(T, H) * PART_STRIDE;
     PagedMergeParams m{};
-    m.partials = p.partials; m.rotation = (const __half*)rotation; m.start = query_start; m.out = p.out; m.splits = cut.splits;
-    m.T = T; m.G = G; m.H = H; m.out_stride = out_stride;
-    const long long pieces = ((long long)T * H + 15) / 16;
-    return launch_kernel(paged_merge_kernel, dim3((unsigned)std::min<long long>(pieces, 4ll * device_props().sm_count)), dim3(256), 0, cs(s), use_pdl(), m);
+    m.partials = (const float*)workspace; m.small_partials = small_sums; m.rotation = (const __half*)rotation; m.start = query_start; m.out = (__half*)out;
+    m.T = T; m.H = H; m.grp = grp; m.out_stride = out_stride; m.small_rows = cut.small ? ROWS_MOST : 0;
+    if (cut.large) {
+        const int qt = PFT_ROWS / grp, bt = cut.mt * qt;
+        const long long requests = std::min<long long>(G, cut.small ? T / (most_small + 1) : T), ctas = (long long)Hkv * (T / bt + requests);
+        if (ctas >= (1ll << 31)) return TQ_ERR_UNSUPPORTED;
+        PagedPrefillParams p{};
+        p.ck = ck_q; p.cv = cv_q; p.kn = (const __half*)k_norms; p.vn = (const __half*)v_norms;
+        p.block_table = block_table; p.lens = seq_lens; p.start = query_start; p.out = (__half*)out; p.partials = (float*)workspace; p.status = status;
+        p.table_stride = table_stride; p.page_shift = shift; p.num_pages = num_pages; p.most_tokens = most;
+        p.T = T; p.G = G; p.H = H; p.Hkv = Hkv; p.grp = grp; p.out_stride = out_stride; p.small_rows = m.small_rows;
+        CUtensorMap tmQ, tmR;
+        r = make_prefill_query_map(&tmQ, q, T, H, grp, qt, q_stride);
+        if (r == TQ_OK) r = make_prefill_rows_map(&tmR, rotation, HEAD_DIM, HEAD_DIM);
+        if (r != TQ_OK) return r;
+        const dim3 grid((unsigned)ctas, 1, (unsigned)cut.splits);
+        if (cut.mt == 2) r = bits == 4 ? launch_paged_prefill<4, 2, false>(tmQ, tmR, p, grid, cs(s)) : launch_paged_prefill<2, 2, false>(tmQ, tmR, p, grid, cs(s));
+        else if (cut.splits == 1) r = bits == 4 ? launch_paged_prefill<4, 1, false>(tmQ, tmR, p, grid, cs(s)) : launch_paged_prefill<2, 1, false>(tmQ, tmR, p, grid, cs(s));
+        else r = bits == 4 ? launch_paged_prefill<4, 1, true>(tmQ, tmR, p, grid, cs(s)) : launch_paged_prefill<2, 1, true>(tmQ, tmR, p, grid, cs(s));
+        if (r != TQ_OK) return r;
+        m.splits = cut.splits > 1 ? cut.splits : 0;
+    }
+    if (cut.small) {
+        PagedRowsParams p{};
+        p.ck = ck_q; p.cv = cv_q; p.kn = (const __half*)k_norms; p.vn = (const __half*)v_norms; p.q = (const __half*)q; p.rotation = (const __half*)rotation;
+        p.block_table = block_table; p.lens = seq_lens; p.start = query_start; p.partials = small_sums; p.status = status;
+        p.table_stride = table_stride; p.page_shift = shift; p.num_pages = num_pages; p.most_tokens = most;
+        p.T = T; p.H = H; p.Hkv = Hkv; p.grp = grp; p.q_stride = q_stride; p.row_blocks = ROWS_MOST / (8 * cut.ncb); p.behind = cut.large;
+        p.by_request = (long long)G * most_small < T ? most_small : 0;
+        p.part_tokens = p.by_request ? G * most_small : T;
+        const long long ctas = (long long)Hkv * p.row_blocks * G;
+        if (ctas >= (1ll << 31)) return TQ_ERR_UNSUPPORTED;
+        const dim3 grid((unsigned)ctas, 1, (unsigned)cut.parts);
+        if (cut.ncb == 1) r = bits == 4 ? launch_rows<4, 1>(p, grid, cs(s)) : launch_rows<2, 1>(p, grid, cs(s));
+        else r = bits == 4 ? launch_rows<4, 2>(p, grid, cs(s)) : launch_rows<2, 2>(p, grid, cs(s));
+        if (r != TQ_OK) return r;
+        m.small_splits = cut.parts; m.part_tokens = p.part_tokens; m.by_request = p.by_request;
+    }
+    if (m.splits == 0 && m.small_splits == 0) return TQ_OK;
+    // (rows of a request: 16 a CTA, which loop where a large one was cut)
+    const long long most_rows = cut.large && m.splits ? (long long)T * H : (long long)std::min(T, most_small) * H;
+    const dim3 grid((unsigned)std::min<long long>((most_rows + 15) / 16, std::max(1, 8 * device_props().sm_count / std::min(G, 8))), (unsigned)G);
+    return launch_kernel(paged_merge_kernel, grid, dim3(256), 0, cs(s), use_pdl(), m);
 }
 
 }  // extern "C"

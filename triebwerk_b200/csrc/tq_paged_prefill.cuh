@@ -16,8 +16,9 @@
 //   * Three warps fetch the tiles' rows (one page number for each 32 tokens) and norms ahead, into a ring in shared memory.
 //   * SPLIT (MT = 1): few query rows, long contexts: the tiles of a block are cut into gridDim.z parts, whose sums meet in
 //     paged_merge_kernel.
-// Blocks are found without a table: request g's blocks begin at floor(start[g] / BT) + g (BT query tokens a CTA), which leaves room for
-// them all; a CTA counts the requests that begin at or before its own number, and one whose block does not exist ends at once.
+// Blocks are found without a table: every CTA takes the running sum of the requests' blocks (BT query tokens each) and looks where its number
+// falls; the launch has room for as many as there can be, and those behind the last end at once.  Requests of few rows (small_rows) have none: those
+// are tq_paged_rows.cuh's.
 // Every wait on a barrier is bounded, as there.
 #pragma once
 
@@ -38,6 +39,7 @@ struct PagedPrefillParams {
     int* status;
     int table_stride, page_shift, num_pages, most_tokens;
     int T, G, H, Hkv, grp, out_stride;
+    int small_rows;           // requests of up to so many score rows (new tokens x heads of a KV head) are not served here
 };
 
 constexpr int PPF_THREADS = 32 * PFT_SOFT_WARPS + 128;  // softmax and operands; one warp for the products, three for rows and norms
@@ -119,23 +121,54 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             *reinterpret_cast<uint4*>(gb + PpfSmem::LUT + 16u * (uint32_t)i) = make_uint4(u, u, u, u);
         }
     }
-    pdl_launch_dependents();
     pdl_wait();  // (lengths, tables, caches, queries: all of earlier launches)
+    pdl_launch_dependents();  // (behind the wait: what starts now knows that those have finished)
     // ---- the request and the block of this CTA ----
-    const int ny = (int)(gridDim.x / (unsigned)p.Hkv);
-    const int kvh = (int)blockIdx.x % p.Hkv, y = ny - 1 - (int)blockIdx.x / p.Hkv;  // the longest causal prefixes of a request first
-    int g = -1;
+    const int kvh = (int)blockIdx.x % p.Hkv, y = (int)blockIdx.x / p.Hkv;
+    // (scratch where K comes later: block counts of the warps, then request, first query, queries, block)
+    int* const scratch = reinterpret_cast<int*>(gb + PpfSmem::K);
+    constexpr int WARPS = PPF_THREADS / 32;
+    if (tid == 0) scratch[WARPS] = -1;
     tc_fence_before();
-    for (int base = 0; base < p.G; base += PPF_THREADS) {  // (at least once: what was made above is in place)
-        const int i = base + tid;
-        g += __syncthreads_count(i < p.G && p.start[i] / BT + i <= y);
+    int before = 0;
+    for (int first = 0; first < p.G; first += PPF_THREADS) {
+        const int i = first + tid;
+        int a = 0, m = 0;
+        if (i < p.G) {
+            a = max(p.start[i], 0);
+            m = max(min(p.start[i + 1], p.T) - a, 0);
+        }
+        const int blocks = m * GRP > p.small_rows ? (m + BT - 1) / BT : 0;
+        int incl = blocks;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += v;
+        }
+        if (lane == 31) scratch[warp] = incl;
+        __syncthreads();
+        int mine = before, all = 0;
+        for (int w = 0; w < WARPS; ++w) {
+            const int v = scratch[w];
+            mine += w < warp ? v : 0;
+            all += v;
+        }
+        const int at = y - (mine + incl - blocks);
+        if (at >= 0 && at < blocks) {  // (the last blocks of a request, whose causal prefixes are the longest, first)
+            scratch[WARPS] = i;
+            scratch[WARPS + 1] = a;
+            scratch[WARPS + 2] = m;
+            scratch[WARPS + 3] = (blocks - 1 - at) * BT;
+        }
+        before += all;
+        __syncthreads();  // (what was made above is in place too)
+        if (before > y) break;
     }
     tc_fence_after();
-    g = max(g, 0);  // (request 0 begins at block 0)
     const uint32_t tmem = *tmem_slot;
-    const int s0 = max(p.start[g], 0), n = min(p.start[g + 1], p.T) - s0, q0 = (y - (s0 / BT + g)) * BT;
-    if (q0 >= n) {  // no such block
-        __syncthreads();
+    const int g = scratch[WARPS], s0 = scratch[WARPS + 1], n = scratch[WARPS + 2], q0 = scratch[WARPS + 3];
+    __syncthreads();
+    if (g < 0) {  // no such block
         if (warp == 0) tmem_dealloc(tmem, 512u);
         return;
     }
@@ -673,14 +706,18 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     if (warp == 0) tmem_dealloc(tmem, 512u);
 }
 
-// The parts of a split call: out[tok][h] = R (sum_z 2^(m_z - M) acc_z / sum_z 2^(m_z - M) l_z).  16 (token, head) rows per CTA, two a warp;
-// fp16 high and low parts of the sums times R on mma.sync, a warp 16 output coordinates.
+// The parts of a request whose tokens were cut: out[tok][h] = R (sum_z 2^(m_z - M) acc_z / sum_z 2^(m_z - M) l_z).  16 (token, head) rows per CTA, two a
+// warp; fp16 high and low parts of the sums times R on mma.sync, a warp 16 output coordinates.
 struct PagedMergeParams {
-    const float* partials;   // [splits][T][H][PART_STRIDE]
-    const __half* rotation;  // R row-major
+    const float* partials;        // [splits][T][H][PART_STRIDE]
+    const float* small_partials;  // PagedRowsParams::partials
+    int part_tokens, by_request;
+    const __half* rotation;       // R row-major
     const int* start;        // [G + 1]
     __half* out;
-    int splits, T, G, H, out_stride;
+    int splits, small_splits;  // parts of the requests of more than small_rows rows (0: none of them is cut), of the others
+    int small_rows;
+    int T, H, grp, out_stride;
 };
 static __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedMergeParams p) {
     __shared__ __align__(16) __half r_s[HEAD_DIM / 2][HEAD_DIM + 8];
@@ -688,6 +725,11 @@ static __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedMerg
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gl = lane >> 2, t4 = lane & 3;
     pdl_launch_dependents();
     pdl_wait();
+    const int s0 = max(p.start[blockIdx.y], 0), n = max(min(p.start[blockIdx.y + 1], p.T) - s0, 0);
+    const bool large = n * p.grp > p.small_rows;
+    const int splits = large ? p.splits : p.small_splits;
+    const long long rows = (long long)n * p.H;
+    if (splits == 0 || 16ll * blockIdx.x >= rows) return;
     uint32_t bf[2][8][2];
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
@@ -706,27 +748,27 @@ static __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedMerg
             bf[1][4 * half + j][0] = r[2]; bf[1][4 * half + j][1] = r[3];
         }
     }
-    const long long rows = (long long)min(p.start[p.G], p.T) * p.H;  // (tokens behind the last request have no sums)
-    const size_t part = (size_t)p.T * p.H * PART_STRIDE;
+    const size_t part = (size_t)(large ? p.T : p.part_tokens) * p.H * PART_STRIDE;
+    const float* const sums = (large ? p.partials : p.small_partials) + (size_t)(!large && p.by_request ? (int)blockIdx.y * p.by_request : s0) * p.H * PART_STRIDE;
     for (long long row0 = 16ll * blockIdx.x; row0 < rows; row0 += 16ll * gridDim.x) {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             const int rr = 2 * warp + k;
-            const float* const src = p.partials + (size_t)(row0 + rr) * PART_STRIDE;
+            const float* const src = sums + (size_t)(row0 + rr) * PART_STRIDE;
             float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
             if (row0 + rr < rows) {
                 float2 ml = make_float2(-1e30f, 0.0f);
-                if (lane < p.splits) ml = __ldcg(reinterpret_cast<const float2*>(src + lane * part + HEAD_DIM));
+                if (lane < splits) ml = __ldcg(reinterpret_cast<const float2*>(src + lane * part + HEAD_DIM));
                 float M = ml.x;
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-                const float e = lane < p.splits ? ex2_approx(ml.x - M) : 0.0f;
+                const float e = lane < splits ? ex2_approx(ml.x - M) : 0.0f;
                 float Z = ml.y * e;
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) Z += __shfl_xor_sync(0xffffffffu, Z, o);
                 const float sc = e / (Z + 1e-8f);
 #pragma unroll 4
-                for (int z = 0; z < p.splits; ++z) {
+                for (int z = 0; z < splits; ++z) {
                     const float4 v = __ldcg(reinterpret_cast<const float4*>(src + z * part) + lane);
                     const float w = __shfl_sync(0xffffffffu, sc, z);
                     a.x = fmaf(w, v.x, a.x); a.y = fmaf(w, v.y, a.y); a.z = fmaf(w, v.z, a.z); a.w = fmaf(w, v.w, a.w);
@@ -750,7 +792,7 @@ static __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedMerg
         for (int r = 0; r < 2; ++r) {
             const long long row = row0 + gl + 8 * r, tok = row / p.H;
             if (row >= rows) continue;
-            __half* const dst = p.out + tok * p.out_stride + (row - tok * p.H) * HEAD_DIM + 16 * warp + 2 * t4;
+            __half* const dst = p.out + (s0 + tok) * p.out_stride + (row - tok * p.H) * HEAD_DIM + 16 * warp + 2 * t4;
 #pragma unroll
             for (int i = 0; i < 2; ++i) *reinterpret_cast<__half2*>(dst + 8 * i) = __floats2half2_rn(c[i][2 * r], c[i][2 * r + 1]);
         }
