@@ -48,8 +48,8 @@ constexpr int PPF_MEET = 32 * PFT_SOFT_WARPS + 32;      // all but those
 // behind 8192 took 618 us, with 32 and 112 1072.)
 constexpr int PPF_STAGES = 4;                          // of a tile's norms and rows: fetched ahead, and the slots may be far apart
 struct PpfSmem {
-    static constexpr uint32_t Q = 0;                       // 2 tiles; at the end: high parts of the results
-    static constexpr uint32_t K = 2 * PFT_TILE;            // 2 stages; at the start R in the second; at the end: low parts
+    static constexpr uint32_t Q = 0;                       // 2 tiles; at the end: the results
+    static constexpr uint32_t K = 2 * PFT_TILE;            // 2 stages; at the start R in the second
     static constexpr uint32_t V = K + 2 * PFT_TILE;        // 2 stages; at the end R in the free one
     static constexpr uint32_t LUT = V + 2 * PFT_TILE;      // byte (4-bit) or nibble -> two centroids, a column per lane; at the end (MT = 1) the slots' maxima and sums
     static constexpr uint32_t LUT_BYTES = 32768u;
@@ -85,7 +85,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     const uint32_t ctrl = sb + PpfSmem::CTRL;
     const uint32_t bar_kfull = ctrl, bar_vfull = ctrl + 16u, bar_kfree = ctrl + 32u, bar_vfree = ctrl + 48u;  // [2] each
     const uint32_t bar_sfull = ctrl + 64u, bar_pfull = ctrl + 80u;                                            // [2 slots] each
-    const uint32_t bar_rot = ctrl + 96u, bar_done = ctrl + 104u, bar_q = ctrl + 112u, bar_r = ctrl + 120u;
+    const uint32_t bar_rot = ctrl + 96u, bar_done = ctrl + 104u, bar_q = ctrl + 112u, bar_r = ctrl + 120u, bar_done1 = ctrl + 248u;
     const uint32_t bar_rows = ctrl + 128u, bar_norms = ctrl + 160u, bar_used = ctrl + 192u;                   // [PPF_STAGES] each
     volatile uint32_t* const tmem_slot = reinterpret_cast<volatile uint32_t*>(gb + PpfSmem::CTRL + 224);
     if (warp == 0) {
@@ -108,27 +108,32 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         }
         mbar_init(bar_rot, 1);
         mbar_init(bar_done, 1);
+        mbar_init(bar_done1, 1);
         mbar_init(bar_q, 1);
         mbar_init(bar_r, 1);
         fence_mbar_init();
     }
     {
-        constexpr int ENTRIES = BITS == 4 ? 256 : 16;
-        for (int i = tid; i < ENTRIES * 8; i += PPF_THREADS) {  // four lanes' columns at a time
-            const int e = i >> 3;
-            constexpr float c = PPF_CENT<BITS>;
-            const uint32_t u = BITS == 4 ? pack_half2(c * kCent4[e & 15], c * kCent4[(e >> 4) & 15]) : pack_half2(c * kCent2[e & 3], c * kCent2[(e >> 2) & 3]);
-            *reinterpret_cast<uint4*>(gb + PpfSmem::LUT + 16u * (uint32_t)i) = make_uint4(u, u, u, u);
+        // (entry (tid >> 3) + 64 i, four lanes' columns: a thread's entries share their first code)
+        constexpr float c = PPF_CENT<BITS>;
+        const int e = tid >> 3;
+        const float first = c * (BITS == 4 ? kCent4[e & 15] : kCent2[e & 3]);
+#pragma unroll
+        for (int i = 0; i < (BITS == 4 ? 4 : 1); ++i) {
+            const uint32_t u = pack_half2(first, c * (BITS == 4 ? kCent4[((tid >> 7) & 3) + 4 * i] : kCent2[(e >> 2) & 3]));
+            if (BITS == 4 ? tid < 512 : tid < 128) *reinterpret_cast<uint4*>(gb + PpfSmem::LUT + 16u * (uint32_t)(tid + 512 * i)) = make_uint4(u, u, u, u);
         }
     }
     pdl_wait();  // (lengths, tables, caches, queries: all of earlier launches)
     pdl_launch_dependents();  // (behind the wait: what starts now knows that those have finished)
     // ---- the request and the block of this CTA ----
     const int kvh = (int)blockIdx.x % p.Hkv, y = (int)blockIdx.x / p.Hkv;
-    // (scratch where K comes later: block counts of the warps, then request, first query, queries, block)
+    // First query, queries of the request, the block's first one, request.  (They wait in shared memory for the end, which is what else needs them: in
+    // registers they cost spills, and those come back from L2, see below.)  The warps' block counts lie where K comes later.
+    volatile int* const kept = reinterpret_cast<volatile int*>(gb + PpfSmem::CTRL + 228);
     int* const scratch = reinterpret_cast<int*>(gb + PpfSmem::K);
     constexpr int WARPS = PPF_THREADS / 32;
-    if (tid == 0) scratch[WARPS] = -1;
+    if (tid == 0) kept[3] = -1;
     tc_fence_before();
     int before = 0;
     for (int first = 0; first < p.G; first += PPF_THREADS) {
@@ -155,10 +160,10 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         }
         const int at = y - (mine + incl - blocks);
         if (at >= 0 && at < blocks) {  // (the last blocks of a request, whose causal prefixes are the longest, first)
-            scratch[WARPS] = i;
-            scratch[WARPS + 1] = a;
-            scratch[WARPS + 2] = m;
-            scratch[WARPS + 3] = (blocks - 1 - at) * BT;
+            kept[0] = a;
+            kept[1] = m;
+            kept[2] = (blocks - 1 - at) * BT;
+            kept[3] = i;
         }
         before += all;
         __syncthreads();  // (what was made above is in place too)
@@ -166,17 +171,12 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     }
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const int g = scratch[WARPS], s0 = scratch[WARPS + 1], n = scratch[WARPS + 2], q0 = scratch[WARPS + 3];
-    __syncthreads();
+    const int s0 = kept[0], n = kept[1], q0 = kept[2], g = kept[3];
     if (g < 0) {  // no such block
         if (warp == 0) tmem_dealloc(tmem, 512u);
         return;
     }
-    volatile int* const kept = reinterpret_cast<volatile int*>(gb + PpfSmem::CTRL + 232);
     if (tid == 32 * MMA_WARP) {
-        kept[0] = s0;
-        kept[1] = n;
-        kept[2] = q0;
         mbar_arrive_expect_tx(bar_q, (uint32_t)(MT * QT * GRP) * 256u + PFT_TILE);
         for (int m = 0; m < MT; ++m) {  // (rows of other requests or past the end: a row's garbage stays in that row and is never stored)
             tma_load_4d(sb + PpfSmem::Q + m * PFT_TILE, &tmQ, bar_q, 0, kvh * GRP, s0 + q0 + m * QT, 0);
@@ -275,39 +275,51 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                 mbar_arrive_expect_tx(bar_r, PFT_TILE);
                 tma_load_3d(sb + PpfSmem::V + (uint32_t)(n_tiles & 1) * PFT_TILE, &tmR, bar_r, 0, 0, 0);
             };
+            // MT = 2: the slots end apart, each with a barrier of its own; MT = 1: together
+            if (MT == 2 && n0 == 0) umma_commit(bar_done);
+            if (MT == 2 && n1 == 0) umma_commit(bar_done1);
             for (int i = 0; i < max(n0, n1); ++i) {
                 if (i < n0) {
                     issue_values(0, i);
                     if (i + 1 < n0) issue_scores(0, i + 1);
+                    else if (MT == 2) umma_commit(bar_done);
                 }
+                if (MT == 2 && i + 1 == n_tiles) fetch_rotation();  // (the products of the tile in front are all on their way)
                 if (i < n1) {
                     issue_values(1, i);
                     if (i + 1 < n1) issue_scores(1, i + 1);
+                    else if (MT == 2) umma_commit(bar_done1);
                 }
             }
-            umma_commit(bar_done);
-            fetch_rotation();
+            if (MT == 1) umma_commit(bar_done);
+            if (MT == 1 || n_tiles == 0) fetch_rotation();
         }
         __syncwarp();
         if (!SPLIT) {
-            // out[d] = sum_k R[k][d] * acc[k]: the results' high and low parts times R
-            named_barrier(1, PPF_MEET);
-            if (lane == 0) {
-                wait_bar(bar_r, 0u);
-                tc_fence_after();
-                if (!dead) {
+            // out[d] = sum_k R[k][d] * acc[k]
+            auto rotate_back = [&](int m, uint32_t bar) {
+                if (lane == 0) {
+                    wait_bar(bar_r, 0u);
+                    tc_fence_after();
+                    if (!dead) {
 #pragma unroll
-                    for (int m = 0; m < MT; ++m)
-#pragma unroll
-                        for (int part = 0; part < 2; ++part)
-#pragma unroll
-                            for (int ks = 0; ks < 8; ++ks)
-                                umma_lo(tmem + 128u * m, pft_lo_k(sb + (part ? PpfSmem::K : PpfSmem::Q) + m * PFT_TILE) + pft_kstep(ks),
-                                        pft_lo_mn(sb + PpfSmem::V + (uint32_t)(n_tiles & 1) * PFT_TILE) + 128u * ks, PFT_IDESC_MN, (part | ks) != 0);
+                        for (int ks = 0; ks < 8; ++ks)
+                            umma_lo(tmem + 128u * m, pft_lo_k(sb + PpfSmem::Q + m * PFT_TILE) + pft_kstep(ks), pft_lo_mn(sb + PpfSmem::V + (uint32_t)(n_tiles & 1) * PFT_TILE) + 128u * ks,
+                                    PFT_IDESC_MN, ks != 0);
+                    }
+                    umma_commit(bar);
                 }
-                umma_commit(bar_rot);
+                __syncwarp();
+            };
+            if (MT == 1) {
+                named_barrier(1, PPF_MEET);
+                rotate_back(0, bar_rot);
+            } else {
+                named_barrier(3, PPF_MEET / 2 + 16);
+                rotate_back(0, bar_rot);
+                named_barrier(4, PPF_MEET / 2 + 16);
+                rotate_back(1, bar_q);
             }
-            __syncwarp();
         }
       } else {
         // ================= rows and norms of the tiles, three warps in turn =================
@@ -455,10 +467,10 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         // ---- softmax of slot `slot`, rows row0 + gl and row0 + gl + 8 ----
         const uint32_t s_col = my_lanes + 128u * slot, o_col = s_col + 256u;
         const int nt = slot ? n1 : n0;
-        const uint32_t by_grp0 = make_by_grp();
-        const int tok0 = token_of(row0 + gl, by_grp0), tok1 = token_of(row0 + gl + 8, by_grp0);
-        const bool some_row = token_in(row0, by_grp0) < QT && my_first + token_in(row0, by_grp0) < n;  // (uniform for the warp)
-        // last token of a row of no query: none
+        const bool some_row = token_of(row0, make_by_grp()) < n;  // (uniform for the warp)
+        const int first_pos = pos0 + my_first;                    // position of the slot's first query
+        // last tokens that the thread's rows attend to (none: a row of no query)
+        const int tok0 = token_of(row0 + gl, make_by_grp()), tok1 = token_of(row0 + gl + 8, make_by_grp());
         const int last0 = tok0 < n ? pos0 + tok0 : -1, last1 = tok1 < n ? pos0 + tok1 : -1;
         float m_run[2] = {-1e30f, -1e30f}, l_run[2] = {0.0f, 0.0f};  // (sums: of this thread's columns)
         for (int j = 0; j < n_tiles; ++j) {
@@ -468,7 +480,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                 wait_bar(bar_sfull + 8u * slot, (uint32_t)(i & 1));
                 tc_fence_after();
                 if (some_row) {
-                    const bool diagonal = col0 + PFT_KT - 1 > pos0 + my_first;  // (uniform for the slot)
+                    const bool diagonal = col0 + PFT_KT - 1 > first_pos;  // (uniform for the slot)
                     const uint8_t* const info = info_of(j);
                     const bool select = *reinterpret_cast<const uint32_t*>(info + PpfSmem::INFO_ODD) != 0u;  // a norm of V that is not finite
                     // Scores of 64 columns at a time, masked: [row][column block].  The second half is read once for the
@@ -587,9 +599,8 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 1);
             l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 2);
         }
-        wait_bar(bar_done, 0u);  // every product has completed (and nobody reads the norms any more)
+        wait_bar(MT == 2 && slot ? bar_done1 : bar_done, 0u);  // every product (of the slot) has completed
         tc_fence_after();
-        // (what only the end needs waits in shared memory: kept in registers it was spilled, see above)
         const int s0_e = kept[0], n_e = kept[1], first_e = kept[2] + (MT == 2 ? slot * QT : 0);
         const uint32_t lanes_e = *tmem_slot + ((uint32_t)row0 << 16);
         auto token_e = [&](int row, uint32_t by_grp) { return token_in(row, by_grp) < QT ? first_e + token_in(row, by_grp) : n_e; };
@@ -620,7 +631,11 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             for (int h = 0; h < 2; ++h) w0[h] = (1.0f / PPF_CENT<BITS>) / (l_run[h] + 1e-8f);
         }
         // rows that attend to nothing (no tile at all, or none up to their position) give zeros whatever tensor memory holds
-        const bool on[2] = {last0 >= 0 && (MT == 1 || nt > 0), last1 >= 0 && (MT == 1 || nt > 0)};
+        auto sees = [&](int r) {
+            const int tok = token_e(row0 + r, make_by_grp());
+            return tok < n_e && first_pos + tok - first_e >= 0 && (MT == 1 || nt > 0);
+        };
+        const bool on[2] = {sees(gl), sees(gl + 8)};
         auto result = [&](int c0, float (&v)[32]) {  // columns c0 .. c0 + 63 in fragment order
             uint32_t r[32];
 #pragma unroll
@@ -654,21 +669,19 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                 if (slot == 0 && t4 == 0) *reinterpret_cast<float2*>(dst + HEAD_DIM) = on[h] ? make_float2(M_all[h], Z_all[h]) : make_float2(-1e30f, 0.0f);
             }
         } else {
-            const uint32_t qtile = PpfSmem::Q + pslot * PFT_TILE, ktile = PpfSmem::K + pslot * PFT_TILE;
-            // the normalised rows, split into fp16 high and low parts, over the Q and K tiles
+            // The normalised rows as fp16 over the Q tile, times R.  (One rounding more, relative to a row 2^-11 at most, as R changes no length; with
+            // a low part beside it the way from the last tile to the end, a third of a short prompt's time, was twice as many products and stores.)
+            const uint32_t qtile = PpfSmem::Q + pslot * PFT_TILE;
 #pragma unroll 1
             for (int c0 = pcol0; c0 < pcol0 + PCOLS; c0 += 64) {
                 float v[32];
                 result(c0, v);
                 put_frag(qtile, c0, v);
-#pragma unroll
-                for (int e = 0; e < 32; ++e) v[e] = low_part(v[e]);
-                put_frag(ktile, c0, v);
             }
             fence_proxy_async_smem();
             tc_fence_before();
-            named_barrier(1, PPF_MEET);
-            wait_bar(bar_rot, 1u);
+            named_barrier(MT == 1 ? 1 : 3 + slot, MT == 1 ? PPF_MEET : PPF_MEET / 2 + 16);
+            wait_bar(MT == 2 && slot ? bar_q : bar_rot, 1u);
             tc_fence_after();
             // the finished values as fp16 through the (consumed) query tile, so that 16 lanes store 256 contiguous bytes of a row
 #pragma unroll 1
