@@ -10,6 +10,11 @@
 
 namespace tq {
 
+// The centroids times these have fp16 neighbours 3.4 times (2-bit: over 1000 times) as close as the centroids themselves (2^-11 x 0.22 and 0.0004
+// against 0.73 and 0.54, relative): the tables hold them scaled, queries and results carry the inverse.
+template <int BITS>
+constexpr float PPF_CENT = BITS == 4 ? 1.211955f : 1.591824f;
+
 // ---- block tables and slot maps -----------------------------------------------------------------------------------------------------
 // With c the tokens that request g holds (0 where it has ended), n its new ones, P the page size:
 //   pages back      ceil(old / P) of every ended request, in order, on top of the stack of free pages;
@@ -198,8 +203,12 @@ static __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(const Pa
 }
 
 // ---- rows of a slot map as vectors ------------------------------------------------------------------------------------------------------
-// out[t][h] = norm * R^T c, c the centroids of row slots[t], head h (zeros where the slot is no row).  Vectors are the M dimension, 64 at a
-// time, of mma.sync: a warp owns 16 output coordinates, whose part of R stays in its registers; the centroids go through shared memory.
+// out[t][h] = norm * R^T c, c the centroids of row slots[t], head h (zeros where the slot is no row).  Vectors are the M dimension of mma.sync,
+// 64 at a time; a warp owns 32 of them and 32 output coordinates, whose part of R stays in its registers; the centroids, and then the results,
+// go through shared memory, so that whole rows leave.  Two dependent trips to memory (slot, codes) stand before a vector's arithmetic: both
+// are made a tile ahead.  8192 tokens, 8 KV heads, 4-bit (42 MB, 6.5 us at the copy rate): 19.8 us; 34.4 with neither, results stored as the
+// products leave them and every warp on all 64 vectors for 16 coordinates (the operand is then read eight times, not four: 22 us by itself).
+// What bounds it now is the table look-ups and operand traffic of shared memory.  64 tokens: the launch and the two trips.
 struct PagedReadParams {
     const uint8_t* ck;
     const __half* kn;
@@ -217,18 +226,50 @@ constexpr int READ_THREADS = 256, READ_VECTORS = 64;
 template <int BITS>
 __global__ void __launch_bounds__(READ_THREADS, 2) paged_read_kernel(const PagedReadParams p) {
     constexpr int BPH = HEAD_DIM * BITS / 8, ENTRIES = BITS == 4 ? 256 : 16;
-    __shared__ uint32_t lut[ENTRIES * 8];
+    constexpr int COPIES = 16;  // of the table: two lanes share a bank
+    __shared__ uint32_t lut[ENTRIES * COPIES];
     __shared__ __align__(16) __half a_s[READ_VECTORS][HEAD_DIM + 8];
     __shared__ float norm_s[READ_VECTORS];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gl = lane >> 2, t4 = lane & 3;
-    for (int i = tid; i < ENTRIES * 8; i += READ_THREADS) {
-        const int e = i >> 3;
-        lut[i] = BITS == 4 ? pack_half2(kCent4[e & 15], kCent4[(e >> 4) & 15]) : pack_half2(kCent2[e & 3], kCent2[(e >> 2) & 3]);
+    const int v_part = 32 * (warp >> 2), c_part = 32 * (warp & 3);  // first vector, first output coordinate of the warp
+    for (int i = tid; i < ENTRIES * COPIES; i += READ_THREADS) {
+        constexpr float c = PPF_CENT<BITS>;  // (the table's centroids times this are closer to fp16 numbers)
+        const int e = i / COPIES;
+        lut[i] = BITS == 4 ? pack_half2(c * kCent4[e & 15], c * kCent4[(e >> 4) & 15]) : pack_half2(c * kCent2[e & 3], c * kCent2[(e >> 2) & 3]);
     }
     pdl_launch_dependents();
     pdl_wait();
-    // B fragments: coordinates n = 16 warp + 8 i + gl, k = 16 j + 2 t4, + 1 (+ 8); R passes through the operand's place, 64 rows at a time
-    uint32_t bf[2][8][2];
+    // four threads a vector, 32 coordinates each.  A tile's vectors: their slots (requested two tiles ahead), then codes and norm (one).
+    const uint32_t per_kind = (uint32_t)p.T * p.Hkv, tiles = (per_kind + READ_VECTORS - 1) / READ_VECTORS;
+    const uint2 by_heads = fastdiv_make((uint32_t)p.Hkv);
+    auto token_of = [&](uint32_t v) { return (uint32_t)fastdiv((int)v, by_heads); };
+    auto slot_of = [&](uint32_t tile) -> long long {
+        if (tile >= 2 * tiles) return -1;
+        const uint32_t v = (tile >= tiles ? tile - tiles : tile) * READ_VECTORS + (uint32_t)(tid >> 2);
+        return v < per_kind ? __ldg(p.slots + token_of(v)) : -1;
+    };
+    uint4 codes;
+    unsigned short norm;
+    auto fetch = [&](uint32_t tile, long long row) {
+        codes = make_uint4(0u, 0u, 0u, 0u);
+        norm = 0;
+        if (row < 0 || row >= p.total_rows) return;
+        const bool is_v = tile >= tiles;
+        const uint32_t v = (is_v ? tile - tiles : tile) * READ_VECTORS + (uint32_t)(tid >> 2);
+        const size_t at = (size_t)row * p.Hkv + (v - token_of(v) * (uint32_t)p.Hkv);
+        const uint8_t* const src = (is_v ? p.cv : p.ck) + at * BPH + (BPH / 4) * (tid & 3);
+        if (BITS == 4) {
+            codes = __ldg(reinterpret_cast<const uint4*>(src));
+        } else {
+            const uint2 u = __ldg(reinterpret_cast<const uint2*>(src));
+            codes = make_uint4(u.x & 0xffffu, u.x >> 16, u.y & 0xffffu, u.y >> 16);
+        }
+        if ((tid & 3) == 0) norm = __ldg(reinterpret_cast<const unsigned short*>(is_v ? p.vn : p.kn) + at);
+    };
+    const uint32_t step = gridDim.x;
+    long long next_row = slot_of(blockIdx.x);
+    // B fragments: coordinates n = c_part + 8 i + gl, k = 16 j + 2 t4, + 1 (+ 8); R passes through the operand's place, 64 rows at a time
+    uint32_t bf[4][8][2];
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
         __syncthreads();
@@ -237,67 +278,73 @@ __global__ void __launch_bounds__(READ_THREADS, 2) paged_read_kernel(const Paged
             const int at = tid + READ_THREADS * i;
             *reinterpret_cast<uint4*>(&a_s[at >> 4][8 * (at & 15)]) = reinterpret_cast<const uint4*>(p.rotation)[1024 * half + at];
         }
+        if (half == 0) {
+            fetch(blockIdx.x, next_row);
+            next_row = slot_of(blockIdx.x + step);
+        }
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            uint32_t r[4];
-            ldmatrix_x4_trans(r, smem_u32(&a_s[16 * j + (lane & 15)][16 * warp + 8 * (lane >> 4)]));
-            bf[0][4 * half + j][0] = r[0]; bf[0][4 * half + j][1] = r[1];
-            bf[1][4 * half + j][0] = r[2]; bf[1][4 * half + j][1] = r[3];
-        }
-    }
-    const long long per_kind = (long long)p.T * p.Hkv, tiles = (per_kind + READ_VECTORS - 1) / READ_VECTORS;
-    for (long long tile = blockIdx.x; tile < 2 * tiles; tile += gridDim.x) {
-        const bool is_v = tile >= tiles;
-        const long long v0 = (is_v ? tile - tiles : tile) * READ_VECTORS;
-        __syncthreads();  // (table; the last tile's operand has been read)
-        {
-            const long long v = v0 + (tid >> 2), t = v / p.Hkv;  // four threads a vector, 32 coordinates each
-            const int h = (int)(v - t * p.Hkv), copy = tid & 7;
-            const long long row = v < per_kind ? p.slots[t] : -1;
-            const bool on = row >= 0 && row < p.total_rows;
-            uint32_t w[4] = {0u, 0u, 0u, 0u};
-            if (on) {
-                const uint8_t* const src = (is_v ? p.cv : p.ck) + ((size_t)row * p.Hkv + h) * BPH + (BPH / 4) * (tid & 3);
-                if (BITS == 4) {
-                    const uint4 u = *reinterpret_cast<const uint4*>(src);
-                    w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
-                } else {
-                    const uint2 u = *reinterpret_cast<const uint2*>(src);
-                    w[0] = u.x & 0xffffu; w[1] = u.x >> 16; w[2] = u.y & 0xffffu; w[3] = u.y >> 16;
-                }
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+                uint32_t r[4];
+                ldmatrix_x4_trans(r, smem_u32(&a_s[16 * j + (lane & 15)][c_part + 8 * i + 8 * (lane >> 4)]));
+                bf[i][4 * half + j][0] = r[0]; bf[i][4 * half + j][1] = r[1];
+                bf[i + 1][4 * half + j][0] = r[2]; bf[i + 1][4 * half + j][1] = r[3];
             }
-            if ((tid & 3) == 0) norm_s[tid >> 2] = on ? __half2float((is_v ? p.vn : p.kn)[(size_t)row * p.Hkv + h]) : 0.0f;
+    }
+    for (uint32_t tile = blockIdx.x; tile < 2 * tiles; tile += step) {
+        const bool is_v = tile >= tiles;
+        const uint32_t v0 = (is_v ? tile - tiles : tile) * READ_VECTORS;
+        __syncthreads();  // (the last tile's results have left)
+        {
+            const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
+            const int copy = tid & (COPIES - 1);
+            if ((tid & 3) == 0) norm_s[tid >> 2] = (1.0f / PPF_CENT<BITS>) * __half2float(__ushort_as_half(norm));
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 uint4 u;
                 constexpr uint32_t M = ENTRIES - 1, W = BITS == 4 ? 8 : 4;
-                u.x = lut[(w[i] & M) * 8 + copy]; u.y = lut[((w[i] >> W) & M) * 8 + copy];
-                u.z = lut[((w[i] >> (2 * W)) & M) * 8 + copy]; u.w = lut[((w[i] >> (3 * W)) & M) * 8 + copy];
+                u.x = lut[(w[i] & M) * COPIES + copy]; u.y = lut[((w[i] >> W) & M) * COPIES + copy];
+                u.z = lut[((w[i] >> (2 * W)) & M) * COPIES + copy]; u.w = lut[((w[i] >> (3 * W)) & M) * COPIES + copy];
                 *reinterpret_cast<uint4*>(&a_s[tid >> 2][32 * (tid & 3) + 8 * i]) = u;
             }
         }
+        fetch(tile + step, next_row);
+        next_row = slot_of(tile + 2 * step);
         __syncthreads();
+        float c[2][4][4];
 #pragma unroll
-        for (int m = 0; m < READ_VECTORS / 16; ++m) {
-            float c[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+        for (int m = 0; m < 2; ++m) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) c[m][i][0] = c[m][i][1] = c[m][i][2] = c[m][i][3] = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 uint32_t a[4];
-                ldmatrix_x4(a, smem_u32(&a_s[16 * m + (lane & 15)][16 * j + 8 * (lane >> 4)]));
+                ldmatrix_x4(a, smem_u32(&a_s[v_part + 16 * m + (lane & 15)][16 * j + 8 * (lane >> 4)]));
 #pragma unroll
-                for (int i = 0; i < 2; ++i) mma16816(c[i], a[0], a[1], a[2], a[3], bf[i][j][0], bf[i][j][1]);
+                for (int i = 0; i < 4; ++i) mma16816(c[m][i], a[0], a[1], a[2], a[3], bf[i][j][0], bf[i][j][1]);
             }
+        }
+        __syncthreads();  // the operand has been read: the results take its place
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                const int at = 16 * m + gl + 8 * r;
-                const long long v = v0 + at, t = v / p.Hkv;
-                if (v >= per_kind) continue;
+                const int at = v_part + 16 * m + gl + 8 * r;
                 const float n = norm_s[at];
-                __half* const dst = (is_v ? p.v_out : p.k_out) + t * p.stride + (v - t * p.Hkv) * HEAD_DIM + 16 * warp + 2 * t4;
 #pragma unroll
-                for (int i = 0; i < 2; ++i) *reinterpret_cast<__half2*>(dst + 8 * i) = __floats2half2_rn(c[i][2 * r] * n, c[i][2 * r + 1] * n);
+                for (int i = 0; i < 4; ++i)
+                    *reinterpret_cast<__half2*>(&a_s[at][c_part + 8 * i + 2 * t4]) = __floats2half2_rn(c[m][i][2 * r] * n, c[m][i][2 * r + 1] * n);
             }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < READ_VECTORS * 16 / READ_THREADS; ++i) {  // 16 lanes a row
+            const int at = (tid >> 4) + (READ_THREADS / 16) * i;
+            const uint32_t v = v0 + (uint32_t)at, t = token_of(v);
+            if (v < per_kind)
+                *(reinterpret_cast<uint4*>((is_v ? p.v_out : p.k_out) + (size_t)t * p.stride + (size_t)(v - t * (uint32_t)p.Hkv) * HEAD_DIM) + (tid & 15)) =
+                    *reinterpret_cast<const uint4*>(&a_s[at][8 * (tid & 15)]);
         }
     }
 }

@@ -22,7 +22,7 @@
 // Every wait on a barrier is bounded, as there.
 #pragma once
 
-#include "tq_prefill_fa.cuh"
+#include "tq_paged.cuh"
 
 namespace tq {
 
@@ -60,10 +60,6 @@ struct PpfSmem {
 };
 static_assert(PpfSmem::BYTES <= 227 * 1024, "one CTA's shared memory");
 constexpr uint32_t PPF_XCH = PpfSmem::LUT;  // (the table is no longer needed then)
-// The centroids times these have fp16 neighbours 3.4 times (2-bit: over 1000 times) as close as the centroids themselves (2^-11 x 0.22 and 0.0004
-// against 0.73 and 0.54, relative): the table holds them scaled, the queries and the results carry the inverse.
-template <int BITS>
-constexpr float PPF_CENT = BITS == 4 ? 1.211955f : 1.591824f;
 
 template <int BITS, int MT, bool SPLIT>
 __global__ void __launch_bounds__(PPF_THREADS, 1)
