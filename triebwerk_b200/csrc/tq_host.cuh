@@ -503,7 +503,10 @@ inline int cluster_split(int bits, long long clusters, int heads, int max_tokens
 // Launchers: their streaming fp16 form has its clears and writes in launches of their own (3 us); packed, the layer form has the same
 // three launches, and the cluster form, which cannot start under the appends, is 3 us ahead in 2-bit only (2-bit 32/4 heads 128 x 600
 // tokens 38.9 us a layer with the appends, streaming 40.9; 4-bit 32/4 48 x 2500 58.9 / 36.3, 16/8 64 x 1500 64.7 / 44.4).
-enum class LayerCaller { Engine, Launchers };
+// Paged: over block tables nothing is appended by either form, and long chains of few clusters lose earlier (cluster / streaming, 2-bit 32/4 heads
+// 4 x 8000 tokens 18.6 / 14.2 us, 16/8 17.3 / 17.3, 4-bit 16/8 19.5 / 17.3; 16 x 2000 18.2 / 19.6, 2-bit 32/4 12.4 / 16.0; 1 x 8000 11.6 / 16.2;
+// 64 x 100 13.5 / 12.6, 2-bit 12.5 / 13.8; 64 x 600 25.2 / 21.2, 2-bit 23.4 / 21.4; 2-bit 32/4 160 x 100 17.4 / 22.2, 160 x 600 30.5 / 29.9).
+enum class LayerCaller { Engine, Launchers, Paged };
 inline bool cluster_layer_faster(int bits, int G, int Hkv, int heads, long long rows, int max_tokens, LayerCaller caller) {
     const long long clusters = (long long)G * Hkv, sms = device_props().sm_count;
     const int S = cluster_split(bits, clusters, heads, max_tokens, true, true);
@@ -513,6 +516,7 @@ inline bool cluster_layer_faster(int bits, int G, int Hkv, int heads, long long 
         chain > (clusters > 2 * sms ? 2.2 : 4 * clusters > 3 * sms ? 2.5 : 2.8))
         return false;
     if (bits == 0) return (heads > 4 ? 0.5 : 1.0) * chain < 7.0 + 1.5 * turns + extra && !(clusters > 768 && chain > 2.0);
+    if (caller == LayerCaller::Paged && chain > 7.5 && clusters <= 32) return false;
     const double many = heads > 2 ? 0.0015 * std::max(0ll, clusters - 800) : 0.02 * std::max(0ll, clusters - 640);
     if (bits == 4 && heads > 4 ? chain * turns > 12.0 : chain > 12.0 + 5e-6 * (double)rows * Hkv) return false;
     return 0.4 * chain + 0.3 * chain * turns + 0.009 * clusters + many < 10.0 + 7e-6 * (double)rows * Hkv + 0.0004 * max_tokens + extra;

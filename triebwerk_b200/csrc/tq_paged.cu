@@ -95,8 +95,10 @@ int tq_paged_append(uint8_t* ck_q, void* k_norms, uint8_t* cv_q, void* v_norms, 
     int* status = nullptr;
     r = paged_status_word(&status);
     if (r != TQ_OK) return r;
-    // A CTA per token (2 * KV heads <= 16 vectors) while that is no more than a few turns of the SMs, tiles of 128 vectors behind that.
-    if (num_kv_heads <= 8 && T <= 4 * device_props().sm_count) {
+    // A CTA per token (2 * KV heads <= 16 vectors) while those are one turn of two per SM, tiles of 128 vectors behind that.  (us for 64, 148, 296, 444,
+    // 592 tokens, token / tile: 4-bit 8 KV heads 5.1 / 6.6, 5.6 / 6.6, 6.8 / 7.4, 10.4 / 7.5, 11.0 / 7.6; 2-bit 4 KV heads 4.5 / 6.5, 4.6 / 6.5, 5.5 / 6.4, 8.3 /
+    // 6.5, 8.5 / 6.5.)
+    if (num_kv_heads <= 8 && T <= 2 * device_props().sm_count) {
         LayerPrepParams p{};
         p.ck = ck_q; p.cv = cv_q; p.kn = (__half*)k_norms; p.vn = (__half*)v_norms;
         p.new_k = (const __half*)k_buf; p.new_v = (const __half*)v_buf; p.rotation = (const __half*)rotation; p.rot_copies = 1; p.status = status;
@@ -165,8 +167,11 @@ static PrefillCut prefill_cut(int T, int G, int H, int Hkv, int most) {
     // 121; 4-bit 64 x 1 behind 2000 66 / 75 / 86 / 96 / 141; 16/8 heads 3 x 4 behind 9000 94 / 59 / 47 / 39 / 28.)
     const long long ctas = (long long)Hkv * std::min((long long)G, (long long)T), room = 2 * sms;
     c.parts = (int)std::max(1ll, std::min({(3 * room + ctas) / (2 * ctas), (long long)most / (16 * ROWS_WARPS * 4), (long long)MAX_SPLITS}));
+    // Two blocks a CTA take 1.3 to 1.4 times as long as one, and the SMs serve a turn of CTAs at a time.  (us, one / two: 4-bit 32/8 heads 1 x 512 tokens
+    // 16.6 / 21.3, 1 x 2048 91.6 / 62.0, 4 x 512 52.4 / 39.6, 1 x 1024 behind 8192 273 / 209; 2-bit 16/8 2 x 512 behind 8192 139 / 186, 4 x 512
+    // 30.7 / 24.6, 4 x 2048 behind 4096 583 / 437.)  Blocks that leave half of the SMs idle are cut (2-bit 16/8 1 x 256 behind 20000: 294 uncut, 99).
     const long long blocks1 = Hkv * G * ((mean + qt - 1) / qt), blocks2 = Hkv * G * ((mean + 2 * qt - 1) / (2 * qt));
-    c.mt = mean > qt && 4 * blocks2 >= 5 * sms ? 2 : 1;
+    c.mt = mean > qt && 27 * ((blocks2 + sms - 1) / sms) < 20 * ((blocks1 + sms - 1) / sms) ? 2 : 1;
     c.splits = c.mt == 2 ? 1 : (int)std::max(1ll, std::min({sms / std::max(blocks1, 1ll), (long long)most / (4 * PFT_KT), (long long)MAX_SPLITS}));
     return c;
 }
@@ -212,7 +217,7 @@ int tq_paged_decode_attention(void* out, const void* q, const uint8_t* ck_q, con
     const int H = num_heads, Hkv = num_kv_heads, most = table_width * page_size, head_blocks = (H / Hkv + CD_HEADS - 1) / CD_HEADS;
     const long long rows = (long long)num_pages * page_size;
     const bool streams = fast_shape(H, Hkv, true) && G <= FUSED_MAX_G;
-    if (!streams || cluster_layer_faster(bits, G, Hkv, H / Hkv, (long long)G * most, most, LayerCaller::Launchers)) {
+    if (!streams || cluster_layer_faster(bits, G, Hkv, H / Hkv, (long long)G * most, most, LayerCaller::Paged)) {
         if (G > 65535 || (long long)Hkv * head_blocks > 65535) return TQ_ERR_UNSUPPORTED;
         ClusterDecodeParams p{};
         p.ck = ck_q; p.cv = cv_q; p.kn = (const __half*)k_norms; p.vn = (const __half*)v_norms; p.q = (const __half*)q; p.rotation = (const __half*)rotation;
