@@ -465,6 +465,44 @@ def test_prefill_norms_that_are_not_finite():
         assert torch.equal(bad, want)
 
 
+@pytest.mark.parametrize("bits", [4, 2])
+@pytest.mark.parametrize("H, Hkv, n", [(32, 8, 5), (16, 8, 12), (14, 2, 3), (32, 4, 3), (32, 8, 8), (16, 8, 16), (40, 8, 4), (16, 1, 2)])
+@pytest.mark.parametrize("G", [1, 7, 48])
+def test_prefill_a_few_tokens_each(H, Hkv, n, G, bits):
+    # as in checking drafted tokens: 17 to 24 score rows per KV head, and 32, of every request
+    past = [0, 1, 11, 12, 16, 31, 32, 33, 200, 640, 1500, 2111]
+    check_prefill([n + past[(5 * g + G) % 12] for g in range(G)], [n] * G, H, Hkv, bits, 32, n + G, tail=0)
+
+
+def test_prefill_one_prompt_beside_single_tokens():
+    rng = np.random.default_rng(17)
+    lens = rng.integers(1, 1200, 61).tolist()
+    lens[30] = 1500
+    check_prefill(lens, [600 if g == 30 else 1 for g in range(61)], 32, 8, 4, 64, 18)
+
+
+@pytest.mark.parametrize("new, n", [(40, 900), (5, 700)])
+def test_prefill_shared_pages_and_two_streams_at_once(new, n):
+    # requests whose rows name the same prompt pages; two calls on two streams, each with a workspace of its own
+    rng = np.random.default_rng(19)
+    G, H, Hkv = 6, 16, 8
+    lens, start = [n] * G, [new * g for g in range(G + 1)]
+    table, q, out, ck, cv, kn, vn, R, _ = attention_inputs(rng, lens, H, Hkv, 4, 64, T=new * G)
+    table[1:, :n // 128] = table[0, :n // 128]
+    d, st = i32(lens), i32(start)
+    q2, out2 = q.flip(0).contiguous(), torch.empty(new * G, H * 128, dtype=torch.float16, device="cuda")
+    work = [ops.paged_workspace(new * G, G, H) for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for s, ws, a, o in zip(streams, work, (q, q2), (out, out2)):
+            with torch.cuda.stream(s):
+                ops.paged_prefill_attention(o, a, ck, cv, kn, vn, R, table, d, st, 64, H, Hkv, 4, ws)
+    torch.cuda.synchronize()
+    for a, o in ((q, out), (q2, out2)):
+        pu.assert_attention(o, pu.attention(a, ck, cv, kn, vn, R, table, lens, start, 64, H, Hkv, 4))
+
+
 # ---- all together -----------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("bits, H, Hkv, page", [(4, 16, 8, 32), (2, 32, 8, 64), (4, 14, 2, 128)])
 def test_a_serving_loop(bits, H, Hkv, page):

@@ -157,16 +157,41 @@ struct PrefillCut {
     int mt, splits;      // large ones: blocks of 128 rows per CTA, parts of a block's tiles
 };
 constexpr int SPLIT_SMS = 160, MAX_SPLITS = 16;
+// Rows of partial sums that those calls may write.  Large requests are cut only while splits * blocks of 128 rows <= the SMs; small ones, of which a request
+// has 32 rows per KV head at most, into as many parts as fit.
+static size_t large_rows(long long T, long long H) { return (size_t)std::min<long long>(MAX_SPLITS * T * H, (long long)SPLIT_SMS * PFT_ROWS); }
+static size_t small_rows(long long T, long long G, long long H) {
+    return (size_t)std::max(std::min(T, (long long)ROWS_MOST * G) * H, std::min<long long>(MAX_SPLITS * T * H, 8ll * SPLIT_SMS * ROWS_MOST));
+}
 static PrefillCut prefill_cut(int T, int G, int H, int Hkv, int most) {
     const long long sms = std::min(device_props().sm_count, SPLIT_SMS), grp = H / Hkv, qt = PFT_ROWS / grp, mean = (T + G - 1) / G;
     PrefillCut c{};
     c.small = grp <= ROWS_MOST && (G > 1 || T * grp <= ROWS_MOST);
     c.large = grp > ROWS_MOST || T * grp > ROWS_MOST;
-    c.ncb = mean * grp <= 8 ? 1 : 2;
-    // One and a half turns of two CTAs per SM, four tiles of 16 tokens a warp at least.  (us by parts 1, 2, 3, 4, 8: 2-bit 32/8 heads 32 x 5 behind 4000 97 / 88 / 91 / 96 /
-    // 121; 4-bit 64 x 1 behind 2000 66 / 75 / 86 / 96 / 141; 16/8 heads 3 x 4 behind 9000 94 / 59 / 47 / 39 / 28.)
-    const long long ctas = (long long)Hkv * std::min((long long)G, (long long)T), room = 2 * sms;
-    c.parts = (int)std::max(1ll, std::min({(3 * room + ctas) / (2 * ctas), (long long)most / (16 * ROWS_WARPS * 4), (long long)MAX_SPLITS}));
+    // Small ones.  A CTA takes start + turn * (its warps' turns of 16 tokens), us by row blocks per CTA below; as many at a time as the SMs hold, and half
+    // a turn more where there are several (contexts differ).  Up to 16 rows in one CTA; 17 to 24, where all requests have as many (T is a multiple of G), in one of three
+    // blocks, alone on its SM, or in two of two.  Requests that differ count for half as many rows again as their mean.  (Two / three blocks, best parts of
+    // each, us: 32/8 heads 32 x 5 behind 4000 2-bit 137 / 115, 4-bit 157 / 140; 4-bit 8 x 5 behind 4000 51 / 47, 64 x 6 behind 1000 112 / 125; 2-bit 2 x 5 behind
+    // 30000 74 / 59; 32/4 16 x 3 behind 6000 68 / 59; 2-bit 32/8 32 x 1 to 5 behind 2000 to 4000 88 / 107.  By parts 1, 2, 3, 4: the last, two blocks 94 / 88 / 91 / 96;
+    // 4-bit 8 x 5, three blocks 69 / 47 / 61 / 58; 16/8 64 x 1 behind 2000 75 / 85 / 97 / 104.)
+    const bool alike = T % G == 0;
+    const long long rows = std::min(mean * grp, (long long)ROWS_MOST), tiles = (most + 15) / 16;
+    const long long most_parts = std::min<long long>(MAX_SPLITS, (long long)small_rows(T, G, H) / std::max(1ll, std::min<long long>(T, G * (ROWS_MOST / grp)) * H));
+    double best = 1e30;
+    for (int ncb = rows <= 8 ? 1 : 2; ncb <= (rows <= 8 ? 1 : alike && rows > 16 && rows <= 24 ? 3 : 2); ++ncb) {
+        const double start = ncb == 1 ? 5.0 : ncb == 2 ? 7.0 : 11.0, turn = ncb == 1 ? 1.6 : ncb == 2 ? 2.4 : 2.7;
+        const long long warps = ncb == 3 ? ROWS_WARPS<3> : ROWS_WARPS<2>, room = ncb == 3 ? sms : 2 * sms;
+        const long long ctas = Hkv * std::min<long long>(G, T) * (((alike ? rows : std::min(rows * 3 / 2, (long long)ROWS_MOST)) + 8 * ncb - 1) / (8 * ncb));
+        for (long long parts = 1; parts <= std::max(1ll, most_parts); ++parts) {
+            const double turns = ctas * parts <= room ? 1.0 : 0.5 + (double)(ctas * parts) / (double)room;
+            const double us = turns * (start + turn * ((tiles + warps * parts - 1) / (warps * parts)));
+            if (us < best) {
+                best = us;
+                c.ncb = ncb;
+                c.parts = (int)parts;
+            }
+        }
+    }
     // Two blocks a CTA take 1.3 to 1.4 times as long as one, and the SMs serve a turn of CTAs at a time.  (us, one / two: 4-bit 32/8 heads 1 x 512 tokens
     // 16.6 / 21.3, 1 x 2048 91.6 / 62.0, 4 x 512 52.4 / 39.6, 1 x 1024 behind 8192 273 / 209; 2-bit 16/8 2 x 512 behind 8192 139 / 186, 4 x 512
     // 30.7 / 24.6, 4 x 2048 behind 4096 583 / 437.)  Blocks that leave half of the SMs idle are cut (2-bit 16/8 1 x 256 behind 20000: 294 uncut, 99).
@@ -175,13 +200,6 @@ static PrefillCut prefill_cut(int T, int G, int H, int Hkv, int most) {
     c.splits = c.mt == 2 ? 1 : (int)std::max(1ll, std::min({sms / std::max(blocks1, 1ll), (long long)most / (4 * PFT_KT), (long long)MAX_SPLITS}));
     return c;
 }
-// Rows of partial sums that those calls write.  Large requests are cut only while splits * blocks of 128 rows <= the SMs; small ones, of which a
-// request has 32 rows per KV head at most, only while parts * CTAs < 4 * 2 SMs.
-static size_t large_rows(long long T, long long H) { return (size_t)std::min<long long>(MAX_SPLITS * T * H, (long long)SPLIT_SMS * PFT_ROWS); }
-static size_t small_rows(long long T, long long G, long long H) {
-    return (size_t)std::max(std::min(T, (long long)ROWS_MOST * G) * H, std::min<long long>(MAX_SPLITS * T * H, 8ll * SPLIT_SMS * ROWS_MOST));
-}
-
 extern "C" {
 
 size_t tq_paged_workspace_bytes(int T, int G, int num_heads) {
@@ -278,7 +296,7 @@ template <int BITS, int NCB>
 static int launch_rows(const PagedRowsParams& p, dim3 grid, cudaStream_t s) {
     constexpr size_t smem = rows_smem_bytes<BITS, NCB>();
     const int r = ensure_dynamic_smem((const void*)paged_rows_kernel<BITS, NCB>, smem);
-    return r != TQ_OK ? r : launch_kernel(paged_rows_kernel<BITS, NCB>, grid, dim3(ROWS_THREADS), smem, s, use_pdl(), p);
+    return r != TQ_OK ? r : launch_kernel(paged_rows_kernel<BITS, NCB>, grid, dim3(ROWS_THREADS<NCB>), smem, s, use_pdl(), p);
 }
 
 extern "C" {
@@ -330,13 +348,14 @@ int tq_paged_prefill_attention(void* out, const void* q, const uint8_t* ck_q, co
         p.ck = ck_q; p.cv = cv_q; p.kn = (const __half*)k_norms; p.vn = (const __half*)v_norms; p.q = (const __half*)q; p.rotation = (const __half*)rotation;
         p.block_table = block_table; p.lens = seq_lens; p.start = query_start; p.partials = small_sums; p.status = status;
         p.table_stride = table_stride; p.page_shift = shift; p.num_pages = num_pages; p.most_tokens = most;
-        p.T = T; p.H = H; p.Hkv = Hkv; p.grp = grp; p.q_stride = q_stride; p.row_blocks = ROWS_MOST / (8 * cut.ncb); p.behind = cut.large;
+        p.T = T; p.H = H; p.Hkv = Hkv; p.grp = grp; p.q_stride = q_stride; p.row_blocks = (ROWS_MOST + 8 * cut.ncb - 1) / (8 * cut.ncb); p.behind = cut.large;
         p.by_request = (long long)G * most_small < T ? most_small : 0;
         p.part_tokens = p.by_request ? G * most_small : T;
         const long long ctas = (long long)Hkv * p.row_blocks * G;
         if (ctas >= (1ll << 31)) return TQ_ERR_UNSUPPORTED;
         const dim3 grid((unsigned)ctas, 1, (unsigned)cut.parts);
         if (cut.ncb == 1) r = bits == 4 ? launch_rows<4, 1>(p, grid, cs(s)) : launch_rows<2, 1>(p, grid, cs(s));
+        else if (cut.ncb == 3) r = bits == 4 ? launch_rows<4, 3>(p, grid, cs(s)) : launch_rows<2, 3>(p, grid, cs(s));
         else r = bits == 4 ? launch_rows<4, 2>(p, grid, cs(s)) : launch_rows<2, 2>(p, grid, cs(s));
         if (r != TQ_OK) return r;
         m.small_splits = cut.parts; m.part_tokens = p.part_tokens; m.by_request = p.by_request;

@@ -1,14 +1,19 @@
 // Attention of requests with few new tokens over paged packed caches, on mma.sync, sm_100a: the part of tq_paged_prefill_attention for
 // requests with at most ROWS_MOST score rows (new tokens x query heads) per KV head; tq_paged_prefill.cuh, whose tcgen05 products take 128
-// rows whatever there is, has the others.  32 requests of 5 tokens behind 4000, 2-bit, 32/8 heads: 131 us there.
+// rows whatever there is, has the others.
 //
 //   * A CTA has up to 8 NCB rows of one request and KV head, and a share of its tokens (gridDim.z parts).  Its warps take 16 tokens at a
 //     time, in turn, each on its own: codes go from global memory into registers in fragment order, a tile ahead, and become fp16
 //     centroids through a shared-memory table (the cluster kernel's layout, tq_decode_cluster.cuh), with no barrier in the loop.
 //   * S^T = K Q^T (tokens in the M dimension, rows of queries in N, 8 to a block) and O^T += V^T P^T.  What is made of the codes is used
 //     for all row blocks: 190 instructions a warp and 16 tokens, and 78 for each block.  (tcgen05: 6500 warp instructions per 128 tokens.)
+//     So a CTA takes all blocks that its registers hold: two with two CTAs per SM, three with one.
 //   * The queries are rotated at the start (R from L2, in fragments) and lie in shared memory in fragment order.
 //   * The warps' sums meet in shared memory, halves in turn; the CTA's go to the workspace, paged_merge_kernel adds the parts up.
+//
+// What bounds it is instruction issue (55 % of the slots used under a profiler) and a CTA's start and end, 5 to 11 us in all: 32 requests of 5 tokens behind
+// 4000, 2-bit, 32/8 heads (71 MB of codes and norms, 11 us at the copy rate) take 115 us with the merge, 4-bit 139; of 1 to 5 tokens behind 2000 to 4000 88 us,
+// 131 us on the tcgen05 kernel.
 #pragma once
 
 #include "tq_decode_cluster.cuh"
@@ -17,7 +22,10 @@
 namespace tq {
 
 constexpr int ROWS_MOST = 32;
-constexpr int ROWS_WARPS = 8, ROWS_THREADS = 32 * ROWS_WARPS;
+template <int NCB>
+constexpr int ROWS_WARPS = NCB <= 2 ? 8 : 12;  // (two CTAs per SM, or one whose sums take the room)
+template <int NCB>
+constexpr int ROWS_THREADS = 32 * ROWS_WARPS<NCB>;
 constexpr uint32_t ROWS_LUT_ABS = 0x8000u;  // one entry (a column per lane) every 256 bytes: one PRMT makes a look-up's address
 constexpr uint32_t ROWS_MAX_BASE = 0x480u;  // dynamic shared memory starts at or below this address
 
@@ -37,7 +45,7 @@ struct PagedRowsParams {
     int table_stride, page_shift, num_pages, most_tokens;
     int T, H, Hkv, grp, q_stride;
     int behind;       // see the kernel
-    int row_blocks;   // CTAs per request, KV head and part: ROWS_MOST / (8 NCB)
+    int row_blocks;   // CTAs per request, KV head and part: ROWS_MOST / (8 NCB), rounded up
 };
 
 template <int NCB>
@@ -53,14 +61,16 @@ constexpr size_t rows_smem_bytes() {  // counted from address 0
 }
 
 template <int BITS, int NCB>
-__global__ void __launch_bounds__(ROWS_THREADS, 2) paged_rows_kernel(const PagedRowsParams p) {
+__global__ void __launch_bounds__(ROWS_THREADS<NCB>, NCB <= 2 ? 2 : 1) paged_rows_kernel(const PagedRowsParams p) {
     extern __shared__ __align__(1024) uint8_t rows_smem[];
+    constexpr int WARPS = ROWS_WARPS<NCB>, THREADS = ROWS_THREADS<NCB>;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gl = lane >> 2, t4 = lane & 3;
     const uint32_t base = (smem_u32(rows_smem) + 127u) & ~127u;
     uint8_t* const gb = rows_smem + (base - smem_u32(rows_smem));
-    static_assert(ROWS_MAX_BASE + RowsSmem<NCB>::END <= ROWS_LUT_ABS && ROWS_MAX_BASE + (ROWS_WARPS / 2) * RowsSmem<NCB>::WARP <= ROWS_LUT_ABS, "below the table");
+    static_assert(ROWS_MAX_BASE + RowsSmem<NCB>::END <= ROWS_LUT_ABS && ROWS_MAX_BASE + (WARPS / 2) * RowsSmem<NCB>::WARP <= ROWS_LUT_ABS, "below the table");
     if (base > ROWS_MAX_BASE) {
         if (tid == 0) atomicMax(p.status, ST_SMEM_LAYOUT);
+        pdl_wait();
         return;
     }
     constexpr int BPH = HEAD_DIM * BITS / 8;
@@ -85,7 +95,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, 2) paged_rows_kernel(const Paged
 #pragma unroll
         for (int i = 0; i < (BITS == 4 ? 8 : 1); ++i) {
             const uint32_t u = pack_half2(first, c * (BITS == 4 ? kCent4[(tid >> 7) + 2 * i] : kCent2[(e >> 2) & 3]));
-            if (BITS == 4 || e < 16)
+            if (BITS == 4 ? tid < 256 : e < 16)
                 asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(ROWS_LUT_ABS + (uint32_t)(e + 32 * i) * 256u + (uint32_t)(tid & 7) * 16u), "r"(u) : "memory");
         }
     }
@@ -106,7 +116,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, 2) paged_rows_kernel(const Paged
     auto fetch_page = [&](int b) { if (b < b_hi) page = (uint32_t)__ldg(my_pages + ((16 * b) >> p.page_shift)); };
     auto use_page = [&](int b) {  // (16 tokens lie within one page; its number is requested a turn ahead)
         row0 = ((size_t)min(page, (uint32_t)p.num_pages - 1u) << p.page_shift) + (size_t)((16 * b) & ((1 << p.page_shift) - 1));
-        fetch_page(b + ROWS_WARPS);
+        fetch_page(b + WARPS);
     };
     // (rows behind the last token: zero codes with zero norms)
     auto load_k = [&](int b) {
@@ -154,12 +164,14 @@ __global__ void __launch_bounds__(ROWS_THREADS, 2) paged_rows_kernel(const Paged
 
     // R's fragments: rows 16 warp .. + 15; step (m, e) of lane t4 covers k = 32 m + 8 t4 + 4 e .. + 3, on both sides
     uint4 bf[2][4];
+    if (warp < 8)
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int m = 0; m < 4; ++m) bf[i][m] = ldg128_now(reinterpret_cast<const uint4*>(p.rotation + (size_t)(8 * (2 * warp + i) + gl) * HEAD_DIM) + t4 + 4 * m);
     // ---- queries: rot[r][c] = sum_k q[r][k] R[c][k], scaled by log2(e) / sqrt(128); a warp has the coordinates 16 warp .. + 15 ----
     {
+        if (warp < 8)
 #pragma unroll
         for (int mt = 0; mt < (NCB + 1) / 2; ++mt) {
             uint4 a[2][4];
@@ -193,7 +205,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, 2) paged_rows_kernel(const Paged
                             pack_half2(c[i][2 * r] * sc, c[i][2 * r + 1] * sc);
         }
         __syncthreads();
-        for (int i = tid; i < NCB * 128; i += ROWS_THREADS) {  // lane l of row block nb: row l / 4, coordinates 32 (l & 3) + 8 m ..
+        for (int i = tid; i < NCB * 128; i += THREADS) {  // lane l of row block nb: row l / 4, coordinates 32 (l & 3) + 8 m ..
             const int nb = i >> 7, m = (i >> 5) & 3, l = i & 31;
             *reinterpret_cast<uint4*>(gb + RowsSmem<NCB>::FRAG + 16u * (uint32_t)i) =
                 *reinterpret_cast<const uint4*>(gb + RowsSmem<NCB>::Q + (uint32_t)((8 * nb + (l >> 2)) * MERGE_ROW + 32 * (l & 3) + 8 * m) * 2u);
@@ -226,8 +238,8 @@ __global__ void __launch_bounds__(ROWS_THREADS, 2) paged_rows_kernel(const Paged
     // (one copy of the loop for each number of row blocks in use: a branch around every product cost a third of the time)
     auto walk = [&](auto used_) {
     constexpr int USED = decltype(used_)::value;
-    for (; b < b_hi; b += ROWS_WARPS) {
-        const int t0 = 16 * b, next = b + ROWS_WARPS;
+    for (; b < b_hi; b += WARPS) {
+        const int t0 = 16 * b, next = b + WARPS;
         // ---- scores: tokens gl and gl + 8, rows 2 t4 and 2 t4 + 1 of each block ----
         float c[USED][4];
 #pragma unroll
@@ -335,6 +347,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, 2) paged_rows_kernel(const Paged
     }
     };
     if (NCB == 1 || used == 1) walk(std::integral_constant<int, 1>());
+    else if (NCB > 2 && used == 2) walk(std::integral_constant<int, NCB < 2 ? 1 : 2>());
     else walk(std::integral_constant<int, NCB>());
 
     // ---- the warps' sums meet: the upper half of those left hand theirs to the lower half, lane by lane ----
@@ -345,19 +358,20 @@ __global__ void __launch_bounds__(ROWS_THREADS, 2) paged_rows_kernel(const Paged
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) l_run[nb][e] += __shfl_xor_sync(0xffffffffu, l_run[nb][e], o);
 #pragma unroll 1
-    for (int half = ROWS_WARPS / 2; half > 0; half >>= 1) {
+    for (int left = WARPS; left > 1;) {
+        const int half = (left + 1) / 2;  // (an odd number: the one in the middle keeps its own)
         float4* const mine = reinterpret_cast<float4*>(gb + (uint32_t)(warp >= half ? warp - half : warp) * RowsSmem<NCB>::WARP) + lane;
 #pragma unroll
         for (int nb = 0; nb < NCB; ++nb) {
             if (nb >= used) continue;  // (uniform)
             __syncthreads();  // (queries are no longer read; the sums before have been)
-            if (warp >= half && warp < 2 * half) {
+            if (warp >= half && warp < left) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) mine[i * 32] = make_float4(acc[nb][i][0], acc[nb][i][1], acc[nb][i][2], acc[nb][i][3]);
                 mine[8 * 32] = make_float4(m_run[nb][0], m_run[nb][1], l_run[nb][0], l_run[nb][1]);
             }
             __syncthreads();
-            if (warp < half) {
+            if (warp < left - half) {
                 const float4 s = mine[8 * 32];
                 const float m2[2] = {s.x, s.y}, l2[2] = {s.z, s.w};
                 float f[2], f2[2];
@@ -379,6 +393,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, 2) paged_rows_kernel(const Paged
                 }
             }
         }
+        left = half;
     }
     leave();
     if (warp > 0) return;
