@@ -411,7 +411,9 @@ int tq_engine_decode_step_host(tq_engine* e, const void* q_host, const void* k_h
  * owners, so such rows are the caller's to release.  A page number outside the pool reads as the pool's last page.  Lengths are
  * those in device memory at the time the kernels run: all calls can be captured into a graph, whose replays follow new lengths.
  * kv_bits 4 and 2, head_dim 128, num_heads a multiple of num_kv_heads.  Codes, q, out, K, V, rotation: 16-byte aligned; strides are in
- * elements, multiples of 8.  Calls check their arguments before anything is enqueued.
+ * elements, multiples of 8.  What a call writes overlaps nothing that it reads, but where that is said.  Fewer than 2^31 rows, 2^30 vectors (T *
+ * num_kv_heads) of a call that stores or reads, 2^31 query rows (T * num_heads); at most 65535 requests of an attention.  Calls check their
+ * arguments before anything is enqueued.
  * =================================================================================================================== */
 
 /* Block tables and slot maps of one step, from lengths.  Request g holds context_lens[g] tokens (a negative value x: ~x, see below)
@@ -457,7 +459,7 @@ int tq_paged_decode_attention(void* out, const void* q, const uint8_t* ck_q, con
 /* Causal attention of several new tokens per request (prompts, chunks behind earlier tokens, drafted tokens): the query tokens
  * query_start[g] .. query_start[g + 1] - 1 (device, [G + 1], ascending from 0, at most T) are the last ones of request g's seq_lens[g] tokens, whose
  * rows are in the cache already; query i of n stands at position seq_lens[g] - n + i and attends to tokens 0 .. there (none: zeros, so
- * also where seq_lens[g] is 0 or negative).  Rows of out behind query_start[G] are left as they are.  Up to 128 query heads per KV head. */
+ * also where seq_lens[g] is 0 or negative; lengths count up to table_width * page_size).  Rows of out behind query_start[G] are left as they are.  Up to 128 query heads per KV head. */
 int tq_paged_prefill_attention(void* out, const void* q, const uint8_t* ck_q, const uint8_t* cv_q, const void* k_norms,
                                const void* v_norms, const void* rotation, const int* block_table, int table_stride, int table_width,
                                const int* seq_lens, const int* query_start, int num_pages, int page_size, int T, int G, int num_heads,

@@ -97,6 +97,9 @@ def attention(q, ck, cv, kn, vn, R, table, lens, start, page, H, Hkv, bits):
     weight, the weight relatively by as much; the weight (times its norm) by EPS^2 / 3; V's centroids by EPS^2 / 3.  The output moves by the
     sum over the tokens of w_t v_t times those: its squared 2-norm is sum_t w_t^2 |v_t|^2 (their variances' sum) in the mean.  Allowed are six
     times its root, and for the result's rounding, and V's centroids' errors, which are the same wherever a code is, 2 EPS |out|.
+    (The prefill kernel for many rows takes the centroids times norms as K's and V's operands, one rounding each as well, and rounds its result before
+    the last product, by R: its roundings are 2^-11 / sqrt(3) of it in the mean there and as much at the end, and V's centroids, scaled, are off by 0.22
+    of EPS at most: 1.4 EPS |out| together.)
     (fp32 sums of 128 and of n terms, 2^-24 each, and weights below fp16's normal range, 2^-25 each next to a sum of at least 1, are far
     below that: n 2^-25 |v| is added for them.)"""
     T = q.shape[0]

@@ -64,7 +64,8 @@ def prefill(**kw):
 
 @pytest.mark.parametrize("change, status", [
     (dict(start=None), -1), (dict(T=-1), -1), (dict(H=258, Hkv=2, qs=258 * 128, os=258 * 128), -4), (dict(bytes=1000), -3), (dict(ws=None), -3), (dict(lens=None), -1),
-    (dict(table=None), -1), (dict(page=24), -4), (dict(G=0), -1), (dict(bits=0), -1), (dict(q=ODD), -1), (dict(qs=2044), -1)])
+    (dict(table=None), -1), (dict(page=24), -4), (dict(G=0), -1), (dict(bits=0), -1), (dict(q=ODD), -1), (dict(qs=2044), -1),
+    (dict(G=65536, bytes=1 << 33), -4), (dict(T=1 << 27), -4)])
 def test_prefill_refuses(change, status):
     assert prefill(**change) == status
 
@@ -78,7 +79,7 @@ def test_prefill_of_no_tokens_is_no_work():
     (dict(H=0), -1), (dict(qs=2040), -1), (dict(qs=2052), -1), (dict(os=2047), -1), (dict(stride=4), -1), (dict(width=0), -1), (dict(pages=0), -1),
     (dict(pages=1 << 26), -4), (dict(out=None), -1), (dict(q=None), -1), (dict(ck=None), -1), (dict(cv=None), -1), (dict(kn=None), -1), (dict(vn=None), -1),
     (dict(R=None), -1), (dict(table=None), -1), (dict(lens=None), -1), (dict(ws=None), -3), (dict(ws=ODD), -3), (dict(bytes=1000), -3), (dict(q=ODD), -1),
-    (dict(out=ODD), -1), (dict(kn=ODD), -1)])
+    (dict(out=ODD), -1), (dict(kn=ODD), -1), (dict(G=65536, bytes=1 << 33), -4)])
 def test_decode_refuses(change, status):
     assert attention(**change) == status
 

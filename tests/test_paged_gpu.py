@@ -1,4 +1,8 @@
 """Paged caches on the GPU: plans against whole numbers, appends against the launchers' bytes, reads and attention against 64 bits."""
+import pathlib
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
@@ -501,6 +505,42 @@ def test_prefill_shared_pages_and_two_streams_at_once(new, n):
     torch.cuda.synchronize()
     for a, o in ((q, out), (q2, out2)):
         pu.assert_attention(o, pu.attention(a, ck, cv, kn, vn, R, table, lens, start, 64, H, Hkv, 4))
+
+
+FIRST_CALLS_CAPTURED = """
+import torch
+from triebwerk_b200 import ops
+R = ops.rotation_matrix().cuda()
+ck, cv = (torch.zeros(256, 8 * 64, dtype=torch.uint8, device="cuda") for _ in range(2))
+kn, vn = (torch.zeros(256, 8, dtype=torch.float16, device="cuda") for _ in range(2))
+k, v, q = (torch.randn(8, n * 128, device="cuda").half() for n in (8, 8, 16))
+out, prompt, k2, v2 = (torch.zeros_like(x) for x in (q, q, k, v))
+i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+table, stack, count, lens, new, start = torch.zeros(8, 2, dtype=torch.int32, device="cuda"), i32(*range(8)), i32(8), i32(*[0] * 8), i32(*[1] * 8), i32(*[0] * 9)
+slots, ws = torch.zeros(8, dtype=torch.int64, device="cuda"), ops.paged_workspace(8, 8, 16)
+graph = torch.cuda.CUDAGraph()
+torch.cuda.synchronize()
+with torch.cuda.graph(graph):
+    ops.page_plan(table, stack, count, count, lens, new, None, 32, lens, start, slots)
+    ops.paged_append(ck, kn, cv, vn, k, v, R, slots, 8, 4)
+    ops.paged_decode_attention(out, q, ck, cv, kn, vn, R, table, lens, 32, 16, 8, 4, ws)
+    ops.paged_prefill_attention(prompt, q, ck, cv, kn, vn, R, table, lens, start, 32, 16, 8, 4, ws)
+    ops.paged_read(k2, v2, ck, kn, cv, vn, R, slots, 8, 4)
+graph.replay()
+torch.cuda.synchronize()
+assert lens.tolist() == [1] * 8 and int(count) == 0 and ops.paged_status() == 0
+# one token each: the attentions give its value back, to five roundings of 2^-11 (weight, centroid, result before and behind R; what was read)
+want = v2.view(8, 8, 1, 128).expand(8, 8, 2, 128).reshape(8, -1).double()
+for got in (out, prompt):
+    assert (got - want).norm() < 5 * 2.0**-11 * want.norm()
+assert (v2 - v).double().square().sum() < 0.012 * v.double().square().sum()  # (0.0095: the 4-bit code book's error)
+"""
+
+
+def test_the_first_calls_of_a_process_captured():
+    root = str(pathlib.Path(__file__).resolve().parent.parent)
+    done = subprocess.run([sys.executable, "-c", FIRST_CALLS_CAPTURED], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
 
 
 # ---- all together -----------------------------------------------------------------------------------------------------------------

@@ -229,14 +229,14 @@ int tq_paged_decode_attention(void* out, const void* q, const uint8_t* ck_q, con
                             num_heads, num_kv_heads, head_dim, q_stride, out_stride, bits);
     if (r != TQ_OK) return r;
     if (!workspace || workspace_bytes < tq_paged_workspace_bytes(G, G, num_heads) || !aligned({workspace}, 256)) return TQ_ERR_WORKSPACE;
+    const int H = num_heads, Hkv = num_kv_heads, most = table_width * page_size, head_blocks = (H / Hkv + CD_HEADS - 1) / CD_HEADS;
+    if (G > 65535 || (long long)Hkv * head_blocks > 65535) return TQ_ERR_UNSUPPORTED;
     int* status = nullptr;
     r = paged_status_word(&status);
     if (r != TQ_OK) return r;
-    const int H = num_heads, Hkv = num_kv_heads, most = table_width * page_size, head_blocks = (H / Hkv + CD_HEADS - 1) / CD_HEADS;
     const long long rows = (long long)num_pages * page_size;
     const bool streams = fast_shape(H, Hkv, true) && G <= FUSED_MAX_G;
     if (!streams || cluster_layer_faster(bits, G, Hkv, H / Hkv, (long long)G * most, most, LayerCaller::Paged)) {
-        if (G > 65535 || (long long)Hkv * head_blocks > 65535) return TQ_ERR_UNSUPPORTED;
         ClusterDecodeParams p{};
         p.ck = ck_q; p.cv = cv_q; p.kn = (const __half*)k_norms; p.vn = (const __half*)v_norms; p.q = (const __half*)q; p.rotation = (const __half*)rotation;
         p.out = (__half*)out; p.positions = seq_lens; p.capacity_rows = most; p.max_seq_len = most; p.status = status;
