@@ -733,12 +733,15 @@ static __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedMerg
     __shared__ __align__(16) __half a_s[2][16][HEAD_DIM + 8];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gl = lane >> 2, t4 = lane & 3;
     pdl_launch_dependents();
-    pdl_wait();
+    // (the kernels before let this one start when what came before the call has finished: R and the batch may be read; the sums not yet)
     const int s0 = max(p.start[blockIdx.y], 0), n = max(min(p.start[blockIdx.y + 1], p.T) - s0, 0);
     const bool large = n * p.grp > p.small_rows;
     const int splits = large ? p.splits : p.small_splits;
     const long long rows = (long long)n * p.H;
-    if (splits == 0 || 16ll * blockIdx.x >= rows) return;
+    if (splits == 0 || 16ll * blockIdx.x >= rows) {
+        pdl_wait();
+        return;
+    }
     uint32_t bf[2][8][2];
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
@@ -757,6 +760,7 @@ static __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedMerg
             bf[1][4 * half + j][0] = r[2]; bf[1][4 * half + j][1] = r[3];
         }
     }
+    pdl_wait();
     const size_t part = (size_t)(large ? p.T : p.part_tokens) * p.H * PART_STRIDE;
     const float* const sums = (large ? p.partials : p.small_partials) + (size_t)(!large && p.by_request ? (int)blockIdx.y * p.by_request : s0) * p.H * PART_STRIDE;
     for (long long row0 = 16ll * blockIdx.x; row0 < rows; row0 += 16ll * gridDim.x) {
