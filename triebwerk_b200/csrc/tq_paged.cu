@@ -168,12 +168,13 @@ static PrefillCut prefill_cut(int T, int G, int H, int Hkv, int most) {
     PrefillCut c{};
     c.small = grp <= ROWS_MOST && (G > 1 || T * grp <= ROWS_MOST);
     c.large = grp > ROWS_MOST || T * grp > ROWS_MOST;
-    // Small ones.  A CTA takes start + turn * (its warps' turns of 16 tokens), us by row blocks per CTA below; as many at a time as the SMs hold, and half
-    // a turn more where there are several (contexts differ).  Up to 16 rows in one CTA; 17 to 24, where all requests have as many (T is a multiple of G), in one of three
-    // blocks, alone on its SM, or in two of two.  Requests that differ count for half as many rows again as their mean.  (Two / three blocks, best parts of
-    // each, us: 32/8 heads 32 x 5 behind 4000 2-bit 137 / 115, 4-bit 157 / 140; 4-bit 8 x 5 behind 4000 51 / 47, 64 x 6 behind 1000 112 / 125; 2-bit 2 x 5 behind
-    // 30000 74 / 59; 32/4 16 x 3 behind 6000 68 / 59; 2-bit 32/8 32 x 1 to 5 behind 2000 to 4000 88 / 107.  By parts 1, 2, 3, 4: the last, two blocks 94 / 88 / 91 / 96;
-    // 4-bit 8 x 5, three blocks 69 / 47 / 61 / 58; 16/8 64 x 1 behind 2000 75 / 85 / 97 / 104.)
+    // Small ones.  A CTA takes start + turn * (its warps' turns of 16 tokens), us by row blocks per CTA below; as many at a time as the SMs hold, and part of
+    // a turn more where there are several (contexts differ; less of it where the longest come first).  Up to 16 rows in one CTA; 17 to 24, where all requests
+    // have as many (T is a multiple of G), in one of three blocks, alone on its SM, or in two of two.  Requests that differ count for half as many rows again as
+    // their mean.  (Two / three blocks, best parts of each, us: 32/8 heads 32 x 5 behind 4000 2-bit 137 / 115, 4-bit 157 / 140; 4-bit 8 x 5 behind 4000 51 / 47,
+    // 64 x 6 behind 1000 112 / 125; 2-bit 2 x 5 behind 30000 74 / 59; 32/4 16 x 3 behind 6000 68 / 59; 2-bit 32/8 32 x 1 to 5 behind 2000 to 4000 86 / 96.  By
+    // parts 1, 2, 3, 4: the last, two blocks 87 / 86 / 92 / 103; 4-bit 8 x 5, three blocks 69 / 47 / 61 / 58; 16/8 64 x 1 behind 2000 75 / 85 / 97 / 104, 48 x 1
+    // behind 100 to 4000 60 / 69 / 83 / 95; 32/8 32 x 5 behind 1000 to 8000 146 / 170 / 197 / 209.)
     const bool alike = T % G == 0;
     const long long rows = std::min(mean * grp, (long long)ROWS_MOST), tiles = (most + 15) / 16;
     const long long most_parts = std::min<long long>(MAX_SPLITS, (long long)small_rows(T, G, H) / std::max(1ll, std::min<long long>(T, G * (ROWS_MOST / grp)) * H));
@@ -183,7 +184,7 @@ static PrefillCut prefill_cut(int T, int G, int H, int Hkv, int most) {
         const long long warps = ncb == 3 ? ROWS_WARPS<3> : ROWS_WARPS<2>, room = ncb == 3 ? sms : 2 * sms;
         const long long ctas = Hkv * std::min<long long>(G, T) * (((alike ? rows : std::min(rows * 3 / 2, (long long)ROWS_MOST)) + 8 * ncb - 1) / (8 * ncb));
         for (long long parts = 1; parts <= std::max(1ll, most_parts); ++parts) {
-            const double turns = ctas * parts <= room ? 1.0 : 0.5 + (double)(ctas * parts) / (double)room;
+            const double turns = ctas * parts <= room ? 1.0 : (G <= ROWS_SORTED ? 0.25 : 0.5) + (double)(ctas * parts) / (double)room;
             const double us = turns * (start + turn * ((tiles + warps * parts - 1) / (warps * parts)));
             if (us < best) {
                 best = us;
@@ -348,12 +349,12 @@ int tq_paged_prefill_attention(void* out, const void* q, const uint8_t* ck_q, co
         p.ck = ck_q; p.cv = cv_q; p.kn = (const __half*)k_norms; p.vn = (const __half*)v_norms; p.q = (const __half*)q; p.rotation = (const __half*)rotation;
         p.block_table = block_table; p.lens = seq_lens; p.start = query_start; p.partials = small_sums; p.status = status;
         p.table_stride = table_stride; p.page_shift = shift; p.num_pages = num_pages; p.most_tokens = most;
-        p.T = T; p.H = H; p.Hkv = Hkv; p.grp = grp; p.q_stride = q_stride; p.row_blocks = (ROWS_MOST + 8 * cut.ncb - 1) / (8 * cut.ncb); p.behind = cut.large;
+        p.T = T; p.G = G; p.H = H; p.Hkv = Hkv; p.grp = grp; p.q_stride = q_stride; p.parts = cut.parts; p.row_blocks = (ROWS_MOST + 8 * cut.ncb - 1) / (8 * cut.ncb); p.behind = cut.large;
         p.by_request = (long long)G * most_small < T ? most_small : 0;
         p.part_tokens = p.by_request ? G * most_small : T;
-        const long long ctas = (long long)Hkv * p.row_blocks * G;
+        const long long ctas = (long long)Hkv * p.row_blocks * cut.parts * G;
         if (ctas >= (1ll << 31)) return TQ_ERR_UNSUPPORTED;
-        const dim3 grid((unsigned)ctas, 1, (unsigned)cut.parts);
+        const dim3 grid((unsigned)ctas);
         if (cut.ncb == 1) r = bits == 4 ? launch_rows<4, 1>(p, grid, cs(s)) : launch_rows<2, 1>(p, grid, cs(s));
         else if (cut.ncb == 3) r = bits == 4 ? launch_rows<4, 3>(p, grid, cs(s)) : launch_rows<2, 3>(p, grid, cs(s));
         else r = bits == 4 ? launch_rows<4, 2>(p, grid, cs(s)) : launch_rows<2, 2>(p, grid, cs(s));

@@ -2,7 +2,7 @@
 // requests with at most ROWS_MOST score rows (new tokens x query heads) per KV head; tq_paged_prefill.cuh, whose tcgen05 products take 128
 // rows whatever there is, has the others.
 //
-//   * A CTA has up to 8 NCB rows of one request and KV head, and a share of its tokens (gridDim.z parts).  Its warps take 16 tokens at a
+//   * A CTA has up to 8 NCB rows of one request and KV head, and a share of its tokens (one of `parts`).  Its warps take 16 tokens at a
 //     time, in turn, each on its own: codes go from global memory into registers in fragment order, a tile ahead, and become fp16
 //     centroids through a shared-memory table (the cluster kernel's layout, tq_decode_cluster.cuh), with no barrier in the loop.
 //   * S^T = K Q^T (tokens in the M dimension, rows of queries in N, 8 to a block) and O^T += V^T P^T.  What is made of the codes is used
@@ -11,8 +11,8 @@
 //   * The queries are rotated at the start (R from L2, in fragments) and lie in shared memory in fragment order.
 //   * The warps' sums meet in shared memory, halves in turn; the CTA's go to the workspace, paged_merge_kernel adds the parts up.
 //
-// What bounds it is instruction issue (55 % of the slots used under a profiler) and a CTA's start and end, 5 to 11 us in all: 32 requests of 5 tokens behind
-// 4000, 2-bit, 32/8 heads (71 MB of codes and norms, 11 us at the copy rate) take 115 us with the merge, 4-bit 139; of 1 to 5 tokens behind 2000 to 4000 88 us,
+// What bounds it is instruction issue (54 % of the slots used under a profiler) and a CTA's start and end, 5 to 11 us in all: 32 requests of 5 tokens behind
+// 4000, 2-bit, 32/8 heads (71 MB of codes and norms, 11 us at the copy rate) take 117 us with the merge, 4-bit 145; of 1 to 5 tokens behind 2000 to 4000 88 us,
 // 131 us on the tcgen05 kernel.
 #pragma once
 
@@ -22,6 +22,7 @@
 namespace tq {
 
 constexpr int ROWS_MOST = 32;
+constexpr int ROWS_SORTED = 128;
 template <int NCB>
 constexpr int ROWS_WARPS = NCB <= 2 ? 8 : 12;  // (two CTAs per SM, or one whose sums take the room)
 template <int NCB>
@@ -39,11 +40,11 @@ struct PagedRowsParams {
     const int* block_table;
     const int* lens;
     const int* start;
-    float* partials;  // [gridDim.z][part_tokens][H][PART_STRIDE], token: of the batch, or by_request times the request plus its own
+    float* partials;  // [parts][part_tokens][H][PART_STRIDE], token: of the batch, or by_request times the request plus its own
     int part_tokens, by_request;
     int* status;
     int table_stride, page_shift, num_pages, most_tokens;
-    int T, H, Hkv, grp, q_stride;
+    int T, G, H, Hkv, grp, q_stride, parts;
     int behind;       // see the kernel
     int row_blocks;   // CTAs per request, KV head and part: ROWS_MOST / (8 NCB), rounded up
 };
@@ -79,9 +80,50 @@ __global__ void __launch_bounds__(ROWS_THREADS<NCB>, NCB <= 2 ? 2 : 1) paged_row
     if (!p.behind) pdl_wait();
     pdl_launch_dependents();
     auto leave = [&]() { if (p.behind) pdl_wait(); };
-    const int kvh = (int)blockIdx.x % p.Hkv, rest = (int)blockIdx.x / p.Hkv, g = rest / p.row_blocks, r0 = 8 * NCB * (rest - g * p.row_blocks);
-    const int s0 = max(p.start[g], 0), n = min(p.start[g + 1], p.T) - s0, all_rows = n * p.grp;
-    const int L = min(max(p.lens[g], 0), p.most_tokens), pos0 = L - n;
+    int rest = (int)blockIdx.x / p.Hkv;
+    const int kvh = (int)blockIdx.x - rest * p.Hkv, by_blocks = rest / p.row_blocks, r0 = 8 * NCB * (rest - by_blocks * p.row_blocks);
+    int g = by_blocks / p.parts;
+    const int part = by_blocks - g * p.parts;
+    // The longest contexts first, so that the last CTAs to run are short ones: the request whose length is the g-th.  (2-bit 32/8 heads 32 x 5 behind 100 to 4000
+    // 91 -> 70 us, 4-bit behind 1000 to 8000 185 -> 145, 16/8 48 x 1 behind 100 to 4000 74 -> 59; equal contexts cost 1 to 4 % more.  More requests than this have enough turns of CTAs to even out.)
+    auto request = [&](int i) {  // first query, queries, tokens
+        const int s = max(p.start[i], 0);
+        return make_int4(s, min(p.start[i + 1], p.T) - s, min(max(p.lens[i], 0), p.most_tokens), 0);
+    };
+    int4 mine = make_int4(0, 0, 0, 0);
+    if (p.G > 1 && p.G <= ROWS_SORTED) {
+        // (where the queries' fragments lie later, behind another barrier)
+        int* const lens_s = reinterpret_cast<int*>(gb + RowsSmem<NCB>::FRAG);
+        volatile int4* const pick = reinterpret_cast<volatile int4*>(gb + RowsSmem<NCB>::FRAG) + ROWS_SORTED / 4;
+        if (tid < p.G) mine = request(tid);
+        const int key = tid >= p.G ? -2 : mine.y > 0 && mine.y * p.grp <= ROWS_MOST ? mine.z : -1;
+        if (tid < ROWS_SORTED) lens_s[tid] = key;
+        if (tid == 0) pick->y = 0;
+        if (__syncthreads_or(key >= 0 && mine.y * p.grp > r0) && tid < p.G) {  // (some request has that many rows)
+            int rank = 0;
+#pragma unroll 4
+            for (int j = 0; j < p.G; j += 4) {
+                const int4 l = *reinterpret_cast<const int4*>(lens_s + j);
+                rank += (l.x > key || (l.x == key && j < tid)) + (l.y > key || (l.y == key && j + 1 < tid)) + (l.z > key || (l.z == key && j + 2 < tid)) +
+                        (l.w > key || (l.w == key && j + 3 < tid));
+            }
+            if (rank == g) {
+                pick->x = mine.x;
+                pick->y = mine.y;
+                pick->z = mine.z;
+                pick->w = tid;
+            }
+        }
+        __syncthreads();
+        mine.x = pick->x;
+        mine.y = pick->y;
+        mine.z = pick->z;
+        g = pick->w;
+    } else {
+        mine = request(g);
+    }
+    const int s0 = mine.x, n = mine.y, all_rows = n * p.grp;
+    const int L = mine.z, pos0 = L - n;
     const int rows = min(8 * NCB, all_rows - r0);                     // this CTA's: r0 .., row = token * grp + head
     if (n <= 0 || all_rows > ROWS_MOST || rows <= 0) {
         leave();
@@ -103,7 +145,7 @@ __global__ void __launch_bounds__(ROWS_THREADS<NCB>, NCB <= 2 ? 2 : 1) paged_row
     const int first_last = pos0 + r0 / p.grp;                         // last token that the first row attends to
     const int end = max(pos0 + (r0 + rows - 1) / p.grp + 1, 0);       // tokens that count for any
     const int blocks = (end + 15) / 16;                               // of 16 tokens
-    const int b_lo = (int)((long long)blocks * blockIdx.z / gridDim.z), b_hi = (int)((long long)blocks * (blockIdx.z + 1) / gridDim.z);
+    const int b_lo = (int)((long long)blocks * part / p.parts), b_hi = (int)((long long)blocks * (part + 1) / p.parts);
     auto row_token = [&](int r) { return (r0 + r) / p.grp; };
 
     // ---- a warp's tokens: 16 at a time, in turn; the first ones are requested before all else ----
@@ -405,7 +447,7 @@ __global__ void __launch_bounds__(ROWS_THREADS<NCB>, NCB <= 2 ? 2 : 1) paged_row
             const int r = 8 * nb + 2 * t4 + e;
             if (r >= rows) continue;
             const int tok = row_token(r);
-            float* const dst = p.partials + (((size_t)blockIdx.z * p.part_tokens + (p.by_request ? g * p.by_request : s0) + tok) * p.H + (size_t)(kvh * p.grp + r0 + r - tok * p.grp)) * PART_STRIDE;
+            float* const dst = p.partials + (((size_t)part * p.part_tokens + (p.by_request ? g * p.by_request : s0) + tok) * p.H + (size_t)(kvh * p.grp + r0 + r - tok * p.grp)) * PART_STRIDE;
             constexpr float k = 1.0f / PPF_CENT<BITS>;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
