@@ -88,3 +88,16 @@ def test_workspace_sizes():
     f = tq.lib().tq_paged_workspace_bytes
     assert f(1, 0, 16) == 0 and f(-1, 1, 16) == 0 and f(1, 1, 0) == 0
     assert 0 < f(4, 4, 16) < f(64, 64, 16) < f(64, 64, 32)
+
+
+# (nothing is launched: what is refused is the overlap, before the device is asked for anything)
+@pytest.mark.parametrize("out, q, qs, os", [(0, 0, 2048, 2048), (2048, 0, 2048, 2048), (0, 2048 * 2, 2048, 2048), (2040, 0, 4096, 4096), (4096 * 2 - 8, 0, 4096, 4096), (64, 0, 2048, 4096)])
+@pytest.mark.parametrize("call", [attention, prefill])
+def test_results_over_queries_are_refused(call, out, q, qs, os):
+    at = lambda halves: C.c_void_p((1 << 20) + 2 * halves)  # noqa: E731
+    assert call(out=at(out), q=at(q), qs=qs, os=os) == -1
+
+
+def test_results_over_results_are_refused():
+    for k, v, stride in ((0, 0, 1024), (0, 1024, 1024), (0, 512, 2048), (1536, 0, 2048)):
+        assert rows("tq_paged_read", k=C.c_void_p((1 << 20) + 2 * k), v=C.c_void_p((1 << 20) + 2 * v), stride=stride) == -1

@@ -1,6 +1,8 @@
 // extern "C" calls over paged packed caches (declared in include/triebwerk_b200.h): a translation unit of its own, so that it compiles
 // beside tq_capi.cu.
 
+#include <atomic>
+
 #include "tq_host.cuh"
 #include "tq_paged.cuh"
 #include "tq_paged_prefill.cuh"
@@ -18,18 +20,15 @@ static inline bool use_pdl() {
 // The status word of all paged calls on a device: a wait that gave up, a shared-memory layout refused.
 static __device__ int g_paged_status;
 static int paged_status_word(int** out) {
-    static std::mutex mu;
-    static std::map<int, int*> known;
+    constexpr int KNOWN = 64;
+    static std::atomic<int*> known[KNOWN];
     int dev = 0;
     TQ_CUDA(cudaGetDevice(&dev));
-    std::lock_guard<std::mutex> lock(mu);
-    int*& p = known[dev];
-    if (!p) {
-        void* a = nullptr;
-        TQ_CUDA(cudaGetSymbolAddress(&a, g_paged_status));
-        p = (int*)a;
-    }
-    *out = p;
+    if (dev < KNOWN && (*out = known[dev].load(std::memory_order_acquire))) return TQ_OK;
+    void* a = nullptr;
+    TQ_CUDA(cudaGetSymbolAddress(&a, g_paged_status));
+    *out = (int*)a;
+    if (dev < KNOWN) known[dev].store(*out, std::memory_order_release);
     return TQ_OK;
 }
 
@@ -50,6 +49,15 @@ static bool aligned(std::initializer_list<const void*> p, unsigned to) {
     uintptr_t all = 0;
     for (const void* a : p) all |= (uintptr_t)a;
     return (all & (to - 1u)) == 0;
+}
+// Do two arrays of `rows` rows of `width` halves, a_stride and b_stride apart, share memory?  (Columns of one wider array need not.)
+static bool overlap(const void* a_, long long a_stride, const void* b_, long long b_stride, long long rows, long long width) {
+    if (rows <= 0) return false;
+    const long long a = (long long)((uintptr_t)a_ / 2), b = (long long)((uintptr_t)b_ / 2);
+    if (a + (rows - 1) * a_stride + width <= b || b + (rows - 1) * b_stride + width <= a) return false;
+    if (a_stride != b_stride) return true;
+    const long long d = ((b - a) % a_stride + a_stride) % a_stride;
+    return d < width || d > a_stride - width;
 }
 
 extern "C" {
@@ -138,6 +146,7 @@ int tq_paged_read(void* k_out, void* v_out, const uint8_t* ck_q, const void* k_n
     if (r != TQ_OK) return r;
     if (!ck_q || !k_norms || !cv_q || !v_norms || !rotation || (T > 0 && (!k_out || !v_out || !slots))) return TQ_ERR_ARG;
     if (!aligned({ck_q, cv_q, rotation, k_out, v_out}, 16)) return TQ_ERR_ARG;
+    if (overlap(k_out, kv_stride, v_out, kv_stride, T, (long long)num_kv_heads * HEAD_DIM)) return TQ_ERR_ARG;
     if (T == 0) return TQ_OK;
     PagedReadParams p{};
     p.ck = ck_q; p.kn = (const __half*)k_norms; p.cv = cv_q; p.vn = (const __half*)v_norms; p.rotation = (const __half*)rotation;
@@ -232,6 +241,7 @@ int tq_paged_decode_attention(void* out, const void* q, const uint8_t* ck_q, con
     if (!workspace || workspace_bytes < tq_paged_workspace_bytes(G, G, num_heads) || !aligned({workspace}, 256)) return TQ_ERR_WORKSPACE;
     const int H = num_heads, Hkv = num_kv_heads, most = table_width * page_size, head_blocks = (H / Hkv + CD_HEADS - 1) / CD_HEADS;
     if (G > 65535 || (long long)Hkv * head_blocks > 65535) return TQ_ERR_UNSUPPORTED;
+    if (overlap(q, q_stride, out, out_stride, G, (long long)H * HEAD_DIM)) return TQ_ERR_ARG;
     int* status = nullptr;
     r = paged_status_word(&status);
     if (r != TQ_OK) return r;
@@ -315,6 +325,7 @@ int tq_paged_prefill_attention(void* out, const void* q, const uint8_t* ck_q, co
     if (!workspace || workspace_bytes < tq_paged_workspace_bytes(T, G, H) || !aligned({workspace}, 256)) return TQ_ERR_WORKSPACE;
     if (T == 0) return TQ_OK;
     if ((long long)T * H >= (1ll << 31) || G > 65535) return TQ_ERR_UNSUPPORTED;
+    if (overlap(q, q_stride, out, out_stride, T, (long long)H * HEAD_DIM)) return TQ_ERR_ARG;
     int* status = nullptr;
     r = paged_status_word(&status);
     if (r != TQ_OK) return r;
