@@ -41,7 +41,9 @@ struct PagePlanParams {
 };
 
 constexpr int PLAN_THREADS = 1024;
-constexpr int PLAN_ONE_LAUNCH = 4096;  // slots that the first launch writes itself
+// Slots that the first launch writes itself.  (us, one / two launches: 64 x 16 new tokens 4.7 / 6.1, 256 x 4 5.2 / 6.8, 64 x 32 5.5 / 6.2, 64 x 64 7.0 / 6.3,
+// 256 x 16 7.7 / 7.1, 64 x 128 9.7 / 6.3, 64 x 1024 51 / 6.6.)
+constexpr int PLAN_ONE_LAUNCH = 2048;
 
 // Token t of the slot map is request a's, start[a] <= t < start[a + 1].
 constexpr int SLOTS_THREADS = 256, SLOTS_SHARED = 8192;  // starts that are searched in shared memory
