@@ -127,3 +127,21 @@ def test_prefill_many_query_heads(H, Hkv, bits):
     check_prefill([4000, 3], [3, 2], H, Hkv, bits, 64, 4)
     check_prefill([700, 200, 333, 12], [300, 200, 31, 12], H, Hkv, bits, 128, 5)  # two blocks a CTA
     check_prefill([900 + 17 * g for g in range(40)], [1] * 40, H, Hkv, bits, 32, 6, tail=0)
+
+
+@pytest.mark.parametrize("G, form", [(4, "streaming"), (5, "cluster"), (40, "cluster")])
+def test_decode_more_tiles_than_can_be_numbered(G, form):
+    # Tables with room for 2^26 - 2048 tiles a request, of shared pages: 5 requests could pass 2^28 and 33 of them 2^31, which the streaming form's tile
+    # numbers do not hold.  The cluster form, which has none, writes nothing to the workspace.
+    rng = np.random.default_rng(G)
+    page, width, H, Hkv, bits = 65536, 32767, 16, 8, 2
+    (ck, kn), (cv, vn) = (pu.random_cache(rng, page, Hkv, bits) for _ in range(2))
+    lens = rng.integers(0, 3000, G).tolist()
+    table = torch.zeros(G, width, dtype=torch.int32, device="cuda")
+    q = torch.from_numpy(rng.standard_normal((G, H * 128)).astype(np.float16)).cuda()
+    out, R, ws = torch.empty_like(q), pu.rotation(5).cuda(), ops.paged_workspace(G, G, H)
+    ws.fill_(77)
+    ops.paged_decode_attention(out, q, ck, cv, kn, vn, R, table, i32(lens), page, H, Hkv, bits, ws)
+    torch.cuda.synchronize()
+    assert (form == "cluster") == bool((ws == 77).all())
+    pu.assert_attention(out, pu.attention(q, ck, cv, kn, vn, R, table, lens, list(range(G + 1)), page, H, Hkv, bits))

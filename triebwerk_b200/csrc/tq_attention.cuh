@@ -566,7 +566,7 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
         ts = p.tile_start;
     }
     __syncthreads();
-    const int N = ts[G];  // (the host refuses caches of 2^31 rows or more)
+    const int N = ts[G];  // (below 2^26: the host refuses caches of 2^31 rows or more; PAGED, where requests may share pages: below 2^28, the host's choice of form)
 
     // ---- work slice of this worker ----
     // At most min(workers, N) workers take part, so that every participant owns at least one tile: the ticket
@@ -580,7 +580,7 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
     }
     if (wid >= W && !copier) return;  // uniform for the worker; no CTA-wide barrier follows
     // Worker w takes the tiles [w * N / W, (w + 1) * N / W).
-    const int n_each = N / W, n_over = N - n_each * W;  // (N < 2^26, W <= 1024)
+    const int n_each = N / W, n_over = N - n_each * W;  // (W <= 1024)
     const int lo = wid * n_each + wid * n_over / W, hi = (wid + 1) * n_each + (wid + 1) * n_over / W;
     int g;  // first sequence of the slice: largest g with tile_start[g] <= lo
     if (!PUBLISH && p.worker_g && !TQ_DBG_FACTOR) {
@@ -597,7 +597,7 @@ decode_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
     const bool idle = copier && (lane > 0 || wid >= W);  // nothing to copy (it returns further down)
     if (idle) g = 0;
     // ---- load cursor over the flat tile list (warp-uniform, advanced in step by every warp of the worker) ----
-    // Tile counts and row numbers fit 32 bits (the host refuses caches of 2^31 rows or more).
+    // Tile counts and row numbers fit 32 bits (the host's doing, see N).
     const int lo_i = idle ? 0 : lo, hi_i = idle ? 0 : hi;
     int cl_tile = lo_i;                         // next tile to load into shared memory
     int cl_g = g;

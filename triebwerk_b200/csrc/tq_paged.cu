@@ -246,7 +246,10 @@ int tq_paged_decode_attention(void* out, const void* q, const uint8_t* ck_q, con
     r = paged_status_word(&status);
     if (r != TQ_OK) return r;
     const long long rows = (long long)num_pages * page_size;
-    const bool streams = fast_shape(H, Hkv, true) && G <= FUSED_MAX_G;
+    // The streaming form numbers the tiles of all requests with 32 bits.  Rows of the table may name the same pages, so the cache's size does not bound them:
+    // below 2^28 the sums stay clear of overflow, and of the distance that stands for no prefetch.
+    constexpr int MOST_TILES = 1 << 28;
+    const bool streams = fast_shape(H, Hkv, true) && G <= FUSED_MAX_G && (long long)G * ((most + TILE_TOKENS - 1) / TILE_TOKENS) < MOST_TILES;
     if (!streams || cluster_layer_faster(bits, G, Hkv, H / Hkv, (long long)G * most, most, LayerCaller::Paged)) {
         ClusterDecodeParams p{};
         p.ck = ck_q; p.cv = cv_q; p.kn = (const __half*)k_norms; p.vn = (const __half*)v_norms; p.q = (const __half*)q; p.rotation = (const __half*)rotation;
@@ -271,7 +274,7 @@ int tq_paged_decode_attention(void* out, const void* q, const uint8_t* ck_q, con
     p.ck = ck_q; p.cv = cv_q; p.kn = (const __half*)k_norms; p.vn = (const __half*)v_norms;
     p.q_rot16 = lp.q_rot16; p.q_rot32 = lp.q_rot32; p.rotation_t = fw.rot_t; p.out = (__half*)out;
     p.positions = seq_lens; p.partials = fw.w.partials; p.status = status; p.total_rows = rows;
-    p.G = G; p.H = H; p.Hkv = Hkv; p.q_dim = out_stride; p.n_layers = 1; p.l2_ahead = 1 << 28;
+    p.G = G; p.H = H; p.Hkv = Hkv; p.q_dim = out_stride; p.n_layers = 1; p.l2_ahead = MOST_TILES;
     p.block_table = block_table; p.table_stride = table_stride; p.page_shift = log2_of(page_size); p.num_pages = num_pages; p.most_tokens = most;
     const int ctas = attention_ctas(G, most);
     if (Hkv == 8) r = bits == 4 ? launch_attention_t<4, 8, 1, true>(tmK, tmV, p, ctas, cs(s), use_pdl()) : launch_attention_t<2, 8, 1, true>(tmK, tmV, p, ctas, cs(s), use_pdl());
