@@ -145,3 +145,23 @@ def test_decode_more_tiles_than_can_be_numbered(G, form):
     torch.cuda.synchronize()
     assert (form == "cluster") == bool((ws == 77).all())
     pu.assert_attention(out, pu.attention(q, ck, cv, kn, vn, R, table, lens, list(range(G + 1)), page, H, Hkv, bits))
+
+
+@pytest.mark.parametrize("new", [1, 7, 60])
+def test_results_between_the_rows_of_queries(new):
+    # one array of four columns: queries in the first (every row), results in the second and fourth in turn, rows half as far apart
+    rng = np.random.default_rng(new)
+    G, H, Hkv, page = 5, 16, 8, 32
+    W, T, lens, start = H * 128, G * new, [100 + 30 * g for g in range(G)], [new * g for g in range(G + 1)]
+    table, q, _, ck, cv, kn, vn, R, _ = attention_inputs(rng, lens, H, Hkv, 4, page, T=T)
+    whole = torch.full((T, 4 * W), 7.0, dtype=torch.float16, device="cuda")
+    mine, out = whole[:, :W], whole.view(2 * T, 2 * W)[:T, W:]
+    mine.copy_(q)
+    apart = torch.empty(T, W, dtype=torch.float16, device="cuda")
+    ws = ops.paged_workspace(T, G, H)
+    for a, o in ((q, apart), (mine, out)):
+        ops.paged_prefill_attention(o, a, ck, cv, kn, vn, R, table, i32(lens), i32(start), page, H, Hkv, 4, ws)
+        if new == 1:
+            ops.paged_decode_attention(o, a, ck, cv, kn, vn, R, table, i32(lens), page, H, Hkv, 4, ws)
+    torch.cuda.synchronize()
+    assert torch.equal(out, apart) and torch.equal(mine, q) and (whole[:, 2 * W:3 * W] == 7).all()

@@ -50,15 +50,32 @@ static bool aligned(std::initializer_list<const void*> p, unsigned to) {
     for (const void* a : p) all |= (uintptr_t)a;
     return (all & (to - 1u)) == 0;
 }
-// Do two arrays of `rows` rows of `width` halves, a_stride and b_stride apart, share memory?  (Columns of one wider array need not.)
-static bool overlap(const void* a_, long long a_stride, const void* b_, long long b_stride, long long rows, long long width) {
-    if (rows <= 0) return false;
-    const long long a = (long long)((uintptr_t)a_ / 2), b = (long long)((uintptr_t)b_ / 2);
-    if (a + (rows - 1) * a_stride + width <= b || b + (rows - 1) * b_stride + width <= a) return false;
-    if (a_stride != b_stride) return true;
-    const long long d = ((b - a) % a_stride + a_stride) % a_stride;
-    return d < width || d > a_stride - width;
+// An array: `rows` rows of `width` bytes, `stride` apart (one row: any).
+struct Span {
+    const void* at;
+    long long width, stride, rows;
+};
+// Do two arrays share memory?  Rows of either may lie between the other's (columns of one wider array).
+static bool overlap(const Span& a, const Span& b) {
+    if (a.rows <= 0 || a.width <= 0 || b.rows <= 0 || b.width <= 0) return false;
+    const long long d = (long long)((uintptr_t)b.at - (uintptr_t)a.at);  // row j of b begins at d + j * b.stride, row i of a at i * a.stride
+    const long long a_last = (a.rows - 1) * a.stride, b_last = d + (b.rows - 1) * b.stride;
+    if (a_last + a.width <= d || b_last + b.width <= 0) return false;
+    if (a.rows > 1 && b.rows > 1 && a.stride == b.stride) {  // (that of one wider array: no loop)
+        const long long r = (d % a.stride + a.stride) % a.stride;
+        return r < a.width || r > a.stride - b.width;
+    }
+    // the first row of either that ends behind the other's row, in turn
+    auto past = [](long long begin, const Span& s, long long first) { return begin + s.width <= first ? (first - begin - s.width) / s.stride + 1 : 0; };
+    for (long long i = 0, j = 0;;) {
+        const long long skip_a = past(i * a.stride, a, d + j * b.stride);
+        if ((i += skip_a) >= a.rows) return false;
+        const long long skip_b = past(d + j * b.stride, b, i * a.stride);
+        if ((j += skip_b) >= b.rows) return false;
+        if (skip_b == 0) return true;  // (row i of a ends behind row j's begin, row j of b behind row i's)
+    }
 }
+static Span half_rows(const void* at, long long rows, long long width, long long stride) { return {at, 2 * width, 2 * stride, rows}; }
 
 extern "C" {
 
@@ -146,7 +163,7 @@ int tq_paged_read(void* k_out, void* v_out, const uint8_t* ck_q, const void* k_n
     if (r != TQ_OK) return r;
     if (!ck_q || !k_norms || !cv_q || !v_norms || !rotation || (T > 0 && (!k_out || !v_out || !slots))) return TQ_ERR_ARG;
     if (!aligned({ck_q, cv_q, rotation, k_out, v_out}, 16)) return TQ_ERR_ARG;
-    if (overlap(k_out, kv_stride, v_out, kv_stride, T, (long long)num_kv_heads * HEAD_DIM)) return TQ_ERR_ARG;
+    if (overlap(half_rows(k_out, T, num_kv_heads * HEAD_DIM, kv_stride), half_rows(v_out, T, num_kv_heads * HEAD_DIM, kv_stride))) return TQ_ERR_ARG;
     if (T == 0) return TQ_OK;
     PagedReadParams p{};
     p.ck = ck_q; p.kn = (const __half*)k_norms; p.cv = cv_q; p.vn = (const __half*)v_norms; p.rotation = (const __half*)rotation;
@@ -241,7 +258,7 @@ int tq_paged_decode_attention(void* out, const void* q, const uint8_t* ck_q, con
     if (!workspace || workspace_bytes < tq_paged_workspace_bytes(G, G, num_heads) || !aligned({workspace}, 256)) return TQ_ERR_WORKSPACE;
     const int H = num_heads, Hkv = num_kv_heads, most = table_width * page_size, head_blocks = (H / Hkv + CD_HEADS - 1) / CD_HEADS;
     if (G > 65535 || (long long)Hkv * head_blocks > 65535) return TQ_ERR_UNSUPPORTED;
-    if (overlap(q, q_stride, out, out_stride, G, (long long)H * HEAD_DIM)) return TQ_ERR_ARG;
+    if (overlap(half_rows(q, G, H * HEAD_DIM, q_stride), half_rows(out, G, H * HEAD_DIM, out_stride))) return TQ_ERR_ARG;
     int* status = nullptr;
     r = paged_status_word(&status);
     if (r != TQ_OK) return r;
@@ -328,7 +345,7 @@ int tq_paged_prefill_attention(void* out, const void* q, const uint8_t* ck_q, co
     if (!workspace || workspace_bytes < tq_paged_workspace_bytes(T, G, H) || !aligned({workspace}, 256)) return TQ_ERR_WORKSPACE;
     if (T == 0) return TQ_OK;
     if ((long long)T * H >= (1ll << 31) || G > 65535) return TQ_ERR_UNSUPPORTED;
-    if (overlap(q, q_stride, out, out_stride, T, (long long)H * HEAD_DIM)) return TQ_ERR_ARG;
+    if (overlap(half_rows(q, T, H * HEAD_DIM, q_stride), half_rows(out, T, H * HEAD_DIM, out_stride))) return TQ_ERR_ARG;
     int* status = nullptr;
     r = paged_status_word(&status);
     if (r != TQ_OK) return r;
