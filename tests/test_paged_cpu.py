@@ -101,3 +101,60 @@ def test_results_over_queries_are_refused(call, out, q, qs, os):
 def test_results_over_results_are_refused():
     for k, v, stride in ((0, 0, 1024), (0, 1024, 1024), (0, 512, 2048), (1536, 0, 2048)):
         assert rows("tq_paged_read", k=C.c_void_p((1 << 20) + 2 * k), v=C.c_void_p((1 << 20) + 2 * v), stride=stride) == -1
+
+
+# Arrays in their order of address, none touching the next: 1 MiB apart, each smaller than that.
+def apart(names):
+    return {n: C.c_void_p((i + 1) << 20) for i, n in enumerate(names)}
+
+
+def shared(a, name, other, size):
+    """`name` on the last bytes of `other`, which has `size` (where its own alignment lets it begin)."""
+    to = 256 if name == "ws" else 16
+    return dict(a, **{name: C.c_void_p(a[other].value + (size - 1) // to * to)})
+
+
+PLAN = dict(table=4 * 32, free=64, count=4, count_out=4, context=16, new=16, finished=4, lens=16, start=20, slots=32, positions=16)
+PLAN_READ = ("count", "context", "new", "finished")
+
+
+@pytest.mark.parametrize("name", PLAN)
+@pytest.mark.parametrize("other", PLAN)
+def test_plan_refuses_arrays_that_share_memory(name, other):
+    # (count and count_out, context and lens may be the same array: not in part, as here, but where an array has 16 bytes or fewer)
+    if name == other or (name in PLAN_READ and other in PLAN_READ) or {name, other} in ({"count", "count_out"}, {"context", "lens"}):
+        return
+    assert plan(**shared(apart(PLAN), name, other, PLAN[other])) == -1
+
+
+def test_plan_refuses_lengths_that_are_the_context_in_part():
+    a = apart(PLAN)
+    a["lens"] = C.c_void_p(a["context"].value + 4)
+    assert plan(**a) == -1
+
+
+ROWS = dict(ck=64 * 512, kn=64 * 16, cv=64 * 512, vn=64 * 16, k=4096, v=4096, R=32768, slots=16)
+
+
+@pytest.mark.parametrize("call, written", [("tq_paged_append", ("ck", "kn", "cv", "vn")), ("tq_paged_read", ("k", "v"))])
+@pytest.mark.parametrize("name", ROWS)
+@pytest.mark.parametrize("other", ROWS)
+def test_rows_refuse_arrays_that_share_memory(call, written, name, other):
+    if name != other and (name in written or other in written):
+        assert rows(call, **shared(apart(ROWS), name, other, ROWS[other])) == -1
+
+
+ATTENTION = dict(out=4 * 4096, q=4 * 4096, ck=512 * 512, cv=512 * 512, kn=512 * 16, vn=512 * 16, R=32768, table=4 * 32, lens=16, ws=4 * 16 * 132 * 4)
+
+
+@pytest.mark.parametrize("call, arrays", [(attention, ATTENTION), (prefill, dict(ATTENTION, out=7 * 4096, q=7 * 4096, start=20))])
+@pytest.mark.parametrize("written", ["out", "ws"])
+@pytest.mark.parametrize("other", [*ATTENTION, "start"])
+def test_attentions_refuse_arrays_that_share_memory(call, arrays, written, other):
+    if other == written or other not in arrays:
+        return
+    a = apart(arrays)
+    a["ws"] = C.c_void_p(64 << 20)
+    assert call(**shared(a, other, written, arrays[written])) == -1
+    if written == "out":
+        assert call(**shared(a, written, other, arrays[other])) == -1

@@ -76,6 +76,18 @@ static bool overlap(const Span& a, const Span& b) {
     }
 }
 static Span half_rows(const void* at, long long rows, long long width, long long stride) { return {at, 2 * width, 2 * stride, rows}; }
+static Span block(const void* at, long long bytes) { return {at, bytes, bytes, at ? 1 : 0}; }
+// Does anything that a call writes share memory with something else that it writes, or with something that it reads?
+static bool clash(std::initializer_list<Span> written, std::initializer_list<Span> read) {
+    for (const Span* w = written.begin(); w != written.end(); ++w) {
+        for (const Span* o = written.begin(); o != w; ++o)
+            if (overlap(*w, *o)) return true;
+        for (const Span& r : read)
+            if (overlap(*w, r)) return true;
+    }
+    return false;
+}
+constexpr long long ROTATION_BYTES = 2ll * HEAD_DIM * HEAD_DIM;
 
 extern "C" {
 
@@ -91,6 +103,11 @@ int tq_page_plan(int* block_table, int table_stride, int table_width, int* free_
     int r = check_pages(table_stride, table_width, num_pages, page_size);
     if (r != TQ_OK) return r;
     if (!block_table || !free_pages || !free_count || !free_count_out || !context_lens || !new_tokens || !seq_lens || !query_start || G <= 0 || T < 0 || (T > 0 && !slots))
+        return TQ_ERR_ARG;
+    if (clash({Span{block_table, 4ll * table_width, 4ll * table_stride, G}, block(free_pages, 4ll * num_pages), block(free_count_out, 4), block(seq_lens, 4ll * G),
+               block(query_start, 4ll * G + 4), block(slots, 8ll * T), block(positions, 4ll * T)},
+              {block(free_count == free_count_out ? nullptr : free_count, 4), block(context_lens == seq_lens ? nullptr : context_lens, 4ll * G), block(new_tokens, 4ll * G),
+               block(finished, G)}))
         return TQ_ERR_ARG;
     PagePlanParams p{};
     p.table = block_table; p.free_pages = free_pages; p.free_count = free_count; p.free_count_out = free_count_out;
@@ -117,6 +134,10 @@ int tq_paged_append(uint8_t* ck_q, void* k_norms, uint8_t* cv_q, void* v_norms, 
     if (!ck_q || !k_norms || !cv_q || !v_norms || !rotation || (T > 0 && (!k_buf || !v_buf || !slots))) return TQ_ERR_ARG;
     if (!aligned({ck_q, cv_q, k_buf, v_buf, rotation}, 16)) return TQ_ERR_ARG;
     if (T == 0) return TQ_OK;
+    const long long codes = total_rows * num_kv_heads * (HEAD_DIM * bits / 8), norms = 2 * total_rows * num_kv_heads;
+    if (clash({block(ck_q, codes), block(cv_q, codes), block(k_norms, norms), block(v_norms, norms)},
+              {half_rows(k_buf, T, num_kv_heads * HEAD_DIM, kv_stride), half_rows(v_buf, T, num_kv_heads * HEAD_DIM, kv_stride), block(rotation, ROTATION_BYTES), block(slots, 8ll * T)}))
+        return TQ_ERR_ARG;
     int* status = nullptr;
     r = paged_status_word(&status);
     if (r != TQ_OK) return r;
@@ -163,8 +184,11 @@ int tq_paged_read(void* k_out, void* v_out, const uint8_t* ck_q, const void* k_n
     if (r != TQ_OK) return r;
     if (!ck_q || !k_norms || !cv_q || !v_norms || !rotation || (T > 0 && (!k_out || !v_out || !slots))) return TQ_ERR_ARG;
     if (!aligned({ck_q, cv_q, rotation, k_out, v_out}, 16)) return TQ_ERR_ARG;
-    if (overlap(half_rows(k_out, T, num_kv_heads * HEAD_DIM, kv_stride), half_rows(v_out, T, num_kv_heads * HEAD_DIM, kv_stride))) return TQ_ERR_ARG;
     if (T == 0) return TQ_OK;
+    const long long codes = total_rows * num_kv_heads * (HEAD_DIM * bits / 8), norms = 2 * total_rows * num_kv_heads;
+    if (clash({half_rows(k_out, T, num_kv_heads * HEAD_DIM, kv_stride), half_rows(v_out, T, num_kv_heads * HEAD_DIM, kv_stride)},
+              {block(ck_q, codes), block(cv_q, codes), block(k_norms, norms), block(v_norms, norms), block(rotation, ROTATION_BYTES), block(slots, 8ll * T)}))
+        return TQ_ERR_ARG;
     PagedReadParams p{};
     p.ck = ck_q; p.kn = (const __half*)k_norms; p.cv = cv_q; p.vn = (const __half*)v_norms; p.rotation = (const __half*)rotation;
     p.slots = slots; p.k_out = (__half*)k_out; p.v_out = (__half*)v_out; p.total_rows = total_rows; p.stride = kv_stride; p.T = T; p.Hkv = num_kv_heads;
@@ -247,6 +271,15 @@ static int check_attention(const void* out, const void* q, const uint8_t* ck, co
     if (!aligned({out, q, ck, cv, kn, vn, rotation}, 16)) return TQ_ERR_ARG;
     return TQ_OK;
 }
+// ... and what they write: results and workspace (T query rows; `start` of prefill alone).
+static bool attention_clash(const void* out, const void* q, const uint8_t* ck, const uint8_t* cv, const void* kn, const void* vn, const void* rotation, const int* table,
+                            int table_stride, int table_width, const int* lens, const int* start, long long rows, int T, int G, int H, int Hkv, int q_stride, int out_stride,
+                            int bits, const void* workspace) {
+    const long long codes = rows * Hkv * (HEAD_DIM * bits / 8), norms = 2 * rows * Hkv;
+    return clash({half_rows(out, T, H * HEAD_DIM, out_stride), block(workspace, (long long)tq_paged_workspace_bytes(T, G, H))},
+                 {half_rows(q, T, H * HEAD_DIM, q_stride), block(ck, codes), block(cv, codes), block(kn, norms), block(vn, norms), block(rotation, ROTATION_BYTES),
+                  Span{table, 4ll * table_width, 4ll * table_stride, G}, block(lens, 4ll * G), block(start, 4ll * G + 4)});
+}
 
 int tq_paged_decode_attention(void* out, const void* q, const uint8_t* ck_q, const uint8_t* cv_q, const void* k_norms, const void* v_norms,
                               const void* rotation, const int* block_table, int table_stride, int table_width, const int* seq_lens, int num_pages,
@@ -258,11 +291,13 @@ int tq_paged_decode_attention(void* out, const void* q, const uint8_t* ck_q, con
     if (!workspace || workspace_bytes < tq_paged_workspace_bytes(G, G, num_heads) || !aligned({workspace}, 256)) return TQ_ERR_WORKSPACE;
     const int H = num_heads, Hkv = num_kv_heads, most = table_width * page_size, head_blocks = (H / Hkv + CD_HEADS - 1) / CD_HEADS;
     if (G > 65535 || (long long)Hkv * head_blocks > 65535) return TQ_ERR_UNSUPPORTED;
-    if (overlap(half_rows(q, G, H * HEAD_DIM, q_stride), half_rows(out, G, H * HEAD_DIM, out_stride))) return TQ_ERR_ARG;
+    const long long rows = (long long)num_pages * page_size;
+    if (attention_clash(out, q, ck_q, cv_q, k_norms, v_norms, rotation, block_table, table_stride, table_width, seq_lens, nullptr, rows, G, G, H, Hkv, q_stride, out_stride, bits,
+                        workspace))
+        return TQ_ERR_ARG;
     int* status = nullptr;
     r = paged_status_word(&status);
     if (r != TQ_OK) return r;
-    const long long rows = (long long)num_pages * page_size;
     // The streaming form numbers the tiles of all requests with 32 bits.  Rows of the table may name the same pages, so the cache's size does not bound them:
     // below 2^28 the sums stay clear of overflow, and of the distance that stands for no prefetch.
     constexpr int MOST_TILES = 1 << 28;
@@ -345,7 +380,9 @@ int tq_paged_prefill_attention(void* out, const void* q, const uint8_t* ck_q, co
     if (!workspace || workspace_bytes < tq_paged_workspace_bytes(T, G, H) || !aligned({workspace}, 256)) return TQ_ERR_WORKSPACE;
     if (T == 0) return TQ_OK;
     if ((long long)T * H >= (1ll << 31) || G > 65535) return TQ_ERR_UNSUPPORTED;
-    if (overlap(half_rows(q, T, H * HEAD_DIM, q_stride), half_rows(out, T, H * HEAD_DIM, out_stride))) return TQ_ERR_ARG;
+    if (attention_clash(out, q, ck_q, cv_q, k_norms, v_norms, rotation, block_table, table_stride, table_width, seq_lens, query_start, (long long)num_pages * page_size, T, G, H,
+                        Hkv, q_stride, out_stride, bits, workspace))
+        return TQ_ERR_ARG;
     int* status = nullptr;
     r = paged_status_word(&status);
     if (r != TQ_OK) return r;
