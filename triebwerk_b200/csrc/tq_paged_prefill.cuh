@@ -186,10 +186,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     }
     const int L = min(max(p.lens[g], 0), p.most_tokens), pos0 = L - n;  // position of the request's first new token
     // tiles that the block whose first query is `first` reads
-    auto tiles_to = [&](int first) {
-        const int last = pos0 + min(first + QT, n) - 1;  // token
-        return first < n && last >= 0 ? last / PFT_KT + 1 : 0;
-    };
+    auto tiles_to = [&](int first) { return first < n ? (int)(((unsigned)max(pos0 + min(first + QT, n), 0) + (PFT_KT - 1u)) / PFT_KT) : 0; };
     const int t_lo = SPLIT ? (int)((long long)tiles_to(q0) * blockIdx.z / gridDim.z) : 0;
     const int n_all = (SPLIT ? (int)((long long)tiles_to(q0) * (blockIdx.z + 1) / gridDim.z) : tiles_to(q0)) - t_lo;
     const int n0 = MT == 2 ? n_all : (n_all + 1) / 2, n1 = MT == 2 ? tiles_to(q0 + QT) : n_all / 2;
