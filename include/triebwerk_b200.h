@@ -410,7 +410,8 @@ int tq_engine_decode_step_host(tq_engine* e, const void* q_host, const void* k_h
  * name the same page (a shared prompt), as long as nothing is appended to it; tq_page_plan's release of ended requests knows no
  * owners, so such rows are the caller's to release.  A page number outside the pool reads as the pool's last page.  Lengths are
  * those in device memory at the time the kernels run: all calls can be captured into a graph, whose replays follow new lengths.
- * kv_bits 4 and 2, head_dim 128, num_heads a multiple of num_kv_heads.  Codes, q, out, K, V, rotation: 16-byte aligned; strides are in
+ * kv_bits 4 and 2, head_dim 128, num_heads a multiple of num_kv_heads.  Codes, q, out, K, V, rotation: 16-byte aligned (norms of an attention too),
+ * all else by the size of its elements; strides are in
  * elements, multiples of 8.  What a call writes overlaps nothing else that it writes or reads, but where that is said.  Fewer than 2^31 rows, 2^30 vectors (T *
  * num_kv_heads) of a call that stores or reads, 2^31 query rows (T * num_heads); at most 65535 requests of an attention.  Calls check their
  * arguments before anything is enqueued.

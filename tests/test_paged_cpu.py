@@ -158,3 +158,25 @@ def test_attentions_refuse_arrays_that_share_memory(call, arrays, written, other
     assert call(**shared(a, other, written, arrays[written])) == -1
     if written == "out":
         assert call(**shared(a, written, other, arrays[other])) == -1
+
+
+# (an address that is no multiple of the element's size would fault on the GPU)
+@pytest.mark.parametrize("name, off", [(n, 2) for n in PLAN if n not in ("finished", "slots")] + [("slots", 4)])
+def test_plan_refuses_addresses_that_no_element_has(name, off):
+    a = apart(PLAN)
+    assert plan(**dict(a, **{name: C.c_void_p(a[name].value + off)})) == -1
+
+
+@pytest.mark.parametrize("call", ["tq_paged_append", "tq_paged_read"])
+@pytest.mark.parametrize("name, off", [("ck", 8), ("cv", 8), ("kn", 1), ("vn", 1), ("k", 8), ("v", 8), ("R", 8), ("slots", 4)])
+def test_rows_refuse_addresses_that_no_element_has(call, name, off):
+    a = apart(ROWS)
+    assert rows(call, **dict(a, **{name: C.c_void_p(a[name].value + off)})) == -1
+
+
+@pytest.mark.parametrize("call, arrays", [(attention, ATTENTION), (prefill, dict(ATTENTION, start=20))])
+@pytest.mark.parametrize("name, off", [(n, 8) for n in ("out", "q", "ck", "cv", "kn", "vn", "R")] + [("table", 2), ("lens", 2), ("start", 2)])
+def test_attentions_refuse_addresses_that_no_element_has(call, arrays, name, off):
+    if name in arrays:
+        a = dict(apart(arrays), ws=C.c_void_p(64 << 20))
+        assert call(**dict(a, **{name: C.c_void_p(a[name].value + off)})) == -1

@@ -104,6 +104,7 @@ int tq_page_plan(int* block_table, int table_stride, int table_width, int* free_
     if (r != TQ_OK) return r;
     if (!block_table || !free_pages || !free_count || !free_count_out || !context_lens || !new_tokens || !seq_lens || !query_start || G <= 0 || T < 0 || (T > 0 && !slots))
         return TQ_ERR_ARG;
+    if (!aligned({block_table, free_pages, free_count, free_count_out, context_lens, new_tokens, seq_lens, query_start, positions}, 4) || !aligned({slots}, 8)) return TQ_ERR_ARG;
     if (clash({Span{block_table, 4ll * table_width, 4ll * table_stride, G}, block(free_pages, 4ll * num_pages), block(free_count_out, 4), block(seq_lens, 4ll * G),
                block(query_start, 4ll * G + 4), block(slots, 8ll * T), block(positions, 4ll * T)},
               {block(free_count == free_count_out ? nullptr : free_count, 4), block(context_lens == seq_lens ? nullptr : context_lens, 4ll * G), block(new_tokens, 4ll * G),
@@ -132,7 +133,7 @@ int tq_paged_append(uint8_t* ck_q, void* k_norms, uint8_t* cv_q, void* v_norms, 
     int r = check_rows(T, num_kv_heads, head_dim, kv_stride, bits, total_rows);
     if (r != TQ_OK) return r;
     if (!ck_q || !k_norms || !cv_q || !v_norms || !rotation || (T > 0 && (!k_buf || !v_buf || !slots))) return TQ_ERR_ARG;
-    if (!aligned({ck_q, cv_q, k_buf, v_buf, rotation}, 16)) return TQ_ERR_ARG;
+    if (!aligned({ck_q, cv_q, k_buf, v_buf, rotation}, 16) || !aligned({k_norms, v_norms}, 2) || !aligned({slots}, 8)) return TQ_ERR_ARG;
     if (T == 0) return TQ_OK;
     const long long codes = total_rows * num_kv_heads * (HEAD_DIM * bits / 8), norms = 2 * total_rows * num_kv_heads;
     if (clash({block(ck_q, codes), block(cv_q, codes), block(k_norms, norms), block(v_norms, norms)},
@@ -183,7 +184,7 @@ int tq_paged_read(void* k_out, void* v_out, const uint8_t* ck_q, const void* k_n
     int r = check_rows(T, num_kv_heads, head_dim, kv_stride, bits, total_rows);
     if (r != TQ_OK) return r;
     if (!ck_q || !k_norms || !cv_q || !v_norms || !rotation || (T > 0 && (!k_out || !v_out || !slots))) return TQ_ERR_ARG;
-    if (!aligned({ck_q, cv_q, rotation, k_out, v_out}, 16)) return TQ_ERR_ARG;
+    if (!aligned({ck_q, cv_q, rotation, k_out, v_out}, 16) || !aligned({k_norms, v_norms}, 2) || !aligned({slots}, 8)) return TQ_ERR_ARG;
     if (T == 0) return TQ_OK;
     const long long codes = total_rows * num_kv_heads * (HEAD_DIM * bits / 8), norms = 2 * total_rows * num_kv_heads;
     if (clash({half_rows(k_out, T, num_kv_heads * HEAD_DIM, kv_stride), half_rows(v_out, T, num_kv_heads * HEAD_DIM, kv_stride)},
@@ -268,7 +269,7 @@ static int check_attention(const void* out, const void* q, const uint8_t* ck, co
     if (G <= 0 || H <= 0 || Hkv <= 0 || H % Hkv != 0 || (bits != 2 && bits != 4)) return TQ_ERR_ARG;
     if ((long long)q_stride < (long long)H * HEAD_DIM || (long long)out_stride < (long long)H * HEAD_DIM || q_stride % 8 != 0 || out_stride % 8 != 0) return TQ_ERR_ARG;
     if (!out || !q || !ck || !cv || !kn || !vn || !rotation || !table || !lens) return TQ_ERR_ARG;
-    if (!aligned({out, q, ck, cv, kn, vn, rotation}, 16)) return TQ_ERR_ARG;
+    if (!aligned({out, q, ck, cv, kn, vn, rotation}, 16) || !aligned({table, lens}, 4)) return TQ_ERR_ARG;
     return TQ_OK;
 }
 // ... and what they write: results and workspace (T query rows; `start` of prefill alone).
@@ -374,7 +375,7 @@ int tq_paged_prefill_attention(void* out, const void* q, const uint8_t* ck_q, co
     int r = check_attention(out, q, ck_q, cv_q, k_norms, v_norms, rotation, block_table, table_stride, table_width, seq_lens, num_pages, page_size, G,
                             num_heads, num_kv_heads, head_dim, q_stride, out_stride, bits);
     if (r != TQ_OK) return r;
-    if (T < 0 || !query_start) return TQ_ERR_ARG;
+    if (T < 0 || !query_start || !aligned({query_start}, 4)) return TQ_ERR_ARG;
     const int H = num_heads, Hkv = num_kv_heads, grp = H / Hkv, most = table_width * page_size;
     if (!prefill_attn_shape(H, Hkv)) return TQ_ERR_UNSUPPORTED;
     if (!workspace || workspace_bytes < tq_paged_workspace_bytes(T, G, H) || !aligned({workspace}, 256)) return TQ_ERR_WORKSPACE;
