@@ -165,3 +165,76 @@ def test_results_between_the_rows_of_queries(new):
             ops.paged_decode_attention(o, a, ck, cv, kn, vn, R, table, i32(lens), page, H, Hkv, 4, ws)
     torch.cuda.synchronize()
     assert torch.equal(out, apart) and torch.equal(mine, q) and (whole[:, 2 * W:3 * W] == 7).all()
+
+
+# ---- one long request among small ones ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("bits", [4, 2])
+@pytest.mark.parametrize("H, Hkv, small, chunk, past, at", [
+    (32, 8, 63, 64, 9000, 0), (32, 8, 63, 65, 9000, 63),   # (the second: tokens in a multiple of the requests)
+    (32, 8, 15, 200, 5000, 7), (16, 8, 31, 100, 3000, 30), (4, 1, 700, 64, 6000, 650), (14, 2, 20, 90, 2500, 3), (16, 1, 5, 40, 4000, 5), (32, 8, 1, 64, 6000, 1)])
+def test_prefill_a_chunk_beside_single_tokens(H, Hkv, small, chunk, past, at, bits):
+    rng = np.random.default_rng(small + chunk)
+    lens, new = rng.integers(0, 700, small).tolist(), [1] * small
+    lens.insert(at, past + chunk)
+    new.insert(at, chunk)
+    check_prefill(lens, new, H, Hkv, bits, 64, small, tail=0)
+    for g in range(0, small, 5):
+        if g != at:
+            new[g] = (0, 3, 2)[g % 3]
+    check_prefill(lens, new, H, Hkv, bits, 64, small + 1, tail=5)
+    lens[at] = chunk // 2  # more queries than tokens
+    check_prefill(lens, new, H, Hkv, bits, 64, small + 2, tail=1)
+
+
+@pytest.mark.parametrize("bits", [4, 2])
+@pytest.mark.parametrize("H, Hkv, new", [(32, 8, [9 + g % 12 for g in range(16)]), (16, 8, list(range(17, 41, 3))), (32, 8, [20 + 5 * g for g in range(8)]), (32, 8, [3, 5, 8, 9, 12, 20, 4, 6, 2, 1, 15, 3])])
+def test_prefill_requests_of_a_few_to_a_few_dozen_tokens(H, Hkv, new, bits):
+    # whole and cut blocks, of one launch
+    check_prefill([n + 2600 + 100 * g for g, n in enumerate(new)], new, H, Hkv, bits, 32, len(new))
+    check_prefill([n + 30 * g for g, n in enumerate(new)], new, H, Hkv, bits, 32, len(new), tail=0)
+
+
+def test_prefill_captured_batches_of_every_kind():
+    # one graph, whose replays hand the same 96 query rows out to the requests in other ways: the parts of a block follow
+    rng = np.random.default_rng(3)
+    T, G, H, Hkv, bits, page = 96, 20, 32, 8, 4, 32
+    lens = [3000 + 50 * g for g in range(G)]
+    table, q, out, ck, cv, kn, vn, R, _ = attention_inputs(rng, lens, H, Hkv, bits, page, T=T)
+    d, st, ws = i32(lens), i32(np.zeros(G + 1)), ops.paged_workspace(T, G, H)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        ops.paged_prefill_attention(out, q, ck, cv, kn, vn, R, table, d, st, page, H, Hkv, bits, ws)
+    for new in ([77] + [1] * 19, [1] * 20, [5] * 19 + [1], [0] * 19 + [96], [9] * 10 + [0] * 10, [0] * 20, [1] * 10 + [43] * 2 + [0] * 8, [48, 48] + [0] * 18, [40, 1, 0] * 2 + [0] * 14):
+        start = [0] + np.cumsum(new).tolist()
+        st.copy_(i32(start))
+        ws.fill_(255)  # (nothing is kept in it)
+        out.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = pu.attention(q, ck, cv, kn, vn, R, table, lens, start, page, H, Hkv, bits)
+        pu.assert_attention(out[:start[-1]], (want[0][:start[-1]], want[1][:start[-1]]), str(new))
+        assert (out[start[-1]:] == 7).all()
+
+
+@pytest.mark.parametrize("chunk", [64, 65])
+def test_single_tokens_do_not_slow_a_chunk_down(chunk):
+    # (Its context is cut along the SMs that idle, with single tokens beside it as alone; uncut beside 63 it took 7 times as long as alone, cut 2.4 times, theirs
+    # included.  The fastest of some rounds, so that other work on the machine does not count.)
+    def us(lens, new, H=32, Hkv=8, bits=4, page=64):
+        rng = np.random.default_rng(0)
+        start = [0] + np.cumsum(new).tolist()
+        table, q, out, ck, cv, kn, vn, R, _ = attention_inputs(rng, lens, H, Hkv, bits, page, T=start[-1])
+        d, st, ws = i32(lens), i32(start), ops.paged_workspace(start[-1], len(lens), H)
+        best = []
+        for _ in range(8):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            for _ in range(10):
+                ops.paged_prefill_attention(out, q, ck, cv, kn, vn, R, table, d, st, page, H, Hkv, bits, ws)
+            b.record()
+            torch.cuda.synchronize()
+            best.append(a.elapsed_time(b))
+        return min(best)
+
+    assert us([30000 + chunk] + [900] * 63, [chunk] + [1] * 63) < 4.5 * us([30000 + chunk], [chunk])

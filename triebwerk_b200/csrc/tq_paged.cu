@@ -205,10 +205,11 @@ int tq_paged_read(void* k_out, void* v_out, const uint8_t* ck_q, const void* k_n
 struct PrefillCut {
     bool small, large;   // whether there may be requests of up to, of more than ROWS_MOST score rows
     int ncb, parts;      // small ones: row blocks of 8 per CTA, parts of a request's tokens
-    int mt, splits;      // large ones: blocks of 128 rows per CTA, parts of a block's tiles
+    int mt, most_parts;  // large ones: blocks of 128 rows per CTA; parts that a block's tiles may be cut into, 1: not cut
+    bool mostly_small;   // requests are small in the mean: none may be large, or one
 };
 constexpr int SPLIT_SMS = 160, MAX_SPLITS = 16;
-// Rows of partial sums that those calls may write.  Large requests are cut only while splits * blocks of 128 rows <= the SMs; small ones, of which a request
+// Rows of partial sums that those calls may write.  Large requests are cut only while parts * blocks of 128 rows <= the SMs and the parts fit; small ones, of which a request
 // has 32 rows per KV head at most, into as many parts as fit.
 static size_t large_rows(long long T, long long H) { return (size_t)std::min<long long>(MAX_SPLITS * T * H, (long long)SPLIT_SMS * PFT_ROWS); }
 static size_t small_rows(long long T, long long G, long long H) {
@@ -246,10 +247,16 @@ static PrefillCut prefill_cut(int T, int G, int H, int Hkv, int most) {
     }
     // Two blocks a CTA take 1.3 to 1.4 times as long as one, and the SMs serve a turn of CTAs at a time.  (us, one / two: 4-bit 32/8 heads 1 x 512 tokens
     // 16.6 / 21.3, 1 x 2048 91.6 / 62.0, 4 x 512 52.4 / 39.6, 1 x 1024 behind 8192 273 / 209; 2-bit 16/8 2 x 512 behind 8192 139 / 186, 4 x 512
-    // 30.7 / 24.6, 4 x 2048 behind 4096 583 / 437.)  Blocks that leave half of the SMs idle are cut (2-bit 16/8 1 x 256 behind 20000: 294 uncut, 99).
+    // 30.7 / 24.6, 4 x 2048 behind 4096 583 / 437.)
     const long long blocks1 = Hkv * G * ((mean + qt - 1) / qt), blocks2 = Hkv * G * ((mean + 2 * qt - 1) / (2 * qt));
     c.mt = mean > qt && 27 * ((blocks2 + sms - 1) / sms) < 20 * ((blocks1 + sms - 1) / sms) ? 2 : 1;
-    c.splits = c.mt == 2 ? 1 : (int)std::max(1ll, std::min({sms / std::max(blocks1, 1ll), (long long)most / (4 * PFT_KT), (long long)MAX_SPLITS}));
+    // Blocks that leave half of the SMs idle are cut (2-bit 16/8 1 x 256 behind 20000: 294 uncut, 99).  Where requests are small in the mean or differ, they may: all tokens
+    // but a few may be one request's, beside single tokens that have no block, so the fewest blocks that T can make decide, and the kernel counts what there is.
+    // (Never cut / so, 4-bit 32/8 heads: 63 single tokens beside 64 behind 30000 560 / 186, 15 beside 200 behind 16000 297 / 185, 12 x 3 to 20 behind 4000 107 / 81,
+    // 31 x 1 and 64 behind 8000 181 / 87; no block to cut in 32 x 1 to 5 behind 2000 to 4000 86.7 / 87.2, too many in 16 x 9 to 20 behind 4000 77.5 / 82.2.)
+    c.mostly_small = mean * grp <= ROWS_MOST;
+    const long long fewest = alike && !c.mostly_small ? blocks1 : std::min(blocks1, Hkv * ((T + qt - 1) / qt));
+    c.most_parts = c.mt == 2 || 2 * fewest > sms ? 1 : (int)std::max(1ll, std::min({(long long)most / (4 * PFT_KT), (long long)MAX_SPLITS, (long long)large_rows(T, H) / ((long long)T * H)}));
     return c;
 }
 extern "C" {
@@ -392,7 +399,7 @@ int tq_paged_prefill_attention(void* out, const void* q, const uint8_t* ck_q, co
     float* const small_sums = (float*)workspace + large_rows(T, H) * PART_STRIDE;
     PagedMergeParams m{};
     m.partials = (const float*)workspace; m.small_partials = small_sums; m.rotation = (const __half*)rotation; m.start = query_start; m.out = (__half*)out;
-    m.T = T; m.H = H; m.grp = grp; m.out_stride = out_stride; m.small_rows = cut.small ? ROWS_MOST : 0;
+    m.T = T; m.G = G; m.H = H; m.Hkv = Hkv; m.grp = grp; m.out_stride = out_stride; m.small_rows = cut.small ? ROWS_MOST : 0;
     if (cut.large) {
         const int qt = PFT_ROWS / grp, bt = cut.mt * qt;
         const long long requests = std::min<long long>(G, cut.small ? T / (most_small + 1) : T), ctas = (long long)Hkv * (T / bt + requests);
@@ -406,12 +413,16 @@ int tq_paged_prefill_attention(void* out, const void* q, const uint8_t* ck_q, co
         r = make_prefill_query_map(&tmQ, q, T, H, grp, qt, q_stride);
         if (r == TQ_OK) r = make_prefill_rows_map(&tmR, rotation, HEAD_DIM, HEAD_DIM);
         if (r != TQ_OK) return r;
-        const dim3 grid((unsigned)ctas, 1, (unsigned)cut.splits);
+        // CTAs: the most blocks that there can be, and where they may be cut, enough for their parts; where none may be there at all, two thirds of the SMs, so that
+        // the launch for few rows starts on the others at once (4-bit 32/8 heads 32 x 1 to 5 behind 2000 to 4000 95 with all, 90; 12 x 1 to 20 behind 4000 78 / 81).
+        const long long sms = std::min(device_props().sm_count, SPLIT_SMS), room = cut.mostly_small ? 2 * sms / 3 : sms;
+        const dim3 grid((unsigned)std::max(ctas, std::min(room, ctas * cut.most_parts)));
+        p.room = (int)std::min<long long>(grid.x, sms); p.most_parts = cut.most_parts;
+        m.room = p.room; m.most_parts = cut.most_parts > 1 ? cut.most_parts : 0;
         if (cut.mt == 2) r = bits == 4 ? launch_paged_prefill<4, 2, false>(tmQ, tmR, p, grid, cs(s)) : launch_paged_prefill<2, 2, false>(tmQ, tmR, p, grid, cs(s));
-        else if (cut.splits == 1) r = bits == 4 ? launch_paged_prefill<4, 1, false>(tmQ, tmR, p, grid, cs(s)) : launch_paged_prefill<2, 1, false>(tmQ, tmR, p, grid, cs(s));
+        else if (cut.most_parts == 1) r = bits == 4 ? launch_paged_prefill<4, 1, false>(tmQ, tmR, p, grid, cs(s)) : launch_paged_prefill<2, 1, false>(tmQ, tmR, p, grid, cs(s));
         else r = bits == 4 ? launch_paged_prefill<4, 1, true>(tmQ, tmR, p, grid, cs(s)) : launch_paged_prefill<2, 1, true>(tmQ, tmR, p, grid, cs(s));
         if (r != TQ_OK) return r;
-        m.splits = cut.splits > 1 ? cut.splits : 0;
     }
     if (cut.small) {
         PagedRowsParams p{};
@@ -430,10 +441,12 @@ int tq_paged_prefill_attention(void* out, const void* q, const uint8_t* ck_q, co
         if (r != TQ_OK) return r;
         m.small_splits = cut.parts; m.part_tokens = p.part_tokens; m.by_request = p.by_request;
     }
-    if (m.splits == 0 && m.small_splits == 0) return TQ_OK;
-    // (rows of a request: 16 a CTA, which loop where a large one was cut)
-    const long long most_rows = cut.large && m.splits ? (long long)T * H : (long long)std::min(T, most_small) * H;
-    const dim3 grid((unsigned)std::min<long long>((most_rows + 15) / 16, std::max(1, 8 * device_props().sm_count / std::min(G, 8))), (unsigned)G);
+    if (m.most_parts == 0 && m.small_splits == 0) return TQ_OK;
+    // Rows of a request: 16 a CTA, which loop where a large one was cut: 16 CTAs per SM in all (as CTAs without work cost their turn), twice that where a large
+    // request's would be few.  (us by 4, 8, 16, 32 of them, 4-bit 32/8 heads: 63 single tokens beside 64 behind 30000 221 / 221 / 198 / 187, 15 beside 200
+    // behind 16000 218 / 198 / 186 / 183, 16 x 9 to 20 behind 600 to 1500, uncut, 37.9 / 38.9 / 39.7 / 41.4.)
+    const long long most_rows = cut.large && m.most_parts ? (long long)T * H : (long long)std::min(T, most_small) * H, few = ((long long)std::min(T, most_small) * H + 15) / 16;
+    const dim3 grid((unsigned)std::min<long long>((most_rows + 15) / 16, std::max<long long>({1, few, (cut.mostly_small ? 32 : 16) * device_props().sm_count / G})), (unsigned)G);
     return launch_kernel(paged_merge_kernel, grid, dim3(256), 0, cs(s), use_pdl(), m);
 }
 

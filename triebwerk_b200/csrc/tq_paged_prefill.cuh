@@ -14,8 +14,9 @@
 //   * All 16 warps make a share of every tile.  MT = 2: K of tile j + 1 before the softmax of tile j, V behind it.  MT = 1: after tile j, which is
 //     one slot's, K of tile j + 2 and V of tile j + 1, so that the other slot's warps need not wait for tile j's products.
 //   * Three warps fetch the tiles' rows (one page number for each 32 tokens) and norms ahead, into a ring in shared memory.
-//   * SPLIT (MT = 1): few query rows, long contexts: the tiles of a block are cut into gridDim.z parts, whose sums meet in
-//     paged_merge_kernel.
+//   * SPLIT (MT = 1): few query rows, long contexts: the tiles of every block are cut into as many parts as the SMs have room for, whose
+//     sums meet in paged_merge_kernel.  How many blocks there are is known here, not on the host, which knows no request's share of the
+//     batch's tokens: single tokens beside a chunk have no block of this kernel (4-bit 32/8 heads, 63 beside 64 tokens behind 30000: 560 us uncut, 186 cut).
 // Blocks are found without a table: every CTA takes the running sum of the requests' blocks (BT query tokens each) and looks where its number
 // falls; the launch has room for as many as there can be, and those behind the last end at once.  Requests of few rows (small_rows) have none: those
 // are tq_paged_rows.cuh's.
@@ -25,6 +26,8 @@
 // instructions, 6500 a warp-wide pair of tiles (issue slots 57 %, products 40 % of the cycles; stamps: 5000 cycles a pair), and at the ends of short prompts a
 // CTA's start (5800 cycles: table, queries times R, first rows) and end.
 #pragma once
+
+#include <climits>
 
 #include "tq_paged.cuh"
 
@@ -39,12 +42,17 @@ struct PagedPrefillParams {
     const int* lens;          // [G]; 0 and less: no token
     const int* start;         // [G + 1]
     __half* out;
-    float* partials;          // SPLIT: [splits][T][H][PART_STRIDE]
+    float* partials;          // SPLIT: [parts][T][H][PART_STRIDE]
     int* status;
     int table_stride, page_shift, num_pages, most_tokens;
     int T, G, H, Hkv, grp, out_stride;
     int small_rows;           // requests of up to so many score rows (new tokens x heads of a KV head) are not served here
+    int room, most_parts;     // SPLIT: see prefill_parts
 };
+// Parts that every block's tiles are cut into: as many as give `room` CTAs a part each.
+__device__ __forceinline__ int prefill_parts(int blocks, int Hkv, int room, int most) {  // blocks: of 128 rows, of all requests and one KV head
+    return (int)max(1ll, min((long long)most, room / ((long long)max(blocks, 1) * Hkv)));
+}
 
 constexpr int PPF_THREADS = 32 * PFT_SOFT_WARPS + 128;  // softmax and operands; one warp for the products, three for rows and norms
 constexpr int PPF_MEET = 32 * PFT_SOFT_WARPS + 32;      // all but those
@@ -127,23 +135,45 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     pdl_wait();  // (lengths, tables, caches, queries: all of earlier launches)
     pdl_launch_dependents();  // (behind the wait: what starts now knows that those have finished)
     // ---- the request and the block of this CTA ----
-    const int kvh = (int)blockIdx.x % p.Hkv, y = (int)blockIdx.x / p.Hkv;
-    // First query, queries of the request, the block's first one, request.  (They wait in shared memory for the end, which is what else needs them: in
+    const int kvh = (int)blockIdx.x % p.Hkv;
+    int y = (int)blockIdx.x / p.Hkv;  // SPLIT: all blocks' first parts, then their second ones
+    // First query, queries of the request, the block's first one, request; SPLIT: part and parts.  (They wait in shared memory for the end, which is what else needs them: in
     // registers they cost spills, and those come back from L2, see below.)  The warps' block counts lie where K comes later.
     volatile int* const kept = reinterpret_cast<volatile int*>(gb + PpfSmem::CTRL + 228);
     int* const scratch = reinterpret_cast<int*>(gb + PpfSmem::K);
     constexpr int WARPS = PPF_THREADS / 32;
     if (tid == 0) kept[3] = -1;
     tc_fence_before();
-    int before = 0;
-    for (int first = 0; first < p.G; first += PPF_THREADS) {
-        const int i = first + tid;
-        int a = 0, m = 0;
+    int before = 0, part = 0, parts = 1;
+    auto blocks_of = [&](int i, int& a, int& m) {
+        a = m = 0;
         if (i < p.G) {
             a = max(p.start[i], 0);
             m = max(min(p.start[i + 1], p.T) - a, 0);
         }
-        const int blocks = m * GRP > p.small_rows ? (m + BT - 1) / BT : 0;
+        return m * GRP > p.small_rows ? (m + BT - 1) / BT : 0;
+    };
+    auto cut = [&](int blocks) {  // of all requests
+        parts = prefill_parts(blocks, p.Hkv, p.room, p.most_parts);
+        part = y / max(blocks, 1);
+        y = part < parts ? y - part * blocks : INT_MAX;
+        if (tid == 0) kept[4] = part | parts << 8;
+    };
+    if (SPLIT && p.G > PPF_THREADS) {  // (otherwise the sum is at hand below)
+        int sum = 0, a, m;
+        for (int i = tid; i < p.G; i += PPF_THREADS) sum += blocks_of(i, a, m);
+        sum = __reduce_add_sync(0xffffffffu, sum);
+        if (lane == 0) scratch[warp] = sum;
+        __syncthreads();
+        sum = 0;
+        for (int w = 0; w < WARPS; ++w) sum += scratch[w];
+        cut(sum);
+        __syncthreads();
+    }
+    for (int first = 0; first < p.G; first += PPF_THREADS) {
+        const int i = first + tid;
+        int a, m;
+        const int blocks = blocks_of(i, a, m);
         int incl = blocks;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -158,6 +188,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             mine += w < warp ? v : 0;
             all += v;
         }
+        if (SPLIT && p.G <= PPF_THREADS) cut(all);
         const int at = y - (mine + incl - blocks);
         if (at >= 0 && at < blocks) {  // (the last blocks of a request, whose causal prefixes are the longest, first)
             kept[0] = a;
@@ -187,11 +218,13 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     const int L = min(max(p.lens[g], 0), p.most_tokens), pos0 = L - n;  // position of the request's first new token
     // tiles that the block whose first query is `first` reads
     auto tiles_to = [&](int first) { return first < n ? (int)(((unsigned)max(pos0 + min(first + QT, n), 0) + (PFT_KT - 1u)) / PFT_KT) : 0; };
-    const int t_lo = SPLIT ? (int)((long long)tiles_to(q0) * blockIdx.z / gridDim.z) : 0;
-    const int n_all = (SPLIT ? (int)((long long)tiles_to(q0) * (blockIdx.z + 1) / gridDim.z) : tiles_to(q0)) - t_lo;
+    const int t_lo = SPLIT ? (int)((long long)tiles_to(q0) * part / parts) : 0;
+    const int n_all = (SPLIT ? (int)((long long)tiles_to(q0) * (part + 1) / parts) : tiles_to(q0)) - t_lo;
     const int n0 = MT == 2 ? n_all : (n_all + 1) / 2, n1 = MT == 2 ? tiles_to(q0 + QT) : n_all / 2;
     const int n_tiles = MT == 2 ? max(n0, n1) : n_all;
     auto tile_of = [&](int s, int i) { return MT == 2 ? i : 2 * i + s; };  // (behind t_lo)
+
+    auto joined = [&]() { return SPLIT && kept[4] >> 8 > 1; };  // (uniform) the results are paged_merge_kernel's
 
     bool dead = false;
     auto wait_bar = [&](uint32_t bar, uint32_t parity) {
@@ -269,7 +302,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             if (n1 > 0) issue_scores(1, 0);
             // R again, for the results, where V of the tile in front of the last was: as soon as its products are done
             auto fetch_rotation = [&]() {
-                if (SPLIT) return;
+                if (joined()) return;
                 if (n_tiles >= 2) wait_bar(bar_vfree + 8u * (n_tiles & 1), (uint32_t)(((n_tiles - 2) >> 1) & 1));
                 if (dead) return;
                 mbar_arrive_expect_tx(bar_r, PFT_TILE);
@@ -295,7 +328,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             if (MT == 1 || n_tiles == 0) fetch_rotation();
         }
         __syncwarp();
-        if (!SPLIT) {
+        if (!joined()) {
             // out[d] = sum_k R[k][d] * acc[k]
             auto rotate_back = [&](int m, uint32_t bar) {
                 if (lane == 0) {
@@ -606,7 +639,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         auto token_e = [&](int row, uint32_t by_grp) { return token_in(row, by_grp) < QT ? first_e + token_in(row, by_grp) : n_e; };
 
         // ================= results =================
-        float w0[2], w1[2] = {0.0f, 0.0f};  // by row: weights of the slots' sums, normalised (MT = 2: of its own; SPLIT: not normalised)
+        float w0[2], w1[2] = {0.0f, 0.0f};  // by row: weights of the slots' sums, normalised (MT = 2: of its own; joined: not normalised)
         float M_all[2], Z_all[2];
         if constexpr (MT == 1) {
             named_barrier(2, 32 * PFT_SOFT_WARPS);  // (every warp has made its last tile)
@@ -622,7 +655,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                 const float M = fmaxf(a.x, b.x), e0 = n0 > 0 ? ex2_approx(a.x - M) : 0.0f, e1 = n1 > 0 ? ex2_approx(b.x - M) : 0.0f;
                 M_all[h] = M;
                 Z_all[h] = a.y * e0 + b.y * e1;
-                const float inv = (1.0f / PPF_CENT<BITS>) * (SPLIT ? 1.0f : 1.0f / (Z_all[h] + 1e-8f));
+                const float inv = (1.0f / PPF_CENT<BITS>) * (joined() ? 1.0f : 1.0f / (Z_all[h] + 1e-8f));
                 w0[h] = e0 * inv;
                 w1[h] = e1 * inv;
             }
@@ -654,21 +687,24 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             }
         };
         if constexpr (SPLIT) {
-            // the sums as they are, with maximum and sum of weights behind them
-            const uint32_t by_grp = make_by_grp();
-            const int c0 = pcol0;
-            float v[32];
-            result(c0, v);
+            if (joined()) {
+                // the sums as they are, with maximum and sum of weights behind them
+                const uint32_t by_grp = make_by_grp();
+                const int c0 = pcol0;
+                float v[32];
+                result(c0, v);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int row = row0 + gl + 8 * h, tok = token_e(row, by_grp);
-                if (tok >= n_e) continue;
-                float* const dst = p.partials + (((size_t)blockIdx.z * p.T + s0_e + tok) * p.H + (size_t)(kvh * GRP + row - token_in(row, by_grp) * GRP)) * PART_STRIDE;
+                for (int h = 0; h < 2; ++h) {
+                    const int row = row0 + gl + 8 * h, tok = token_e(row, by_grp);
+                    if (tok >= n_e) continue;
+                    float* const dst = p.partials + (((size_t)(kept[4] & 255) * p.T + s0_e + tok) * p.H + (size_t)(kvh * GRP + row - token_in(row, by_grp) * GRP)) * PART_STRIDE;
 #pragma unroll
-                for (int b = 0; b < 8; ++b) *reinterpret_cast<float2*>(dst + c0 + 8 * b + 2 * t4) = make_float2(v[4 * b + 2 * h], v[4 * b + 2 * h + 1]);
-                if (slot == 0 && t4 == 0) *reinterpret_cast<float2*>(dst + HEAD_DIM) = on[h] ? make_float2(M_all[h], Z_all[h]) : make_float2(-1e30f, 0.0f);
+                    for (int b = 0; b < 8; ++b) *reinterpret_cast<float2*>(dst + c0 + 8 * b + 2 * t4) = make_float2(v[4 * b + 2 * h], v[4 * b + 2 * h + 1]);
+                    if (slot == 0 && t4 == 0) *reinterpret_cast<float2*>(dst + HEAD_DIM) = on[h] ? make_float2(M_all[h], Z_all[h]) : make_float2(-1e30f, 0.0f);
+                }
             }
-        } else {
+        }
+        if (!joined()) {
             // The normalised rows as fp16 over the Q tile, times R.  (One rounding more, relative to a row 2^-11 at most, as R changes no length; with
             // a low part beside it the way from the last tile to the end, a third of a short prompt's time, was twice as many products and stores.)
             const uint32_t qtile = PpfSmem::Q + pslot * PFT_TILE;
@@ -722,28 +758,49 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 // The parts of a request whose tokens were cut: out[tok][h] = R (sum_z 2^(m_z - M) acc_z / sum_z 2^(m_z - M) l_z).  16 (token, head) rows per CTA, two a
 // warp; fp16 high and low parts of the sums times R on mma.sync, a warp 16 output coordinates.
 struct PagedMergeParams {
-    const float* partials;        // [splits][T][H][PART_STRIDE]
+    const float* partials;        // PagedPrefillParams::partials
     const float* small_partials;  // PagedRowsParams::partials
     int part_tokens, by_request;
     const __half* rotation;       // R row-major
     const int* start;        // [G + 1]
     __half* out;
-    int splits, small_splits;  // parts of the requests of more than small_rows rows (0: none of them is cut), of the others
+    int room, most_parts;  // PagedPrefillParams' (most_parts 0: no request of more than small_rows rows is cut)
+    int small_splits;      // parts of the others (0: there are none)
     int small_rows;
-    int T, H, grp, out_stride;
+    int T, G, H, Hkv, grp, out_stride;
 };
 static __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedMergeParams p) {
     __shared__ __align__(16) __half r_s[HEAD_DIM / 2][HEAD_DIM + 8];
     __shared__ __align__(16) __half a_s[2][16][HEAD_DIM + 8];
+    __shared__ int blocks_s[8];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gl = lane >> 2, t4 = lane & 3;
     pdl_launch_dependents();
     // (the kernels before let this one start when what came before the call has finished: R and the batch may be read; the sums not yet)
     const int s0 = max(p.start[blockIdx.y], 0), n = max(min(p.start[blockIdx.y + 1], p.T) - s0, 0);
     const bool large = n * p.grp > p.small_rows;
-    const int splits = large ? p.splits : p.small_splits;
     const long long rows = (long long)n * p.H;
+    int splits = p.small_splits;
+    if (large) {
+        splits = 0;
+        if (p.most_parts > 0 && 16ll * blockIdx.x < rows) {  // as the kernel that made them
+            const int qt = PFT_ROWS / p.grp;
+            int blocks = 0;
+            for (int i = tid; i < p.G; i += 256) {
+                const int m = max(min(p.start[i + 1], p.T) - max(p.start[i], 0), 0);
+                if (m * p.grp > p.small_rows) blocks += (m + qt - 1) / qt;
+            }
+            blocks = __reduce_add_sync(0xffffffffu, blocks);
+            if (lane == 0) blocks_s[warp] = blocks;
+            __syncthreads();
+            blocks = 0;
+#pragma unroll
+            for (int w = 0; w < 8; ++w) blocks += blocks_s[w];
+            splits = prefill_parts(blocks, p.Hkv, p.room, p.most_parts);
+            if (splits == 1) splits = 0;  // (the results are in place)
+        }
+    }
     if (splits == 0 || 16ll * blockIdx.x >= rows) {
-        pdl_wait();
+        if (blockIdx.x + blockIdx.y == 0) pdl_wait();  // (this launch ends behind the ones before; whoever has work waits below)
         return;
     }
     uint32_t bf[2][8][2];
