@@ -368,7 +368,7 @@ static int launch_paged_prefill(const CUtensorMap& tmQ, const CUtensorMap& tmR, 
 
 template <int BITS, int NCB>
 static int launch_rows(const PagedRowsParams& p, dim3 grid, cudaStream_t s) {
-    constexpr size_t smem = rows_smem_bytes<BITS, NCB>();
+    constexpr size_t smem = rows_smem_bytes<BITS>();
     const int r = ensure_dynamic_smem((const void*)paged_rows_kernel<BITS, NCB>, smem);
     return r != TQ_OK ? r : launch_kernel(paged_rows_kernel<BITS, NCB>, grid, dim3(ROWS_THREADS<NCB>), smem, s, use_pdl(), p);
 }

@@ -397,7 +397,6 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         // ================= operands and softmax =================
         // ---- a thread's share of every tile: piece tid & 3 of row tid >> 2 ----
         const int mrow = tid >> 2, piece = tid & 3;
-        constexpr int FORMS = 4;        // 16-byte pieces of fp16 per share
         uint4 kc, vc;                   // codes of the next tile (2-bit: x, y)
         auto info_of = [&](int j) { return gb + PpfSmem::INFO + (uint32_t)(j & (PPF_STAGES - 1)) * PpfSmem::INFO_BYTES; };
         // (four words in the order in which put_codes takes them)

@@ -56,7 +56,7 @@ struct RowsSmem {
     static constexpr uint32_t END = FRAG + NCB * 2048u;
     static constexpr uint32_t WARP = 9u * 32u * 16u;                     // a warp's sums of one row block, at the end: [9][32 lanes][4 floats]
 };
-template <int BITS, int NCB>
+template <int BITS>
 constexpr size_t rows_smem_bytes() {  // counted from address 0
     return ROWS_LUT_ABS + (BITS == 4 ? 0x10000u : 0x1000u);
 }
