@@ -180,3 +180,9 @@ def test_attentions_refuse_addresses_that_no_element_has(call, arrays, name, off
     if name in arrays:
         a = dict(apart(arrays), ws=C.c_void_p(64 << 20))
         assert call(**dict(a, **{name: C.c_void_p(a[name].value + off)})) == -1
+
+
+def test_no_query_rows_need_no_arrays():
+    # (an empty tensor has no address)
+    assert prefill(T=0, out=None, q=None) == 0
+    assert prefill(out=None) == -1 and prefill(q=None) == -1

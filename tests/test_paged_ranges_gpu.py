@@ -238,3 +238,20 @@ def test_single_tokens_do_not_slow_a_chunk_down(chunk):
         return min(best)
 
     assert us([30000 + chunk] + [900] * 63, [chunk] + [1] * 63) < 4.5 * us([30000 + chunk], [chunk])
+
+
+def test_a_step_without_tokens():
+    # every call of a step takes empty arrays; nothing is launched but the plan
+    rng = np.random.default_rng(1)
+    G, H, Hkv, page = 3, 16, 8, 32
+    table, q, out, ck, cv, kn, vn, R, _ = attention_inputs(rng, [40, 0, 7], H, Hkv, 4, page, T=0)
+    q, out = q.contiguous(), out.contiguous()
+    lens, start, count, slots = i32([40, 0, 7]), i32([9] * 4), i32([2]), torch.zeros(0, dtype=torch.int64, device="cuda")
+    kv = torch.zeros(0, Hkv * 128, dtype=torch.float16, device="cuda")
+    before = [x.clone() for x in (ck, kn.view(torch.int16), cv, vn.view(torch.int16))]
+    ops.page_plan(table, i32([0, 1, 2, 3]), count, count, lens, i32([0, 0, 0]), None, page, lens, start, slots)
+    ops.paged_append(ck, kn, cv, vn, kv, kv, R, slots, Hkv, 4)
+    ops.paged_read(kv, kv, ck, kn, cv, vn, R, slots, Hkv, 4)
+    ops.paged_prefill_attention(out, q, ck, cv, kn, vn, R, table, lens, start, page, H, Hkv, 4, ops.paged_workspace(0, G, H))
+    assert lens.tolist() == [40, 0, 7] and start.tolist() == [0] * 4 and int(count) == 2
+    assert all(torch.equal(a, b) for a, b in zip(before, (ck, kn.view(torch.int16), cv, vn.view(torch.int16))))

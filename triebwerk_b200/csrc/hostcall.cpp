@@ -137,7 +137,7 @@ struct Args {
 };
 // Rows of a 2-D tensor whose elements lie side by side: how far apart they begin.
 int row_stride(const at::Tensor& t, const char* what) {
-    need(t.dim() == 2 && (t.size(1) <= 1 || t.stride(1) == 1), what);
+    need(t.dim() == 2 && (t.numel() == 0 || t.size(1) <= 1 || t.stride(1) == 1), what);  // (an empty one may have any strides)
     const long long s = t.size(0) <= 1 ? std::max<long long>(t.size(1), 1) : t.stride(0);
     need(s >= t.size(1) && s <= INT_MAX && t.size(0) <= INT_MAX, what);
     return (int)s;

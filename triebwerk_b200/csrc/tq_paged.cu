@@ -268,14 +268,14 @@ size_t tq_paged_workspace_bytes(int T, int G, int num_heads) {
 
 // What both attentions check of their arguments.
 static int check_attention(const void* out, const void* q, const uint8_t* ck, const uint8_t* cv, const void* kn, const void* vn, const void* rotation,
-                           const int* table, int table_stride, int table_width, const int* lens, int num_pages, int page_size, int G, int H, int Hkv,
+                           const int* table, int table_stride, int table_width, const int* lens, int num_pages, int page_size, int T, int G, int H, int Hkv,
                            int head_dim, int q_stride, int out_stride, int bits) {
     int r = check_pages(table_stride, table_width, num_pages, page_size);
     if (r != TQ_OK) return r;
     if (head_dim != HEAD_DIM) return TQ_ERR_UNSUPPORTED;
     if (G <= 0 || H <= 0 || Hkv <= 0 || H % Hkv != 0 || (bits != 2 && bits != 4)) return TQ_ERR_ARG;
     if ((long long)q_stride < (long long)H * HEAD_DIM || (long long)out_stride < (long long)H * HEAD_DIM || q_stride % 8 != 0 || out_stride % 8 != 0) return TQ_ERR_ARG;
-    if (!out || !q || !ck || !cv || !kn || !vn || !rotation || !table || !lens) return TQ_ERR_ARG;
+    if (!ck || !cv || !kn || !vn || !rotation || !table || !lens || (T > 0 && (!out || !q))) return TQ_ERR_ARG;
     if (!aligned({out, q, ck, cv, kn, vn, rotation}, 16) || !aligned({table, lens}, 4)) return TQ_ERR_ARG;
     return TQ_OK;
 }
@@ -293,7 +293,7 @@ int tq_paged_decode_attention(void* out, const void* q, const uint8_t* ck_q, con
                               const void* rotation, const int* block_table, int table_stride, int table_width, const int* seq_lens, int num_pages,
                               int page_size, int G, int num_heads, int num_kv_heads, int head_dim, int q_stride, int out_stride, int bits,
                               void* workspace, size_t workspace_bytes, tq_stream_t s) {
-    int r = check_attention(out, q, ck_q, cv_q, k_norms, v_norms, rotation, block_table, table_stride, table_width, seq_lens, num_pages, page_size, G,
+    int r = check_attention(out, q, ck_q, cv_q, k_norms, v_norms, rotation, block_table, table_stride, table_width, seq_lens, num_pages, page_size, G, G,
                             num_heads, num_kv_heads, head_dim, q_stride, out_stride, bits);
     if (r != TQ_OK) return r;
     if (!workspace || workspace_bytes < tq_paged_workspace_bytes(G, G, num_heads) || !aligned({workspace}, 256)) return TQ_ERR_WORKSPACE;
@@ -379,7 +379,7 @@ int tq_paged_prefill_attention(void* out, const void* q, const uint8_t* ck_q, co
                                const void* rotation, const int* block_table, int table_stride, int table_width, const int* seq_lens,
                                const int* query_start, int num_pages, int page_size, int T, int G, int num_heads, int num_kv_heads, int head_dim,
                                int q_stride, int out_stride, int bits, void* workspace, size_t workspace_bytes, tq_stream_t s) {
-    int r = check_attention(out, q, ck_q, cv_q, k_norms, v_norms, rotation, block_table, table_stride, table_width, seq_lens, num_pages, page_size, G,
+    int r = check_attention(out, q, ck_q, cv_q, k_norms, v_norms, rotation, block_table, table_stride, table_width, seq_lens, num_pages, page_size, T, G,
                             num_heads, num_kv_heads, head_dim, q_stride, out_stride, bits);
     if (r != TQ_OK) return r;
     if (T < 0 || !query_start || !aligned({query_start}, 4)) return TQ_ERR_ARG;
