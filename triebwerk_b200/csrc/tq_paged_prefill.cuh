@@ -22,7 +22,7 @@
 // are tq_paged_rows.cuh's.
 // Every wait on a barrier is bounded, as there.
 //
-// 4-bit: 8 prompts of 512, 16/8 heads, 45 us; 4 x 1024 behind 5100 to 8192, 32/8 heads, 605 to 630 us (0.73 PFLOP/s; GPUs differ).  What bounds it is the number of
+// 4-bit: 8 prompts of 512, 16/8 heads, 45 us; 4 x 1024 behind 5100 to 8192, 32/8 heads, 605 to 639 us (0.70 to 0.74 PFLOP/s; GPUs differ).  What bounds it is the number of
 // instructions, 6500 a warp-wide pair of tiles (issue slots 57 %, products 40 % of the cycles; stamps: 5000 cycles a pair), and at the ends of short prompts a
 // CTA's start (5800 cycles: table, queries times R, first rows) and end.
 #pragma once

@@ -12,7 +12,7 @@
 //   * The warps' sums meet in shared memory, halves in turn; the CTA's go to the workspace, paged_merge_kernel adds the parts up.
 //
 // What bounds it is instruction issue (54 % of the slots used under a profiler) and a CTA's start and end, 5 to 11 us in all: 32 requests of 5 tokens behind
-// 4000, 2-bit, 32/8 heads (71 MB of codes and norms, 11 us at the copy rate) take 117 us with the merge, 4-bit 145; of 1 to 5 tokens behind 2000 to 4000 88 us,
+// 4000, 2-bit, 32/8 heads (71 MB of codes and norms, 11 us at the copy rate) take 118 us with the merge, 4-bit 146; of 1 to 5 tokens behind 2000 to 4000 88 us,
 // 131 us on the tcgen05 kernel.
 #pragma once
 
