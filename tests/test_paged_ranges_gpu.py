@@ -255,3 +255,151 @@ def test_a_step_without_tokens():
     ops.paged_prefill_attention(out, q, ck, cv, kn, vn, R, table, lens, start, page, H, Hkv, 4, ops.paged_workspace(0, G, H))
     assert lens.tolist() == [40, 0, 7] and start.tolist() == [0] * 4 and int(count) == 2
     assert all(torch.equal(a, b) for a, b in zip(before, (ck, kn.view(torch.int16), cv, vn.view(torch.int16))))
+
+
+# ---- offsets of more than 32 bits ---------------------------------------------------------------------------------------------------
+def test_pages_behind_the_first_4_gigabytes():
+    # the same rows in a small pool and at the end of one whose code arrays pass 4 GB and 2^32 bytes of offsets: the same bytes, rows and results
+    rng = np.random.default_rng(21)
+    H, Hkv, bits, page, G, R = 32, 8, 4, 64, 4, pu.rotation(6).cuda()
+    lens, new = [900, 64, 2500, 31], [40, 5, 600, 1]
+    start = [0] + np.cumsum(new).tolist()
+    small = 80
+    far = (9 << 20) // page  # pages: 9 Mi rows of 512 bytes
+    table, used = pu.tables(rng, lens, page)
+    assert used <= small
+    tables = [table, torch.where(table >= 0, table + (far - small), table)]
+    pools = [[torch.empty(n * page, w, dtype=t, device="cuda") for w, t in ((Hkv * 64, torch.uint8), (Hkv, torch.float16)) * 2] for n in (small, far)]
+    k, v = (torch.from_numpy(rng.standard_normal((sum(lens), Hkv * 128)).astype(np.float16)).cuda() for _ in range(2))
+    q = torch.from_numpy(rng.standard_normal((start[-1], H * 128)).astype(np.float16)).cuda()
+    ws, results = ops.paged_workspace(start[-1], G, H), []
+    for t, (ck, kn, cv, vn) in zip(tables, pools):
+        slots = torch.cat([pu.rows_of(t[g], n, page) for g, n in enumerate(lens)])
+        cut = 200  # (a first part by the form for few tokens)
+        for a, b in ((0, cut), (cut, sum(lens))):
+            ops.paged_append(ck, kn, cv, vn, k[a:b], v[a:b], R, slots[a:b], Hkv, bits)
+        k_out, v_out, out, one, wide = torch.empty_like(k), torch.empty_like(v), torch.empty_like(q), torch.empty_like(q[:G]), torch.empty_like(q[:G])
+        ops.paged_read(k_out, v_out, ck, kn, cv, vn, R, slots, Hkv, bits)
+        ops.paged_prefill_attention(out, q, ck, cv, kn, vn, R, t, i32(lens), i32(start), page, H, Hkv, bits, ws)
+        long = torch.empty(1, H * 128, dtype=torch.float16, device="cuda")
+        lone = torch.empty_like(q[:20])
+        ops.paged_prefill_attention(lone, q[:20], ck, cv, kn, vn, R, t[2:3], i32(lens[2:3]), i32([0, 20]), page, H, Hkv, bits, ws)  # cut along the context
+        ops.paged_decode_attention(one, q[:G], ck, cv, kn, vn, R, t, i32(lens), page, H, Hkv, bits, ws)
+        ops.paged_decode_attention(long, q[:1], ck, cv, kn, vn, R, t[2:3, :1], i32(lens[2:3]), page, H, Hkv, bits, ws)
+        more = torch.cat([t, torch.full((G, 400), -1, dtype=torch.int32, device="cuda")], 1)  # (a bound for which the streaming form is taken)
+        ops.paged_decode_attention(wide, q[:G], ck, cv, kn, vn, R, more, i32(lens), page, H, Hkv, bits, ws)
+        torch.cuda.synchronize()
+        results.append([k_out, v_out, out, lone, one, long, wide, *(x[slots].view(torch.uint8) for x in (ck, kn, cv, vn))])
+    for i, (a, b) in enumerate(zip(*results)):
+        assert torch.equal(a, b), i
+    ck, kn, cv, vn = pools[1]
+    for got, at, st in ((results[1][2], lens, start), (results[1][4], lens, list(range(G + 1))), (results[1][6], lens, list(range(G + 1)))):
+        pu.assert_attention(got, pu.attention(q[:st[-1]], ck, cv, kn, vn, R, tables[1], at, st, page, H, Hkv, bits))
+
+
+@pytest.mark.parametrize("T, G", [(340, 34), (40, 40), (330, 2)])
+def test_rows_far_apart(T, G):
+    # strides that put the last rows more than 2^32 bytes behind the first
+    rng = np.random.default_rng(T)
+    H, Hkv, bits, page, R = 16, 8, 4, 64, pu.rotation(7).cuda()
+    new = [T // G] * G
+    lens, start = [n + 50 + 7 * g for g, n in enumerate(new)], [T // G * g for g in range(G + 1)]
+    stride = ((5 << 29) // T + 4096) // 8 * 8  # halves: 5 GB of them
+    whole = torch.empty(T * stride, dtype=torch.float16, device="cuda")
+    column = lambda at, heads: whole.as_strided((T, heads * 128), (stride, 1), at)  # noqa: E731
+    table, q, _, ck, cv, kn, vn, _, _ = attention_inputs(rng, lens, H, Hkv, bits, page, T=T)
+    kv = torch.from_numpy(rng.standard_normal((T, 2 * Hkv * 128)).astype(np.float16)).cuda()
+    far_q, far_k, far_v = column(0, H), column(2048, Hkv), column(2048 + Hkv * 128 + 8, Hkv)
+    slots = torch.cat([pu.rows_of(table[g], n, page)[n - new[g]:] for g, n in enumerate(lens)])
+    ws = ops.paged_workspace(T, G, H)
+    k, v = kv[:, :Hkv * 128], kv[:, Hkv * 128:]
+    caches = [[x.clone() for x in (ck, kn, cv, vn)] for _ in range(2)]
+    far_k.copy_(k)
+    far_v.copy_(v)
+    for (c, n, d, m), a, b in zip(caches, (k, far_k), (v, far_v)):
+        ops.paged_append(c, n, d, m, a, b, R, slots, Hkv, bits)
+    for x, y in zip(*caches):
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+    c, n, d, m = caches[0]
+    near_k, near_v = torch.empty_like(k), torch.empty_like(v)
+    ops.paged_read(near_k, near_v, c, n, d, m, R, slots, Hkv, bits)
+    ops.paged_read(far_k, far_v, c, n, d, m, R, slots, Hkv, bits)
+    assert torch.equal(near_k, far_k) and torch.equal(near_v, far_v)
+    far_q.copy_(q)
+    near = torch.empty(T, H * 128, dtype=torch.float16, device="cuda")
+    calls = [lambda o, a: ops.paged_prefill_attention(o, a, c, d, n, m, R, table, i32(lens), i32(start), page, H, Hkv, bits, ws)]
+    if T == G:
+        calls.append(lambda o, a: ops.paged_decode_attention(o, a, c, d, n, m, R, table, i32(lens), page, H, Hkv, bits, ws))
+    for call in calls:
+        call(near, q)
+        mid = torch.empty(T, H * 128, dtype=torch.float16, device="cuda")
+        call(mid, far_q)                 # queries far apart
+        far_res = column(2048, H)        # (where K and V were)
+        far_res.fill_(7.0)
+        call(far_res, far_q)             # both: columns of one array
+        torch.cuda.synchronize()
+        assert torch.equal(mid, near) and torch.equal(far_res, near)
+
+
+# ---- whole steps, two at a time, and captured ---------------------------------------------------------------------------------------
+class Loop:
+    """A pool, its requests, and three kinds of step: prompts, single tokens beside a chunk, a decode step."""
+
+    def __init__(self, seed, H=32, Hkv=8, bits=4, page=32, G=6, width=80):
+        rng = np.random.default_rng(seed)
+        self.a, self.page, self.G, self.T = (H, Hkv, bits), page, G, 2600
+        pool = G * width // 2
+        self.R, self.table = pu.rotation(seed).cuda(), i32(np.full((G, width), -1))
+        self.stack, self.count, self.lens = i32(rng.permutation(pool)), i32([pool]), i32(np.zeros(G))
+        self.cache = [torch.zeros(pool * page, w, dtype=t, device="cuda") for w, t in ((Hkv * 16 * bits, torch.uint8), (Hkv, torch.float16)) * 2]
+        self.start, self.slots, self.pos = i32(np.zeros(G + 1)), torch.zeros(self.T, dtype=torch.int64, device="cuda"), i32(np.zeros(self.T))
+        self.ws = ops.paged_workspace(self.T, G, H)
+        self.steps = [rng.integers(100, 400, G), np.where(np.arange(G) == 2, 150, 1), np.ones(G, int), np.where(np.arange(G) == 4, 0, 1)]
+        self.ended = [None, None, np.arange(G) % 3 == 0, None]
+        self.steps[2] = np.where(np.arange(G) % 3 == 0, 37, 1)
+        self.steps = [i32(s) for s in self.steps]
+        self.ended = [None if e is None else torch.from_numpy(e).cuda() for e in self.ended]
+        self.qkv = [torch.from_numpy(rng.standard_normal((self.T, (H + 2 * Hkv) * 128)).astype(np.float16)).cuda() for _ in range(4)]
+        self.out = [torch.zeros(self.T, H * 128, dtype=torch.float16, device="cuda") for _ in range(5)]
+
+    def run(self):
+        (H, Hkv, bits), (ck, kn, cv, vn) = self.a, self.cache
+        for i in range(4):
+            q, k, v = self.qkv[i][:, :H * 128], self.qkv[i][:, H * 128:(H + Hkv) * 128], self.qkv[i][:, (H + Hkv) * 128:]
+            ops.page_plan(self.table, self.stack, self.count, self.count, self.lens, self.steps[i], self.ended[i], self.page, self.lens, self.start, self.slots, self.pos)
+            ops.paged_append(ck, kn, cv, vn, k, v, self.R, self.slots, Hkv, bits)
+            ops.paged_prefill_attention(self.out[i], q, ck, cv, kn, vn, self.R, self.table, self.lens, self.start, self.page, H, Hkv, bits, self.ws)
+        ops.paged_decode_attention(self.out[4][:self.G], self.qkv[3][:self.G, :H * 128], ck, cv, kn, vn, self.R, self.table, self.lens, self.page, H, Hkv, bits, self.ws)
+
+    def state(self):
+        return [self.table, self.stack, self.count, self.lens, self.start, self.slots, self.pos, *(x.view(torch.uint8) for x in self.cache), *self.out]
+
+
+def test_steps_on_two_streams_and_from_one_graph():
+    want = []
+    for seed in (1, 2):
+        loop = Loop(seed)
+        loop.run()
+        torch.cuda.synchronize()
+        assert loop.lens.min() > 0 and int(loop.count) >= 0
+        want.append([x.clone() for x in loop.state()])
+    for _ in range(4):
+        loops, streams = [Loop(1), Loop(2)], [torch.cuda.Stream() for _ in range(2)]
+        torch.cuda.synchronize()
+        for loop, s in zip(loops, streams):
+            with torch.cuda.stream(s):
+                loop.run()
+        torch.cuda.synchronize()
+        for loop, w in zip(loops, want):
+            assert all(torch.equal(a, b) for a, b in zip(loop.state(), w))
+    loop, graph = Loop(1), torch.cuda.CUDAGraph()
+    keep = [x.clone() for x in loop.state()]
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        loop.run()
+    for _ in range(3):
+        for a, b in zip(loop.state(), keep):
+            a.copy_(b)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(loop.state(), want[0]))
